@@ -1,0 +1,426 @@
+"""The paged cache and packed prompts on the GPU against plain forms in 64 bits."""
+import random
+
+import pytest
+import torch
+
+import paged_plain as plain
+
+pytestmark = pytest.mark.gpu
+
+HEADS = [(1, 1, 16, 16), (12, 4, 64, 64), (8, 2, 128, 128), (4, 1, 256, 256), (28, 4, 128, 128), (6, 2, 80, 48), (5, 5, 72, 104), (24, 8, 192, 128),
+         (40, 1, 96, 33), (3, 1, 8, 200)]
+
+
+def randn(seed, dtype, *shape):
+    return torch.randn(*shape, generator=torch.Generator("cuda").manual_seed(seed), device="cuda").to(dtype)
+
+
+def i32(v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+# ---- the plan
+def book_of(table, book, pages):
+    first, count = table.span.tolist()
+    free = table.free.tolist()
+    assert [free[(first + j) % pages] for j in range(count)] == book.free
+    assert table.lens.tolist() == book.lens
+    for row, held in zip(table.tables.tolist(), book.tables):
+        assert row[:len(held)] == held
+
+
+@pytest.mark.parametrize("requests,pages,page,most,chunk", [
+    (1, 8, 16, 8, 40), (7, 60, 16, 12, 70), (300, 2500, 32, 20, 200), (1500, 9000, 64, 6, 150), (8192, 30000, 16, 5, 30), (3, 9, 1024, 3, 1500)])
+@pytest.mark.parametrize("in_place", [True, False])
+def test_plan_over_many_steps(zq, requests, pages, page, most, chunk, in_place):
+    rng = random.Random(requests)
+    table, book = zq.PageTable(pages, page, requests, most), plain.Pages(pages, page, requests, most)
+    refused = 0
+    for step in range(12):
+        new = [rng.choice((-1, 0, 1, 1, 1, rng.randint(0, chunk))) for _ in range(requests)]
+        new = [min(n, page * most - l) for n, l in zip(new, book.lens)]
+        rows = sum(max(n, 0) for n in new) + rng.choice((0, 0, 5))
+        if step % 5 == 4:
+            rows = max(0, rows - 6)
+        want = book.step(new, rows)
+        if in_place:
+            got = table.plan(i32(new), rows)
+        else:
+            got = zq.page_plan(i32(new), table.lens, table.tables, table.free, table.span, page, rows)
+            table.lens, table.span = got.lens, got.span
+        status = int(got.status)
+        if want is None:
+            refused += 1
+            want = [0] * (requests + 1), [0] * rows, [-1] * rows
+            assert status in (1, 4, 5)
+            with pytest.raises(RuntimeError):
+                got.check()
+        else:
+            assert status == 0
+        assert got.row_start.tolist() == want[0] and got.pos.tolist() == want[1] and got.places.tolist() == want[2]
+        book_of(table, book, pages)
+    assert refused < 12
+
+
+def test_plan_is_refused_as_a_whole(zq):
+    """Each cause alone; lengths, tables and ring stay as they were."""
+    def status(new, rows, lens=(20, 3), span=(1, 4), width=3):
+        lens, span, free = i32(list(lens)), i32(list(span)), i32([5, 4, 3, 2, 1, 0])
+        tables = torch.full((2, width), -1, dtype=torch.int32, device="cuda")
+        before = [t.clone() for t in (lens, span, free, tables)]
+        p = zq.page_plan(i32(new), lens, tables, free, span, 16, rows, in_place=True)
+        code = int(p.status)
+        if code:
+            assert all(torch.equal(a, b) for a, b in zip((lens, span, free, tables), before))
+            assert p.row_start.tolist() == [0, 0, 0] and p.places.tolist() == [-1] * rows and p.pos.tolist() == [0] * rows
+        return code
+    assert status([28, 45], 80) == 0
+    assert status([28, 45], 72) == zq.PLAN_ROWS
+    assert status([29, 0], 80) == zq.PLAN_TABLE
+    assert status([2 ** 31 - 1, 2 ** 31 - 1], 80) & zq.PLAN_TABLE
+    assert status([28, 45], 80, span=(1, 2)) == zq.PLAN_PAGES
+    assert status([1, 1], 80, lens=(-1, 3)) == zq.PLAN_INCONSISTENT
+    assert status([1, 1], 80, lens=(49, 3)) == zq.PLAN_INCONSISTENT
+    for span in ((-1, 2), (6, 2), (0, -1), (0, 7)):
+        assert status([1, 1], 80, span=span) & zq.PLAN_INCONSISTENT
+    assert status([-1, 1], 80, span=(0, 5)) == zq.PLAN_INCONSISTENT  # two pages given back beside five free ones of six
+    assert status([-5, 1], 80, span=(0, 4)) == 0
+
+
+def test_plan_without_rows(zq):
+    table = zq.PageTable(4, 16, 2, 2)
+    p = table.plan(i32([0, 0]), 0).check()
+    assert p.row_start.tolist() == [0, 0, 0] and p.places.numel() == 0
+
+
+# ---- the write
+@pytest.mark.parametrize("heads,kv_heads,dim,vdim", HEADS)
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("mix", ["none", "store", "mix"])
+def test_write(zq, heads, kv_heads, dim, vdim, f32, mix):
+    rows, pages, P = 23, 5, 16
+    cache = zq.PagedCache(heads, kv_heads, dim, vdim, pages, P, 0.1, temp_coef=0.2, temp_every=7.0, f32=f32)
+    cache.k.fill_(3.0)
+    cache.v.fill_(3.0)
+    x = randn(1, torch.float32, rows, (heads + kv_heads) * dim + kv_heads * vdim)
+    q_norm, k_norm = 1 + randn(2, torch.float32, dim) * 0.1, 1 + randn(3, torch.float32, dim) * 0.1
+    vmix = randn(4, torch.float32, 1) if mix == "mix" else None
+    first = randn(5, torch.float32, rows, kv_heads * vdim) if mix != "none" else None
+    kept = first.clone() if mix == "mix" else None
+    places = random.Random(1).sample(range(pages * P), rows)
+    places[3], places[7], places[11] = -1, pages * P, 2 ** 31 - 1
+    pos = i32([5 * r for r in range(rows)])
+    q = cache.write(x, q_norm, k_norm, pos, i32(places), vmix, first)
+    wq, wk, wv = plain.write(x, heads, kv_heads, dim, vdim, q_norm, k_norm, pos, vmix, kept, 0.2, 7.0)
+    # a norm is a sum of dim squares, a root, three products; the temperature a logarithm; a mix two products and a sum of terms
+    # that may cancel: relative to their sizes
+    unit = plain.U32 * (dim / 2 + 16) + (0 if f32 else plain.U16)
+    assert ((q[..., :dim].double() - wq).abs() <= unit * wq.abs() + 1e-30).all() and (q[..., dim:] == 0).all()
+    k, v = cache.k.view(-1, kv_heads, cache.k.shape[3]), cache.v.view(-1, kv_heads, cache.v.shape[3])
+    size = wv.abs() if mix != "mix" else (1 + vmix.abs().double()) * (x[:, (heads + kv_heads) * dim:].double().abs().view(wv.shape) + kept.double().abs().view(wv.shape))
+    written = set()
+    for r, at in enumerate(places):
+        if 0 <= at < pages * P:
+            written.add(at)
+            assert ((k[at, :, :dim].double() - wk[r]).abs() <= unit * wk[r].abs() + 1e-30).all() and (k[at, :, dim:] == 0).all()
+            assert ((v[at, :, :vdim].double() - wv[r]).abs() <= 4 * plain.U32 * size[r] + (0 if f32 else plain.U16) * wv[r].abs()).all()
+            assert (v[at, :, vdim:] == 0).all()
+    rest = [t for t in range(pages * P) if t not in written]
+    assert (k[rest] == 3).all() and (v[rest] == 3).all()
+    if mix == "store":
+        assert torch.equal(first, x[:, (heads + kv_heads) * dim:])
+    if mix == "mix":
+        assert torch.equal(first, kept)
+
+
+# ---- attention over pages
+def paged_case(zq, heads, kv_heads, dim, vdim, f32, page, held, new, seed=0, pad=0, spread=1.0, scale=None, spoil=True):
+    """A cache with pages in a shuffled order, what is behind a request's last token spoilt, and its rows."""
+    dtype, lens = torch.float32 if f32 else torch.bfloat16, [h + n for h, n in zip(held, new)]
+    count = [-(-l // page) for l in lens]
+    pages, width = sum(count) + 2, max(count + [1]) + 1
+    cache = zq.PagedCache(heads, kv_heads, dim, vdim, pages, page, dim ** -0.5 if scale is None else scale, f32=f32)
+    if spoil:
+        cache.k[..., :dim] = float("nan")
+        cache.v[..., :vdim] = float("inf")
+    order = random.Random(seed).sample(range(pages), sum(count))
+    tables, row_start, keys, values = torch.full((len(held), width), -1, dtype=torch.int32), [0], [], []
+    for i, l in enumerate(lens):
+        mine, order = order[:count[i]], order[count[i]:]
+        tables[i, :count[i]] = torch.tensor(mine, dtype=torch.int32)
+        keys.append(randn(seed * 1000 + i, dtype, l, kv_heads, dim) * spread)
+        values.append(randn(seed * 1000 + 500 + i, dtype, l, kv_heads, vdim))
+        for j, at in enumerate(mine):
+            part = slice(j * page, min((j + 1) * page, l))
+            n = part.stop - part.start
+            cache.k[at, :n, :, :dim], cache.v[at, :n, :, :vdim] = keys[i][part], values[i][part]
+        row_start.append(row_start[-1] + new[i])
+    rows = row_start[-1] + pad
+    q = torch.zeros(rows, heads, cache.k.shape[3], dtype=dtype, device="cuda")
+    q[..., :dim] = randn(seed + 77, dtype, rows, heads, dim) * spread
+    return cache, q, i32(row_start), i32(lens), tables.cuda(), keys, values
+
+
+def check_paged(zq, heads, kv_heads, dim, vdim, f32, page, held, new, seed=0, pad=3, **more):
+    cache, q, row_start, lens, tables, keys, values = paged_case(zq, heads, kv_heads, dim, vdim, f32, page, held, new, seed, pad, **more)
+    out = torch.full((q.shape[0], zq.dense_pitch(heads * vdim)), 7.0, dtype=q.dtype, device="cuda")
+    got = cache.attend(q, row_start, lens, tables, out=out)
+    assert got is out
+    for i, (k, v) in enumerate(zip(keys, values)):
+        a, b = row_start[i].item(), row_start[i + 1].item()
+        see = lens[i].item() - new[i] + 1 + torch.arange(new[i], device="cuda")
+        want, tol = plain.attention(q[a:b, :, :dim], k, v, see, cache.g.scale, not f32)
+        off = (got[a:b, :heads * vdim].view(-1, heads, vdim).double() - want).abs()
+        assert (off <= tol).all(), (i, held[i], new[i], (off / tol).max().item())
+    assert (got[:row_start[-1], heads * vdim:] == 0).all()
+    assert (got[row_start[-1]:] == 7).all()
+    assert torch.equal(cache.attend(q, row_start, lens, tables, out=torch.full_like(out, 7.0)), got)  # the same bits every time
+    return got
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,vdim", HEADS)
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("page", [16, 128])
+def test_single_tokens(zq, heads, kv_heads, dim, vdim, f32, page):
+    held = [0, 15, 16, 17, 63, 64, 200, 1000, 0, 333]
+    check_paged(zq, heads, kv_heads, dim, vdim, f32, page, held, [1, 1, 1, 1, 1, 1, 1, 1, 0, 1])
+    check_paged(zq, heads, kv_heads, dim, vdim, f32, page, [700], [1], seed=1, pad=0)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,vdim", HEADS)
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("page", [16, 64, 256])
+def test_chunks(zq, heads, kv_heads, dim, vdim, f32, page):
+    check_paged(zq, heads, kv_heads, dim, vdim, f32, page, [0, 100, 0, 5, 513, 40], [130, 67, 1, 0, 128, 33])
+    check_paged(zq, heads, kv_heads, dim, vdim, f32, page, [257], [300], seed=2, pad=0)
+
+
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("new", [2, 3, 5])
+def test_a_few_tokens_of_each(zq, f32, new):
+    check_paged(zq, 8, 2, 128, 128, f32, 32, [9, 100, 400, 0, 31], [new] * 5)
+    check_paged(zq, 4, 1, 256, 256, f32, 16, [9, 100, 400, 0, 31], [new, 0, new, 1, new], seed=3)
+
+
+@pytest.mark.parametrize("f32", [False, True])
+def test_a_long_cache_beside_short_ones(zq, f32):
+    check_paged(zq, 8, 2, 64, 64, f32, 64, [9000, 3, 70, 2500], [1, 1, 1, 1])
+    check_paged(zq, 8, 2, 128, 128, f32, 64, [9000, 3, 70, 2500], [150, 1, 200, 1], seed=1)
+
+
+@pytest.mark.parametrize("scale", [-0.3, 0.0])
+@pytest.mark.parametrize("new", [1, 90])
+def test_scales_that_are_not_positive(zq, scale, new):
+    check_paged(zq, 6, 2, 64, 64, False, 16, [30, 200], [new, new], scale=scale)
+    check_paged(zq, 6, 2, 64, 64, True, 16, [30, 200], [new, new], scale=scale)
+
+
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("new", [1, 140])
+def test_scores_far_apart(zq, f32, new):
+    """Scores of hundreds: maxima that grow from tile to tile, weights that vanish."""
+    check_paged(zq, 8, 2, 128, 128, f32, 16, [600, 30], [new, new], spread=6.0)
+
+
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("new", [1, 70])
+def test_entries_that_are_no_page_stand_for_zeros(zq, f32, new):
+    heads, kv_heads, dim, vdim, page = 8, 2, 64, 64, 16
+    cache, q, row_start, lens, tables, keys, values = paged_case(zq, heads, kv_heads, dim, vdim, f32, page, [150, 40], [new, new])
+    for at, entry in ((1, -1), (4, cache.k.shape[0]), (6, -2 ** 31), (8, 2 ** 31 - 1)):
+        tables[0, at] = entry
+        keys[0][at * page:(at + 1) * page], values[0][at * page:(at + 1) * page] = 0, 0
+    got = cache.attend(q, row_start, lens, tables)
+    for i in range(2):
+        a, b = i * new, (i + 1) * new
+        want, tol = plain.attention(q[a:b, :, :dim], keys[i], values[i], lens[i] - new + 1 + torch.arange(new, device="cuda"), cache.g.scale, not f32)
+        assert ((got[a:b].view(-1, heads, vdim).double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("new", [1, 40])
+def test_rows_that_see_nothing_are_zero(zq, f32, new):
+    """A request that holds fewer tokens than it has rows: its first rows lie before its first token."""
+    cache, q, row_start, lens, tables, keys, values = paged_case(zq, 4, 2, 64, 64, f32, 16, [60, 20], [new, new])
+    short = i32([new // 2, -3])
+    got = cache.attend(q, row_start, short, tables)
+    hidden = new - new // 2
+    assert (got[:hidden] == 0).all() and (got[new:] == 0).all()
+    if new > 1:
+        want, tol = plain.attention(q[hidden:new, :, :64], keys[0][:new // 2], values[0][:new // 2], 1 + torch.arange(new // 2, device="cuda"), cache.g.scale, not f32)
+        assert ((got[hidden:new].view(-1, 4, 64).double() - want).abs() <= tol).all()
+
+
+def test_numbers_beyond_the_tables_are_cut_off(zq):
+    """Lengths beyond the table and row numbers beyond the rows reach no memory that is not the call's."""
+    cache, q, row_start, lens, tables, keys, values = paged_case(zq, 4, 2, 64, 64, False, 16, [60, 20], [1, 1])
+    got = cache.attend(q, i32([0, 1, 2 ** 31 - 1]), i32([61, 2 ** 31 - 1]), tables)
+    assert got.shape[0] == 2 and torch.isfinite(got[0].float()).all()
+    got = cache.attend(q, i32([-5, 1, -9]), lens, tables, out=torch.full((2, 256), 7.0, dtype=torch.bfloat16, device="cuda"))
+    assert (got[1] == 7).all()
+
+
+# ---- packed prompts
+def check_packed(zq, heads, kv_heads, dim, vdim, f32, lens, pad=0, offset=0, wide=0, spoil=None, scale=None):
+    dtype, up = torch.float32 if f32 else torch.bfloat16, lambda n: (n + 15) // 16 * 16
+    dp, vp, rows = up(dim), up(vdim), sum(lens) + pad
+    x = torch.zeros(rows, offset + (heads + kv_heads) * dp + kv_heads * vp + wide, dtype=dtype, device="cuda")
+    at = [offset, offset + heads * dp, offset + (heads + kv_heads) * dp, x.shape[1] - wide]
+    q, k, v = (x[:, a:b].unflatten(1, (n, d)) for a, b, n, d in zip(at, at[1:], (heads, kv_heads, kv_heads), (dp, dp, vp)))
+    for i, (t, d) in enumerate(((q, dim), (k, dim), (v, vdim))):
+        t[..., :d] = randn(i, dtype, rows, t.shape[1], d)
+    row_start = [0]
+    for l in lens:
+        row_start.append(row_start[-1] + l)
+    if spoil is not None:
+        a, b = row_start[spoil], row_start[spoil + 1]
+        k[a:b, :, :dim], v[a:b, :, :vdim] = float("nan"), float("inf")
+    k[row_start[-1]:], v[row_start[-1]:] = float("nan"), float("nan")
+    out = torch.full((rows, zq.dense_pitch(heads * vdim)), 7.0, dtype=dtype, device="cuda")
+    scale = dim ** -0.5 if scale is None else scale
+    got = zq.packed_attention(q, k, v, i32(row_start), scale, vdim=vdim, out=out)
+    for i, (a, b) in enumerate(zip(row_start, row_start[1:])):
+        if i == spoil or a == b:
+            continue
+        want, tol = plain.attention(q[a:b, :, :dim], k[a:b, :, :dim], v[a:b, :, :vdim], 1 + torch.arange(b - a, device="cuda"), scale, not f32)
+        off = (got[a:b, :heads * vdim].view(-1, heads, vdim).double() - want).abs()
+        assert (off <= tol).all(), (i, lens[i], (off / tol).max().item())
+        assert (got[a:b, heads * vdim:] == 0).all()
+    assert (got[row_start[-1]:] == 7).all()
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,vdim", HEADS)
+@pytest.mark.parametrize("f32", [False, True])
+def test_packed(zq, heads, kv_heads, dim, vdim, f32):
+    check_packed(zq, heads, kv_heads, dim, vdim, f32, [1, 0, 130, 64, 300, 0, 17], pad=5)
+    check_packed(zq, heads, kv_heads, dim, vdim, f32, [257], offset=16, wide=48)
+    check_packed(zq, heads, kv_heads, dim, vdim, f32, [3, 1, 2, 1, 4], pad=1)
+
+
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("spoil", [0, 1, 2])
+def test_a_sequence_does_not_reach_its_neighbours(zq, f32, spoil):
+    check_packed(zq, 8, 2, 64, 64, f32, [90, 77, 140], pad=30, spoil=spoil)
+    check_packed(zq, 8, 2, 128, 128, f32, [2, 3, 1], pad=4, spoil=spoil)
+
+
+def test_packed_long(zq):
+    check_packed(zq, 4, 1, 128, 128, False, [3001, 1100, 700])
+    check_packed(zq, 2, 1, 256, 256, False, [2200])
+
+
+# ---- together
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 2, 128), (4, 1, 256), (6, 3, 40)])
+def test_steps_of_several_requests(zq, f32, heads, kv_heads, dim):
+    """Prompts in chunks of any size, single tokens, requests that end and pages that are used again: every row as over its own
+    sequence alone."""
+    n, P, pages = 5, 16, 40
+    table, book = zq.PageTable(pages, P, n, 12), plain.Pages(pages, P, n, 12)
+    cache = zq.PagedCache(heads, kv_heads, dim, dim, pages, P, dim ** -0.5, f32=f32)
+    ones, rng, width = torch.ones(dim, device="cuda"), random.Random(4), (heads + 2 * kv_heads) * dim
+    said = [torch.zeros(0, width, device="cuda") for _ in range(n)]
+    for step in range(14):
+        new = [-1 if l > 90 else rng.choice((0, 1, 1, 20, 50)) for l in book.lens]
+        rows = sum(max(x, 0) for x in new)
+        want = book.step(new, rows)
+        p = table.plan(i32(new), rows + 3).check()
+        assert want and p.places.tolist() == want[2] + [-1] * 3
+        x = randn(100 + step, torch.float32, rows + 3, width)
+        q = cache.write(x, ones, ones, p.pos, p.places)
+        got = cache.attend(q, p.row_start, p.lens, table.tables)
+        for i in range(n):
+            a, b = want[0][i], want[0][i + 1]
+            said[i] = said[i][:0] if new[i] < 0 else torch.cat([said[i], x[a:b]])
+            if a == b:
+                continue
+            _, k, v = plain.write(said[i], heads, kv_heads, dim, dim, ones, ones, i32([0] * len(said[i])), None, None, 0, 0)
+            see = len(said[i]) - (b - a) + 1 + torch.arange(b - a, device="cuda")
+            o, tol = plain.attention(q[a:b, :, :dim], k.to(q.dtype), v.to(q.dtype), see, dim ** -0.5, not f32)
+            if f32:
+                tol = tol + 1e-5 * o.abs().max()  # the keys were normed in 32 bits: dim / 2 + 16 of half a step, times scores of up to 12, twice
+            else:  # keys whose norm falls on the other side of a rounding: a step of bf16 in some products of a score
+                tol = tol + 2 * plain.U16 * o.abs().max()
+            assert ((got[a:b, :heads * dim].view(-1, heads, dim).double() - o).abs() <= tol).all()
+    book_of(table, book, pages)
+
+
+def test_a_recorded_step_replays(zq):
+    """Plan, write and attention in a graph: what changes from step to step is read on the device, two graphs with their own buffers
+    take turns."""
+    n, P, pages, heads, kv_heads, dim, rows = 3, 16, 30, 8, 2, 128, 3
+    ones = torch.ones(dim, device="cuda")
+
+    def program():
+        table = zq.PageTable(pages, P, n, 10)
+        return table, zq.PagedCache(heads, kv_heads, dim, dim, pages, P, dim ** -0.5)
+
+    def step(table, cache, new, x):
+        p = table.plan(new, rows)
+        return cache.attend(cache.write(x, ones, ones, p.pos, p.places), p.row_start, p.lens, table.tables)
+
+    width = (heads + 2 * kv_heads) * dim
+    recorded = []
+    for _ in range(2):
+        table, cache = program()
+        new, x = i32([0, 0, 0]), torch.zeros(rows, width, device="cuda")
+        step(table, cache, new, x)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step(table, cache, new, x)
+        recorded.append((graph, table, new, x, out, cache))  # the graph reads and writes the cache
+    table, cache = program()
+    for t in range(40):
+        new, x = i32([1, 1 if t % 3 else 0, 1 if t > 20 else 0]), randn(t, torch.float32, rows, width)
+        want = step(table, cache, new, x)
+        real = int(new.sum())
+        for graph, _, new_in, x_in, out, _ in recorded:
+            new_in.copy_(new)
+            x_in.copy_(x)
+            graph.replay()
+            assert torch.equal(out[:real], want[:real]), t
+    assert table.lens.tolist() == recorded[0][1].lens.tolist() == recorded[1][1].lens.tolist()
+
+
+def test_calls_on_two_streams_at_once(zq):
+    cases = [paged_case(zq, 8, 2, 128, 128, False, 16, [2000 + i, 30], [1 + 90 * i, 1], seed=i) for i in range(2)]
+    want = [c[0].attend(*c[1:5]) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        got = []
+        for s, c in zip(streams, cases):
+            with torch.cuda.stream(s):
+                got.append(c[0].attend(*c[1:5]))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# ---- refusals
+def test_refusals(zq):
+    from zignn_b200 import _lib
+    cache, q, row_start, lens, tables, *_ = paged_case(zq, 4, 2, 64, 64, False, 16, [60, 20], [1, 1])
+
+    def refused(call, status=None):
+        with pytest.raises(_lib.ZqError if status else ValueError) as e:
+            call()
+        assert status is None or e.value.status == status
+    refused(lambda: cache.attend(q.float(), row_start, lens, tables))
+    refused(lambda: cache.attend(q[:, :2], row_start, lens, tables))
+    refused(lambda: cache.attend(q, row_start[:2], lens, tables))
+    refused(lambda: cache.attend(q, row_start, lens.long(), tables))
+    refused(lambda: cache.attend(q, row_start, lens, tables.cpu()))
+    refused(lambda: cache.attend(q, row_start, lens, tables, out=q))
+    refused(lambda: zq.packed_attention(q, q[:, :2], q[:, :2, :40], row_start, 0.1))
+    refused(lambda: zq.packed_attention(q, q[:, :2].float(), q[:, :2], row_start, 0.1))
+    refused(lambda: zq.packed_attention(q.transpose(1, 2), q, q, row_start, 0.1))
+    refused(lambda: zq.packed_attention(q, q[:, :2], q[:, :2], row_start, 0.1, vdim=40))
+    refused(lambda: zq.packed_attention(q, q[:, :3], q[:, :3], row_start, 0.1), 1)
+    refused(lambda: zq.page_plan(row_start, lens, tables, lens, lens, 16, 2))
+    refused(lambda: zq.PageTable(8, 24, 2, 2).plan(lens, 2), 2)
+    refused(lambda: zq.PageTable(1 << 17, 1 << 10, 1, 1 << 22).plan(lens[:1], 2), 5)
+    refused(lambda: zq.PageTable(8, 16, 8193, 2).plan(torch.zeros(8193, dtype=torch.int32, device="cuda"), 2), 5)
+    refused(lambda: zq.PagedCache(2, 1, 520, 64, 2, 16, 0.1).attend(torch.zeros(1, 2, 528, dtype=torch.bfloat16, device="cuda"), i32([0, 1]), i32([1]), i32([[0]])), 5)
+    refused(lambda: cache.write(torch.zeros(2, 100, device="cuda"), lens, lens, lens, lens))

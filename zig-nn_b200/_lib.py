@@ -102,6 +102,12 @@ SIGNATURES = {
     "zq_gqa_cache_write": (i, [P(S.Gqa), vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, u32, i, vp]),
     "zq_gqa_work_bytes": (sz, [P(S.Gqa), u32]),
     "zq_gqa_attention": (i, [P(S.Gqa), vp, vp, vp, vp, vp, vp, u32, i, u32, vp, i, vp]),
+    "zq_page_plan": (i, [P(S.Pages), vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, u32, vp, vp]),
+    "zq_paged_cache_write": (i, [P(S.Gqa), P(S.Pages), vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, u32, i, vp]),
+    "zq_paged_attention": (i, [P(S.Gqa), P(S.Pages), vp, vp, vp, vp, vp, vp, vp, u32, vp, sz, i, vp]),
+    "zq_paged_work_bytes": (sz, [P(S.Gqa), P(S.Pages), u32, i]),
+    "zq_packed_attention": (i, [P(S.Gqa), vp, sz, vp, sz, vp, sz, vp, vp, u32, u32, vp, sz, i, vp]),
+    "zq_packed_work_bytes": (sz, [P(S.Gqa), u32, u32, i]),
     "zq_token_shift": (i, [vp, vp, vp, vp, u32, u32, u32, vp, i, vp]),
     "zq_wkv": (i, [vp, u32, u32, u32, vp, vp, vp, vp, f, vp, vp, u32, i, vp, vp, i, vp]),
     "zq_wkv_work_floats": (sz, [u32, u32, u32]),

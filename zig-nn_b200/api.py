@@ -579,6 +579,170 @@ class GqaCache:
         return out
 
 
+# ---- a cache of pages that requests share, packed prompts (include/zq.h: zq_page_plan, zq_paged_*, zq_packed_attention)
+PLAN_PAGES, PLAN_TABLE, PLAN_ROWS, PLAN_INCONSISTENT = 1, 2, 4, 8
+
+
+def _int_rows(t, name, *shape):
+    """t, a contiguous int32 tensor of that shape (-1: any) on the current device."""
+    if not (isinstance(t, torch.Tensor) and t.dtype == torch.int32 and t.is_cuda and t.is_contiguous() and t.dim() == len(shape)
+            and all(n in (-1, m) for n, m in zip(shape, t.shape))):
+        raise ValueError("%s: expected a contiguous int32 CUDA tensor of shape %s" % (name, list(shape)))
+    return _here(t, name)
+
+
+def _here(t, name):
+    if t.get_device() != torch._C._cuda_getDevice():
+        raise ValueError("%s is on device %d, the current one is %d" % (name, t.get_device(), torch._C._cuda_getDevice()))
+    return t
+
+
+class PagePlan:
+    """The rows of a step: row_start [requests + 1], pos and places [rows]; lens [requests] and span [2] afterwards; status [1]."""
+
+    __slots__ = ("lens", "span", "row_start", "pos", "places", "status")
+
+    def check(self):
+        """Raises when the step could not be planned (synchronises)."""
+        status = int(self.status)
+        if status:
+            raise RuntimeError("page plan: " + ", ".join(w for b, w in (
+                (PLAN_PAGES, "too few free pages"), (PLAN_TABLE, "a request longer than its table"), (PLAN_ROWS, "too many rows"),
+                (PLAN_INCONSISTENT, "inconsistent lengths or ring")) if status & b))
+        return self
+
+
+def page_plan(new, lens, tables, free, span, page_size, rows, in_place=False):
+    """Plans a step on the device: request i, which holds lens[i] tokens, brings new[i] more, or is done (new[i] < 0). tables
+    [requests, max_pages] and the ring of free pages `free` [pages] are written; lens [requests] and span [2] too when in_place."""
+    requests = _int_rows(lens, "lens", -1).shape[0]
+    _int_rows(new, "new", requests)
+    _int_rows(tables, "tables", requests, -1)
+    _int_rows(free, "free", -1)
+    _int_rows(span, "span", 2)
+    if rows < 0:
+        raise ValueError("rows %d" % rows)
+    p = PagePlan()
+    p.lens, p.span = (lens, span) if in_place else (torch.empty_like(lens), torch.empty_like(span))
+    p.row_start, p.status = new.new_empty(requests + 1), new.new_empty(1)
+    p.pos, p.places = new.new_empty(rows), new.new_empty(rows)
+    shape = S.Pages(free.shape[0], page_size, requests, tables.shape[1])
+    rc = _lib.load().zq_page_plan(C.byref(shape), new.data_ptr(), lens.data_ptr(), p.lens.data_ptr(), tables.data_ptr(),
+                                  free.data_ptr(), span.data_ptr(), p.span.data_ptr(), p.row_start.data_ptr(), p.pos.data_ptr(),
+                                  p.places.data_ptr(), rows, p.status.data_ptr(), _raw_stream())
+    _lib.check(rc, "zq_page_plan")
+    return p
+
+
+class PageTable:
+    """Which pages each of n_requests requests holds, and which are free; shared by the caches of all layers."""
+
+    def __init__(self, pages, page_size, n_requests, max_pages):
+        self.page_size = int(page_size)
+        self.tables = torch.full((n_requests, max_pages), -1, dtype=torch.int32, device="cuda")
+        self.lens = torch.zeros(n_requests, dtype=torch.int32, device="cuda")
+        self.free = torch.arange(pages, dtype=torch.int32, device="cuda")
+        self.span = _i32([0, pages])
+
+    def plan(self, new, rows):
+        """The step in which request i brings new[i] tokens (int32 CUDA tensor [n_requests]; negative: it is done) -> PagePlan."""
+        return page_plan(new, self.lens, self.tables, self.free, self.span, self.page_size, rows, in_place=True)
+
+
+class PagedCache:
+    """Keys and values of a layer in pages that requests share."""
+
+    def __init__(self, heads, kv_heads, dim, vdim, pages, page_size, scale, norm_eps=1e-6, temp_coef=0.0, temp_every=0.0, f32=False):
+        self.g = S.Gqa(heads, kv_heads, dim, vdim, page_size, pages, scale, norm_eps, temp_coef, temp_every)
+        self.f32, self._dtype = bool(f32), _act_dtype(f32)
+        self._pitch = dense_pitch(heads * vdim)
+        up16 = lambda n: (n + 15) // 16 * 16
+        self.k = torch.zeros(pages, page_size, kv_heads, up16(dim), dtype=self._dtype, device="cuda")
+        self.v = torch.zeros(pages, page_size, kv_heads, up16(vdim), dtype=self._dtype, device="cuda")
+        self._pages = S.Pages(pages, page_size, 1, 1)
+        self._need = (0, 0, 0, 0)  # requests, pages of a table, rows and work bytes of the last call
+
+    def write(self, qkv, q_norm, k_norm, pos, places, vmix=None, v_first=None):
+        """Normalised queries [rows, heads, dim up to 16] of the projected rows; their keys and values go to the places of the plan."""
+        g, rows = self.g, qkv.shape[0]
+        if _here(_dev_f32(qkv), "qkv").shape != (rows, (g.heads + g.kv_heads) * g.dim + g.kv_heads * g.vdim):
+            raise ValueError("qkv: shape %s" % list(qkv.shape))
+        _int_rows(pos, "pos", rows)
+        _int_rows(places, "places", rows)
+        for t, n, what in ((q_norm, g.dim, "q_norm"), (k_norm, g.dim, "k_norm"), (vmix, 1, "vmix"), (v_first, rows * g.kv_heads * g.vdim, "v_first")):
+            if (t is not None or n == g.dim) and _here(_dev_f32(t), what).numel() != n:
+                raise ValueError("%s: %d values" % (what, t.numel()))
+        q = torch.empty(rows, g.heads, self.k.shape[3], dtype=self._dtype, device=qkv.device)
+        rc = _lib.load().zq_paged_cache_write(C.byref(g), C.byref(self._pages), qkv.data_ptr(), q_norm.data_ptr(), k_norm.data_ptr(),
+                                              _address(vmix), _address(v_first), q.data_ptr(), self.k.data_ptr(), self.v.data_ptr(),
+                                              pos.data_ptr(), places.data_ptr(), rows, int(self.f32), _raw_stream())
+        _lib.check(rc, "zq_paged_cache_write")
+        return q
+
+    def attend(self, q, row_start, lens, tables, out=None):
+        """[rows, pitch of heads * vdim] of a step's rows: rows row_start[i] ... row_start[i + 1] - 1 are the last tokens of request i,
+        which holds lens[i] tokens in the pages tables[i]. Rows of no request are left as they are in `out`."""
+        lib, g, rows = _lib.load(), self.g, q.shape[0]
+        requests, width = _int_rows(tables, "tables", -1, -1).shape
+        _int_rows(row_start, "row_start", requests + 1)
+        _int_rows(lens, "lens", requests)
+        if q.dtype != self._dtype or not q.is_contiguous() or q.shape != (rows, g.heads, self.k.shape[3]):
+            raise ValueError("q: expected the contiguous %s rows of write()" % self._dtype)
+        out = _result(_here(q, "q"), out, rows, self._pitch)
+        p = self._pages
+        p.requests, p.max_pages = requests, width
+        if self._need[:3] != (requests, width, rows):
+            self._need = (requests, width, rows, lib.zq_paged_work_bytes(C.byref(g), C.byref(p), rows, int(self.f32)))
+        need = self._need[3]
+        work = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        rc = lib.zq_paged_attention(C.byref(g), C.byref(p), q.data_ptr(), self.k.data_ptr(), self.v.data_ptr(), out.data_ptr(),
+                                    row_start.data_ptr(), lens.data_ptr(), tables.data_ptr(), rows, _address(work), need,
+                                    int(self.f32), _raw_stream())
+        _lib.check(rc, "zq_paged_attention")
+        return out
+
+
+def _result(q, out, rows, pitch):
+    if out is None:
+        return torch.empty(rows, pitch, dtype=q.dtype, device=q.device)
+    if out.dtype != q.dtype or out.shape != (rows, pitch) or not out.is_contiguous() or out.device != q.device:
+        raise ValueError("out: expected a contiguous %s tensor of shape %s" % (q.dtype, [rows, pitch]))
+    return out
+
+
+def packed_attention(q, k, v, row_start, scale, vdim=None, out=None):
+    """Causal grouped-query attention of whole sequences behind one another: rows row_start[i] ... row_start[i + 1] - 1 are sequence i.
+    q [rows, heads, d], k [rows, kv_heads, d], v [rows, kv_heads, e], bf16 or f32, d and e multiples of 16 (zeros beyond a head's
+    values); the rows may be parts of longer ones. -> [rows, pitch of heads * vdim], vdim: a head's values (e)."""
+    lib, (rows, heads, d) = _lib.load(), q.shape
+    kv_heads, e = v.shape[1:]
+    f32 = q.dtype == torch.float32
+    if q.dtype not in (torch.float32, torch.bfloat16) or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError("q, k and v: expected float32 or bfloat16, the same for all")
+    if k.shape != (rows, kv_heads, d) or v.shape[0] != rows or d % 16 or e % 16:
+        raise ValueError("shapes %s, %s, %s" % (list(q.shape), list(k.shape), list(v.shape)))
+    lds = []
+    for t, name in ((q, "q"), (k, "k"), (v, "v")):
+        _here(t, name)
+        n, ld = t.shape[1] * t.shape[2], t.stride(0)
+        if t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != t.shape[2]) or (rows > 1 and ld < n):
+            raise ValueError("%s: a row's heads have to lie behind one another" % name)
+        lds.append(ld if rows > 1 else n)
+    _int_rows(row_start, "row_start", -1)
+    vdim = e if vdim is None else int(vdim)
+    if not e - 16 < vdim <= e:
+        raise ValueError("vdim %d of %d columns" % (vdim, e))
+    out = _result(q, out, rows, (heads * vdim + 63) // 64 * 64)
+    g = S.Gqa(heads, kv_heads, d, vdim, 0, 0, scale, 0.0, 0.0, 0.0)
+    sequences = row_start.shape[0] - 1
+    need = lib.zq_packed_work_bytes(C.byref(g), sequences, rows, int(f32))
+    work = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    rc = lib.zq_packed_attention(C.byref(g), q.data_ptr(), lds[0], k.data_ptr(), lds[1], v.data_ptr(), lds[2], out.data_ptr(),
+                                 row_start.data_ptr(), sequences, rows, _address(work), need, int(f32), _raw_stream())
+    _lib.check(rc, "zq_packed_attention")
+    return out
+
+
 def token_shift(h, mu, prev, slot=0, f32=False):
     """h [rows, width], mu [n, width], prev [slots, width] -> [n, rows, pitch]."""
     (rows, width), slots = h.shape, _i32([slot])

@@ -1,0 +1,166 @@
+// C entry points of the paged cache and of packed prompts (include/zq.h): argument checks around the launchers of paged.h.
+#include "paged.h"
+
+using namespace zq;
+
+namespace {
+
+bool known(int precision) { return precision == ZQ_PRECISION_BF16 || precision == ZQ_PRECISION_F32; }
+bool is_f32(int precision) { return precision == ZQ_PRECISION_F32; }
+bool aligned(const void* p) { return ((uintptr_t)p & 15u) == 0; }
+
+bool valid(const zq_gqa* g) { return g && g->heads && g->kv_heads && g->heads % g->kv_heads == 0 && g->dim && g->vdim; }
+GqaShape shape_of(const zq_gqa* g) {
+    return GqaShape{g->heads, g->kv_heads, g->dim, g->vdim, pad_to(g->dim, 16), pad_to(g->vdim, 16), 0, 0};
+}
+bool small(const zq_gqa* g) { return g->dim <= kMaxPagedDim && g->vdim <= kMaxPagedDim && g->heads <= 65536; }
+
+int check(const zq_pages* p, uint32_t& shift) {
+    if (!p || !p->pages || !p->page_size || !p->requests || !p->max_pages) return ZQ_ERR_BAD_ARG;
+    for (shift = 4; shift <= 10; ++shift)
+        if (p->page_size == 1u << shift) break;
+    if (shift > 10) return ZQ_ERR_UNSUPPORTED;
+    if ((uint64_t)p->pages * p->page_size >= (1ull << 31) || (uint64_t)p->max_pages * p->page_size >= (1ull << 31)) return ZQ_ERR_LIMIT;
+    return ZQ_OK;
+}
+
+RaggedArgs args_of(const zq_gqa* g, uint32_t rows, uint32_t requests, uint32_t capacity) {
+    RaggedArgs a{};
+    a.s = shape_of(g);
+    a.q_ld = (size_t)g->heads * a.s.dimp;
+    a.k_ld = (size_t)g->kv_heads * a.s.dimp;
+    a.v_ld = (size_t)g->kv_heads * a.s.vdimp;
+    a.out_pitch = pad64(g->heads * g->vdim);
+    a.scale = g->scale;
+    a.rows = rows;
+    a.requests = requests;
+    a.capacity = capacity;
+    return a;
+}
+
+}  // namespace
+
+extern "C" {
+
+int zq_page_plan(const zq_pages* p, const int32_t* d_new, const int32_t* d_lens, int32_t* d_lens_out, int32_t* d_tables, int32_t* d_free,
+                 const int32_t* d_span, int32_t* d_span_out, int32_t* d_row_start, int32_t* d_pos, int32_t* d_places, uint32_t rows,
+                 int32_t* d_status, zq_stream stream) {
+    PagePlanArgs a{};
+    const int rc = check(p, a.shift);
+    if (rc != ZQ_OK) return rc;
+    if (!d_new || !d_lens || !d_lens_out || !d_tables || !d_free || !d_span || !d_span_out || !d_row_start || !d_status ||
+        (rows && (!d_pos || !d_places)))
+        return ZQ_ERR_BAD_ARG;
+    if (rows >= 1u << 30) return ZQ_ERR_LIMIT;
+    a.pages = p->pages;
+    a.requests = p->requests;
+    a.table_ld = p->max_pages;
+    a.rows = rows;
+    a.fresh = d_new;
+    a.lens = d_lens;
+    a.lens_out = d_lens_out;
+    a.tables = d_tables;
+    a.free = d_free;
+    a.span = d_span;
+    a.span_out = d_span_out;
+    a.row_start = d_row_start;
+    a.pos = d_pos;
+    a.places = d_places;
+    a.status = d_status;
+    return launch_page_plan(a, as_stream(stream));
+}
+
+int zq_paged_cache_write(const zq_gqa* g, const zq_pages* p, const float* d_qkv, const float* d_q_norm, const float* d_k_norm,
+                         const float* d_vmix, float* d_v_first, void* d_q, void* d_k_cache, void* d_v_cache, const int32_t* d_pos,
+                         const int32_t* d_places, uint32_t rows, int precision, zq_stream stream) {
+    uint32_t shift;
+    if (!valid(g)) return ZQ_ERR_BAD_ARG;
+    const int rc = check(p, shift);
+    if (rc != ZQ_OK) return rc;
+    if (!d_k_cache || !d_v_cache || !d_q_norm || !d_k_norm || !known(precision)) return ZQ_ERR_BAD_ARG;
+    if (rows == 0) return ZQ_OK;
+    if (!d_qkv || (d_vmix && !d_v_first) || !d_q || !d_pos || !d_places) return ZQ_ERR_BAD_ARG;
+    PagedWriteArgs a{};
+    a.s = shape_of(g);
+    a.qkv = d_qkv;
+    a.q_norm = d_q_norm;
+    a.k_norm = d_k_norm;
+    a.eps = g->norm_eps;
+    a.temp_coef = g->temp_coef;
+    a.temp_every = g->temp_every;
+    a.vmix = d_vmix;
+    a.v_first = d_v_first;
+    a.q = d_q;
+    a.kc = d_k_cache;
+    a.vc = d_v_cache;
+    a.pos = d_pos;
+    a.places = d_places;
+    a.n_places = p->pages * p->page_size;
+    return launch_paged_write(a, rows, is_f32(precision), as_stream(stream));
+}
+
+size_t zq_paged_work_bytes(const zq_gqa* g, const zq_pages* p, uint32_t rows, int precision) {
+    uint32_t shift;
+    if (!valid(g) || !small(g) || check(p, shift) != ZQ_OK || !known(precision)) return 0;
+    return ragged_work_bytes(args_of(g, rows, p->requests, p->max_pages * p->page_size), is_f32(precision));
+}
+
+int zq_paged_attention(const zq_gqa* g, const zq_pages* p, const void* d_q, const void* d_k_cache, const void* d_v_cache, void* d_out,
+                       const int32_t* d_row_start, const int32_t* d_lens, const int32_t* d_tables, uint32_t rows, void* d_work,
+                       size_t work_bytes, int precision, zq_stream stream) {
+    uint32_t shift;
+    if (!valid(g)) return ZQ_ERR_BAD_ARG;
+    const int rc = check(p, shift);
+    if (rc != ZQ_OK) return rc;
+    if (!d_k_cache || !d_v_cache || !d_row_start || !d_lens || !d_tables || !known(precision)) return ZQ_ERR_BAD_ARG;
+    if (!small(g) || rows >= 1u << 30) return ZQ_ERR_LIMIT;
+    if (rows == 0) return ZQ_OK;
+    if (!d_q || !d_out || !aligned(d_q) || !aligned(d_k_cache) || !aligned(d_v_cache) || !aligned(d_work)) return ZQ_ERR_BAD_ARG;
+    RaggedArgs a = args_of(g, rows, p->requests, p->max_pages * p->page_size);
+    a.q = d_q;
+    a.k = d_k_cache;
+    a.v = d_v_cache;
+    a.out = d_out;
+    a.row_start = d_row_start;
+    a.lens = d_lens;
+    a.tables = d_tables;
+    a.table_ld = p->max_pages;
+    a.shift = shift;
+    a.pages = p->pages;
+    a.work = d_work;
+    const size_t need = ragged_work_bytes(a, is_f32(precision));
+    if (need && (!d_work || work_bytes < need)) return ZQ_ERR_BAD_ARG;
+    return launch_ragged_attention(a, is_f32(precision), as_stream(stream));
+}
+
+size_t zq_packed_work_bytes(const zq_gqa* g, uint32_t sequences, uint32_t rows, int precision) {
+    if (!valid(g) || !small(g) || !known(precision)) return 0;
+    return ragged_work_bytes(args_of(g, rows, sequences, rows), is_f32(precision));
+}
+
+int zq_packed_attention(const zq_gqa* g, const void* d_q, size_t q_ld, const void* d_k, size_t k_ld, const void* d_v, size_t v_ld,
+                        void* d_out, const int32_t* d_row_start, uint32_t sequences, uint32_t rows, void* d_work, size_t work_bytes,
+                        int precision, zq_stream stream) {
+    if (!valid(g) || !d_row_start || !sequences || !known(precision)) return ZQ_ERR_BAD_ARG;
+    if (!small(g) || rows >= 1u << 30) return ZQ_ERR_LIMIT;
+    if (rows == 0) return ZQ_OK;
+    RaggedArgs a = args_of(g, rows, sequences, rows);
+    const size_t even = is_f32(precision) ? 4 : 8;  // rows start on 16-byte boundaries
+    if (!d_q || !d_k || !d_v || !d_out || !aligned(d_q) || !aligned(d_k) || !aligned(d_v) || !aligned(d_work) || q_ld < a.q_ld ||
+        k_ld < a.k_ld || v_ld < a.v_ld || q_ld % even || k_ld % even || v_ld % even)
+        return ZQ_ERR_BAD_ARG;
+    a.q = d_q;
+    a.k = d_k;
+    a.v = d_v;
+    a.q_ld = q_ld;
+    a.k_ld = k_ld;
+    a.v_ld = v_ld;
+    a.out = d_out;
+    a.row_start = d_row_start;
+    a.work = d_work;
+    const size_t need = ragged_work_bytes(a, is_f32(precision));
+    if (need && (!d_work || work_bytes < need)) return ZQ_ERR_BAD_ARG;
+    return launch_ragged_attention(a, is_f32(precision), as_stream(stream));
+}
+
+}  // extern "C"

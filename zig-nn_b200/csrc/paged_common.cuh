@@ -1,0 +1,133 @@
+// What the kernels of ragged attention share: the walk over the items of a call, the address of a token's key or value.
+//
+// An item is (request, tile of query rows, range of keys, key head, tile of heads). Rows are packed: row m of a tile is token m / R,
+// head m % R of the key head's R query heads; where R exceeds the tile's M rows, a tile is M heads of one token. How often a
+// request's keys are cut follows from its own length and from what the host knows (requests, heads, capacity), so that a row's
+// ranges, and with them its bits, do not depend on what the other requests hold.
+#pragma once
+#include "paged.h"
+
+namespace zq {
+namespace {
+
+constexpr uint32_t kRangeKeys = 64;  // ranges are whole multiples of this
+
+struct RaggedPlan {
+    uint32_t R, tokens, head_tiles;  // query heads per key head; tokens and tiles of heads of a row tile
+    uint32_t fill, most_keys;        // ranges that fill the GPU; keys of a range at most
+    uint32_t max_ranges;
+    float* part;                     // [rows][heads][max_ranges][vdimp], then [rows][heads][max_ranges][2]: maximum, sum
+    uint32_t* n_ranges;              // [rows]
+};
+
+struct Item {
+    uint32_t request, tile, range, ranges, g, head_tile;
+    uint32_t row0, n_rows;    // of the request
+    int32_t len;              // tokens that the request holds
+    uint32_t k_begin, k_end;  // keys of the range
+};
+
+__host__ __device__ inline uint32_t ranges_of(uint32_t len, uint32_t fill, uint32_t most_keys, uint32_t& per) {
+    const uint32_t blocks = (len + kRangeKeys - 1) / kRangeKeys;
+    if (blocks == 0) {
+        per = kRangeKeys;
+        return 1;
+    }
+    uint32_t n = blocks < fill ? blocks : fill;
+    const uint32_t least = (len + most_keys - 1) / most_keys;
+    if (n < least) n = least;
+    per = (blocks + n - 1) / n * kRangeKeys;
+    return (len + per - 1) / per;
+}
+
+// Calls body(item) for the items of this CTA: every gridDim.x-th. All threads take the same way. The requests are looked at as many at
+// once as the CTA has threads: a prefix sum over their counts of items, then a bisection per item.
+template <uint32_t THREADS, typename Body>
+__device__ __forceinline__ void for_items(const RaggedArgs& a, const RaggedPlan& p, Body body) {
+    __shared__ uint32_t first[THREADS + 1];
+    __shared__ uint32_t sums[THREADS / 32];
+    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, per_unit = a.s.kv_heads * p.head_tiles;
+    uint32_t next = blockIdx.x, base = 0;
+    auto span_of = [&](uint32_t i, uint32_t& row0, uint32_t& n_rows, int32_t& len) {
+        const int32_t b = a.row_start[i], e = a.row_start[i + 1];
+        row0 = b < 0 ? 0 : min((uint32_t)b, a.rows);
+        const uint32_t end = e < 0 ? 0 : min((uint32_t)e, a.rows);
+        n_rows = end > row0 ? end - row0 : 0;
+        len = a.lens ? min(a.lens[i], (int32_t)a.capacity) : (int32_t)n_rows;
+    };
+    for (uint32_t c = 0; c < a.requests; c += THREADS) {
+        uint32_t count = 0;
+        if (c + tid < a.requests) {
+            uint32_t row0, n_rows, per;
+            int32_t len;
+            span_of(c + tid, row0, n_rows, len);
+            count = (n_rows + p.tokens - 1) / p.tokens * ranges_of(len > 0 ? len : 0, p.fill, p.most_keys, per) * per_unit;
+        }
+        uint32_t scan = count;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const uint32_t o = __shfl_up_sync(0xFFFFFFFFu, scan, off);
+            if (lane >= (uint32_t)off) scan += o;
+        }
+        __syncthreads();
+        if (lane == 31) sums[warp] = scan;
+        __syncthreads();
+        for (uint32_t w = 0; w < warp; ++w) scan += sums[w];
+        first[tid + 1] = scan;
+        if (tid == 0) first[0] = 0;
+        __syncthreads();
+        const uint32_t total = first[THREADS];
+        while (next < base + total) {
+            const uint32_t x = next - base;
+            uint32_t lo = 0, hi = THREADS;
+            while (hi - lo > 1) {
+                const uint32_t mid = (lo + hi) >> 1;
+                if (first[mid] <= x) lo = mid;
+                else hi = mid;
+            }
+            Item it;
+            it.request = c + lo;
+            span_of(it.request, it.row0, it.n_rows, it.len);
+            uint32_t per, u = x - first[lo];
+            const uint32_t len = it.len > 0 ? it.len : 0;
+            it.ranges = ranges_of(len, p.fill, p.most_keys, per);
+            it.head_tile = u % p.head_tiles;
+            u /= p.head_tiles;
+            it.g = u % a.s.kv_heads;
+            u /= a.s.kv_heads;
+            it.range = u % it.ranges;
+            it.tile = u / it.ranges;
+            it.k_begin = it.range * per;
+            it.k_end = min(len, it.k_begin + per);
+            body(it);
+            next += gridDim.x;
+        }
+        base += total;
+    }
+}
+
+// Token and head of row m of an item's tile; false: no such row.
+__device__ __forceinline__ bool row_of(const RaggedPlan& p, const Item& it, uint32_t m, uint32_t M, uint32_t& token, uint32_t& head) {
+    if (p.head_tiles > 1) {
+        token = it.tile;
+        head = it.head_tile * M + m;
+        return head < p.R;
+    }
+    token = it.tile * p.tokens + m / p.R;
+    head = m % p.R;
+    return m < p.tokens * p.R && token < it.n_rows;
+}
+// Keys that token t of the request's rows sees.
+__device__ __forceinline__ int32_t seen_by(const Item& it, uint32_t t) { return it.len - (int32_t)it.n_rows + (int32_t)t + 1; }
+
+// First value of a token's keys (or values) of all heads; null: a page of zeros.
+template <typename T>
+__device__ __forceinline__ const T* token_row(const RaggedArgs& a, const Item& it, const T* base, size_t ld, uint32_t key) {
+    if (!a.lens) return base + (size_t)(it.row0 + key) * ld;
+    const uint32_t page = (uint32_t)__ldg(a.tables + (size_t)it.request * a.table_ld + (key >> a.shift));
+    if (page >= a.pages) return nullptr;
+    return base + (((size_t)page << a.shift) + (key & ((1u << a.shift) - 1))) * ld;
+}
+
+}  // namespace
+}  // namespace zq

@@ -1,0 +1,229 @@
+// Bookkeeping of a paged key / value cache on the device: which rows, positions, places and pages a step has, and the write of the
+// rows' keys and values to their places.
+#include "paged.h"
+
+namespace zq {
+namespace {
+
+constexpr uint32_t kPlanThreads = 1024;
+
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
+// Last i < n with first[i] <= x (first ascending, first[0] = 0): the request that x falls to. Requests without any x are passed over.
+__device__ __forceinline__ uint32_t owner(const int32_t* first, uint32_t n, int32_t x) {
+    uint32_t lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) >> 1;
+        if (first[mid] <= x) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+__device__ __forceinline__ int64_t warp_scan(int64_t v, uint32_t lane) {
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+        const int64_t o = __shfl_up_sync(0xFFFFFFFFu, v, off);
+        if (lane >= (uint32_t)off) v += o;
+    }
+    return v;
+}
+
+// With N_i tokens brought and L_i held, page P: pages taken by request i are ceil((L + N) / P) - ceil(L / P); rows, pages taken and
+// pages given back are three prefix sums over the requests. Every CTA of the cluster makes all three (a few requests per thread,
+// shuffles, one pass through shared memory): that is cheaper than to hand them round. Behind a barrier of the cluster, which ends all
+// reads of what may be overwritten in place, the CTAs share rows and pages; a row, or a page, finds its request by bisection.
+// What bounds it: latency (a load, the sums, a barrier, 6 to 13 steps of bisection, a load of the table, a store).
+__global__ void __launch_bounds__(kPlanThreads)
+page_plan_kernel(const __grid_constant__ PagePlanArgs a) {
+    extern __shared__ __align__(16) int32_t sm[];
+    __shared__ int64_t part[3][32];
+    pdl_launch_dependents();
+    pdl_wait();
+    const uint32_t n = a.requests, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, P = 1u << a.shift;
+    int32_t *row0 = sm, *take0 = sm + n + 1, *give0 = sm + 2 * (n + 1), *len = sm + 3 * (n + 1);
+    const int64_t cap = (int64_t)a.table_ld << a.shift;
+    const int32_t first = a.span[0], count = a.span[1];
+    int bad = first < 0 || (uint32_t)first >= a.pages || count < 0 || (uint32_t)count > a.pages ? ZQ_PLAN_INCONSISTENT : 0;
+
+    const uint32_t each = (n + kPlanThreads - 1) / kPlanThreads, i0 = min(tid * each, n), i1 = min(i0 + each, n);
+    int64_t sum[3] = {0, 0, 0}, got[3];
+    auto of = [&](uint32_t i, int64_t& rows, int64_t& take, int64_t& give) {  // what request i adds
+        const int64_t l = a.lens[i], m = a.fresh[i];
+        const int64_t have = (l + P - 1) >> a.shift;
+        rows = m > 0 ? m : 0;
+        take = m > 0 ? ((l + m + P - 1) >> a.shift) - have : 0;
+        give = m < 0 ? have : 0;
+        if (l < 0 || l > cap) {
+            bad |= ZQ_PLAN_INCONSISTENT;
+            rows = take = give = 0;
+        } else if (l + rows > cap) {
+            bad |= ZQ_PLAN_TABLE;
+            rows = take = 0;
+        }
+        return (int32_t)l;
+    };
+    for (uint32_t i = i0; i < i1; ++i) {
+        int64_t x[3];
+        len[i] = of(i, x[0], x[1], x[2]);
+#pragma unroll
+        for (int k = 0; k < 3; ++k) sum[k] += x[k];
+    }
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+        got[k] = warp_scan(sum[k], lane);
+        if (lane == 31) part[k][warp] = got[k];
+    }
+    __syncthreads();
+    int64_t total[3];
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+        const int64_t p = warp_scan(part[k][lane], lane);
+        total[k] = __shfl_sync(0xFFFFFFFFu, p, 31);
+        got[k] += (warp ? __shfl_sync(0xFFFFFFFFu, p, warp - 1) : 0) - sum[k];  // ahead of this thread's requests
+    }
+    if (total[0] > (int64_t)a.rows) bad |= ZQ_PLAN_ROWS;
+    if (total[1] > count) bad |= ZQ_PLAN_PAGES;
+    if (count + total[2] > (int64_t)a.pages) bad |= ZQ_PLAN_INCONSISTENT;
+    // the flags of the threads, or-ed: one vote per flag
+    int status = 0;
+#pragma unroll
+    for (int f = ZQ_PLAN_PAGES; f <= ZQ_PLAN_INCONSISTENT; f <<= 1) status |= __syncthreads_or(bad & f) ? f : 0;
+    if (status == 0) {
+        for (uint32_t i = i0; i < i1; ++i) {
+            int64_t x[3];
+            of(i, x[0], x[1], x[2]);
+            row0[i] = (int32_t)got[0];
+            take0[i] = (int32_t)got[1];
+            give0[i] = (int32_t)got[2];
+#pragma unroll
+            for (int k = 0; k < 3; ++k) got[k] += x[k];
+        }
+    }
+    if (tid == 0) {
+        row0[n] = status ? 0 : (int32_t)total[0];
+        take0[n] = status ? 0 : (int32_t)total[1];
+        give0[n] = status ? 0 : (int32_t)total[2];
+    }
+    __syncthreads();
+    cluster_arrive();  // lengths, tokens and span have been read
+    cluster_wait();
+
+    const uint32_t grid = gridDim.x * kPlanThreads, me = blockIdx.x * kPlanThreads + tid;
+    const int32_t rows = row0[n], taken = take0[n], given = give0[n];
+    auto wrap = [&](uint32_t x) { return x >= a.pages ? x - a.pages : x; };
+    if (me == 0) {
+        *a.status = status;
+        a.span_out[0] = status ? first : (int32_t)wrap((uint32_t)first + taken);
+        a.span_out[1] = status ? count : count - taken + given;
+        a.row_start[n] = rows;
+    }
+    for (uint32_t i = me; i < n; i += grid) {
+        const int32_t l = len[i];
+        a.row_start[i] = status ? 0 : row0[i];
+        const bool done = !status && give0[i + 1] > give0[i];
+        a.lens_out[i] = status ? l : done ? 0 : l + row0[i + 1] - row0[i];
+    }
+    for (uint32_t t = me; t < (uint32_t)taken; t += grid) {
+        const uint32_t i = owner(take0, n, (int32_t)t);
+        const uint32_t have = ((uint32_t)len[i] + P - 1) >> a.shift;
+        a.tables[(size_t)i * a.table_ld + have + (t - take0[i])] = a.free[wrap((uint32_t)first + t)];
+    }
+    for (uint32_t t = me; t < (uint32_t)given; t += grid) {  // behind the free ones: no place that this call takes from
+        const uint32_t i = owner(give0, n, (int32_t)t);
+        a.free[wrap(wrap((uint32_t)first + count) + t)] = a.tables[(size_t)i * a.table_ld + (t - give0[i])];
+    }
+    for (uint32_t r0 = me * 4; r0 < a.rows; r0 += grid * 4) {
+        int32_t pos[4], place[4];
+        uint32_t i = (int32_t)r0 < rows ? owner(row0, n, (int32_t)r0) : 0;
+#pragma unroll
+        for (uint32_t e = 0; e < 4; ++e) {
+            const int32_t r = (int32_t)(r0 + e);
+            pos[e] = 0;
+            place[e] = -1;
+            if (r < rows) {
+                while (row0[i + 1] <= r) ++i;
+                pos[e] = len[i] + r - row0[i];
+                const uint32_t j = (uint32_t)pos[e] >> a.shift, have = ((uint32_t)len[i] + P - 1) >> a.shift;
+                const int32_t page = j < have ? a.tables[(size_t)i * a.table_ld + j] : a.free[wrap((uint32_t)first + take0[i] + (j - have))];
+                if ((uint32_t)page < a.pages) place[e] = (page << a.shift) + (pos[e] & (int32_t)(P - 1));
+            }
+        }
+        if (r0 + 4 <= a.rows && ((((uintptr_t)a.pos) | ((uintptr_t)a.places)) & 15u) == 0) {
+            *reinterpret_cast<int4*>(a.pos + r0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
+            *reinterpret_cast<int4*>(a.places + r0) = make_int4(place[0], place[1], place[2], place[3]);
+        } else {
+            for (uint32_t e = 0; e < 4 && r0 + e < a.rows; ++e) {
+                a.pos[r0 + e] = pos[e];
+                a.places[r0 + e] = place[e];
+            }
+        }
+    }
+}
+
+// A warp per head of a row: norms and temperature for queries and keys, the mix for values.
+template <typename TA>
+__global__ void __launch_bounds__(128)
+paged_write_kernel(const __grid_constant__ PagedWriteArgs a) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const GqaShape& s = a.s;
+    const uint32_t lane = threadIdx.x & 31, item = blockIdx.y * 4 + (threadIdx.x >> 5), r = blockIdx.x;
+    if (item >= s.heads + 2 * s.kv_heads) return;
+    const float* row = a.qkv + (size_t)r * ((s.heads + s.kv_heads) * s.dim + s.kv_heads * s.vdim);
+    const uint32_t place = (uint32_t)a.places[r];
+    const bool kept = place < a.n_places;
+    if (item < s.heads + s.kv_heads) {
+        const bool is_q = item < s.heads;
+        if (!is_q && !kept) return;
+        const float t = is_q ? query_temperature((uint32_t)a.pos[r], a.temp_coef, a.temp_every) : 1.0f;
+        TA* o = is_q ? static_cast<TA*>(a.q) + ((size_t)r * s.heads + item) * s.dimp
+                     : static_cast<TA*>(a.kc) + ((size_t)place * s.kv_heads + (item - s.heads)) * s.dimp;
+        norm_head(row + (size_t)item * s.dim, is_q ? a.q_norm : a.k_norm, s.dim, s.dimp, a.eps, t, o, lane);
+    } else {
+        const uint32_t g = item - s.heads - s.kv_heads;
+        const float* v = row + (size_t)(s.heads + s.kv_heads) * s.dim + (size_t)g * s.vdim;
+        float* first = a.v_first ? a.v_first + ((size_t)r * s.kv_heads + g) * s.vdim : nullptr;
+        TA* o = static_cast<TA*>(a.vc) + ((size_t)place * s.kv_heads + g) * s.vdimp;
+        for (uint32_t i = lane; i < s.vdimp; i += 32) {
+            const TA x = to_act<TA>(i < s.vdim ? mixed_value(v[i], a.vmix, first, i) : 0.0f);
+            if (kept) o[i] = x;
+        }
+    }
+}
+
+int done(cudaError_t e) { return e == cudaSuccess ? ZQ_OK : cuda_fail(e); }
+
+}  // namespace
+
+int launch_page_plan(const PagePlanArgs& a, cudaStream_t st) {
+    if (a.requests > kMaxPlanRequests) return ZQ_ERR_LIMIT;
+    const uint32_t smem = 4 * (a.requests + 1) * sizeof(int32_t);
+    ZQ_CUDA(cudaFuncSetAttribute(page_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 4 * (kMaxPlanRequests + 1) * sizeof(int32_t)));
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[2];
+    const uint32_t ctas = a.rows <= 4 * kPlanThreads && a.requests <= kPlanThreads ? 1 : 8;
+    cfg.gridDim = dim3(ctas);
+    cfg.blockDim = dim3(kPlanThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = ctas;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    return done(cudaLaunchKernelEx(&cfg, page_plan_kernel, a));
+}
+
+int launch_paged_write(const PagedWriteArgs& a, uint32_t rows, bool f32, cudaStream_t st) {
+    if (rows == 0) return ZQ_OK;
+    const dim3 grid(rows, (a.s.heads + 2 * a.s.kv_heads + 3) / 4);
+    return done(f32 ? launch_pdl(paged_write_kernel<float>, grid, dim3(128), 0, st, a)
+                    : launch_pdl(paged_write_kernel<bf16>, grid, dim3(128), 0, st, a));
+}
+
+}  // namespace zq

@@ -103,6 +103,10 @@ class Gqa(C.Structure):
         (n, C.c_float) for n in ("scale", "norm_eps", "temp_coef", "temp_every")]
 
 
+class Pages(C.Structure):
+    _fields_ = [(n, C.c_uint32) for n in ("pages", "page_size", "requests", "max_pages")]
+
+
 class DecoderConfig(C.Structure):
     _fields_ = [(n, C.c_uint32) for n in ("vocab", "width", "layers", "ctx", "n_seq")] + [
         ("precision", C.c_int32), ("embed_scale", C.c_float), ("norm_eps", C.c_float)]
