@@ -47,5 +47,9 @@ struct RaggedArgs {
 };
 size_t ragged_work_bytes(const RaggedArgs& a, bool f32);
 int launch_ragged_attention(const RaggedArgs& a, bool f32, cudaStream_t st);
+// Its form on tcgen05, for requests with more than a few rows (bf16): whether it has one, its work memory.
+bool ragged_tc_takes(const RaggedArgs& a);
+size_t ragged_tc_work_bytes(const RaggedArgs& a);
+int launch_ragged_tc(const RaggedArgs& a, cudaStream_t st);
 
 }  // namespace zq

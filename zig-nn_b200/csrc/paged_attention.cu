@@ -290,11 +290,15 @@ int plain_any(const RaggedCall& c, uint32_t M, cudaStream_t st) {
 
 }  // namespace
 
-size_t ragged_work_bytes(const RaggedArgs& a, bool) { return plan_bytes(a, plan_of(a, tile_rows(a))); }
+size_t ragged_work_bytes(const RaggedArgs& a, bool f32) {
+    const uint32_t M = tile_rows(a);
+    return !f32 && M == 64 && ragged_tc_takes(a) ? ragged_tc_work_bytes(a) : plan_bytes(a, plan_of(a, M));
+}
 
 int launch_ragged_attention(const RaggedArgs& a, bool f32, cudaStream_t st) {
     if (a.rows == 0 || a.requests == 0) return ZQ_OK;
     const uint32_t M = tile_rows(a);
+    if (!f32 && M == 64 && ragged_tc_takes(a)) return launch_ragged_tc(a, st);
     const RaggedCall c{a, plan_of(a, M)};
     int rc = f32 ? plain_any<float>(c, M, st) : plain_any<bf16>(c, M, st);
     if (rc != ZQ_OK || c.p.max_ranges < 2) return rc;

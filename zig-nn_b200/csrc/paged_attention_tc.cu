@@ -1,0 +1,836 @@
+// Attention of ragged rows on the 5th-generation tensor cores: 128 packed query rows (token, head of the group) against tiles of 128
+// keys, softmax in f32.
+//
+//   S = Q K^T   both operands K-major in shared memory (128-byte swizzle), S in tensor memory;
+//   softmax     one thread per row (its row is a tensor-memory lane), no exchange between threads; the running maximum is raised, and
+//               the output rescaled, only when it grows by more than 2^8: until then the weights are taken against the older maximum;
+//   O += P V    P (bf16) is the A operand from tensor memory, where it overwrites its own scores; V as it lies in the cache (rows
+//               of keys: MN-major).
+// Up to 128 dimensions two such tiles of rows (STREAMS = 2) take turns on one stream of keys: the tensor cores work on one while the
+// other's softmax runs. Beyond that O takes half of tensor memory; one tile, two buffers of scores.
+// Keys and values come through one ring of 16 KB slots: a slot holds 64 dimensions of 128 keys, or all dimensions of 128 / VS keys
+// as values, brought in by tensor copies of a page's rows (or 128 packed rows). Pages that do not exist are coordinates outside the
+// tensor: zeros. Values behind the last key that the tile sees are overwritten with zeros, whatever the page holds there.
+//
+// Work is cut evenly: the tiles' key tiles (and a constant per tile), one behind the other, are shared out in equal contiguous parts,
+// one per SM. What a part has of a tile that it does not cover alone goes to a slot of partial sums; a third kernel joins these.
+// Roles: warps 0-3 (and 4-7 with two streams) softmax and results; then a warp that issues copies, and one that issues MMAs and owns
+// the tensor memory. Every wait is bounded, as in gemm_bf16.cu.
+#include "paged.h"
+#include "tc_common.cuh"
+
+namespace zq {
+namespace {
+
+constexpr uint32_t TK = 128;                // keys of a tile
+constexpr uint32_t SLOT = 128 * 128;        // bytes of 128 keys x 64 dimensions
+constexpr uint32_t kMaxSlots = 12;
+constexpr uint32_t kMaxParts = 160;         // CTAs
+constexpr float kRaise = 8.0f;              // powers of two that the maximum may lag behind
+constexpr uint32_t kTileCost = 1;           // what a tile costs besides its keys, in key tiles
+constexpr uint32_t kLeastPart = 3;          // key tiles that a CTA is started for
+constexpr uint32_t kPrepThreads = 1024;
+constexpr uint32_t kSearchTiles = 4096;     // tiles whose costs the search keeps in shared memory
+
+struct TileRec {
+    uint32_t row0;     // first row of the tile
+    uint32_t tokens;   // of the request, from row0 on; at most the tile's
+    int32_t see0;      // keys that the first of them sees
+    uint32_t kt;       // key tiles
+    uint32_t request, first_row;  // and the request's first row
+    uint32_t cost0_lo, cost0_hi;  // cost of the tiles ahead (per key head)
+};
+struct PartRec {
+    uint32_t tile, g, off, n_units;
+};
+struct SplitRec {  // the tile that begins in this part and ends in part `last`; tile = ~0: none
+    uint32_t tile, g, last, pad;
+};
+struct TcWork {
+    uint32_t* head;  // parts
+    PartRec* parts;
+    SplitRec* splits;
+    TileRec* tiles;
+    float* partial;
+};
+struct TcParams {
+    RaggedArgs a;
+    TcWork w;
+    uint32_t R, rt;            // heads of a group; tokens of a stream's tile
+    uint32_t max_parts, max_tiles;
+    float scale2;
+    uint32_t dk, dv;           // 64-wide blocks of a key / value row
+    uint32_t vs, vk;           // slots of a tile's values, keys of such a slot
+    uint32_t kbox, vbox;       // rows of a copy
+    uint32_t n_slots, slots_at;
+    unsigned int* err;
+};
+
+__device__ __forceinline__ uint64_t cost0_of(const TileRec& t) { return ((uint64_t)t.cost0_hi << 32) | t.cost0_lo; }
+
+// ---- the list of tiles and the parts ------------------------------------------------------------------------------------
+__device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t* sums, uint64_t& total) {  // inclusive; sums: 32
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+        const uint64_t o = __shfl_up_sync(0xFFFFFFFFu, v, off);
+        if (lane >= (uint32_t)off) v += o;
+    }
+    __syncthreads();
+    if (lane == 31) sums[warp] = v;
+    __syncthreads();
+    uint64_t s = sums[lane];
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+        const uint64_t o = __shfl_up_sync(0xFFFFFFFFu, s, off);
+        if (lane >= (uint32_t)off) s += o;
+    }
+    total = __shfl_sync(0xFFFFFFFFu, s, 31);
+    const uint64_t before = __shfl_sync(0xFFFFFFFFu, s, (warp + 31) & 31);
+    return v + (warp ? before : 0);
+}
+
+__global__ void __launch_bounds__(kPrepThreads)
+ragged_prep_kernel(const __grid_constant__ TcParams p, uint32_t tile_tokens) {
+    __shared__ uint64_t sums[32];
+    __shared__ uint32_t first[kPrepThreads + 1];
+    __shared__ uint32_t rows_of[kPrepThreads];
+    __shared__ int32_t len_of[kPrepThreads];
+    __shared__ uint64_t cost0[kSearchTiles];
+    pdl_launch_dependents();
+    pdl_wait();
+    const RaggedArgs& a = p.a;
+    const uint32_t tid = threadIdx.x;
+    uint32_t n_tiles = 0;
+    uint64_t cost = 0;
+    for (uint32_t c = 0; c < a.requests; c += kPrepThreads) {
+        uint32_t n_rows = 0, tiles = 0;
+        if (c + tid < a.requests) {
+            const int32_t b = a.row_start[c + tid], e = a.row_start[c + tid + 1];
+            const uint32_t row0 = b < 0 ? 0 : min((uint32_t)b, a.rows), end = e < 0 ? 0 : min((uint32_t)e, a.rows);
+            n_rows = end > row0 ? end - row0 : 0;
+            len_of[tid] = a.lens ? min(a.lens[c + tid], (int32_t)a.capacity) : (int32_t)n_rows;
+            rows_of[tid] = n_rows;
+            tiles = (n_rows + tile_tokens - 1) / tile_tokens;
+        }
+        uint64_t total;
+        const uint64_t scan = block_scan(tiles, sums, total);
+        first[tid + 1] = (uint32_t)scan;
+        if (tid == 0) first[0] = 0;
+        __syncthreads();
+        for (uint32_t t0 = 0; t0 < (uint32_t)total; t0 += kPrepThreads) {
+            const uint32_t t = t0 + tid;
+            TileRec r{};
+            uint32_t mine = 0;
+            if (t < (uint32_t)total && n_tiles + t < p.max_tiles) {
+                uint32_t lo = 0, hi = kPrepThreads;
+                while (hi - lo > 1) {
+                    const uint32_t mid = (lo + hi) >> 1;
+                    if (first[mid] <= t) lo = mid;
+                    else hi = mid;
+                }
+                const uint32_t token0 = (t - first[lo]) * tile_tokens, rows = rows_of[lo];
+                const int32_t b = a.row_start[c + lo];
+                r.first_row = b < 0 ? 0 : (uint32_t)b;
+                r.row0 = r.first_row + token0;
+                r.tokens = min(tile_tokens, rows - token0);
+                r.see0 = len_of[lo] - (int32_t)rows + (int32_t)token0 + 1;
+                const int32_t last = r.see0 + (int32_t)r.tokens - 1;
+                r.kt = last > 0 ? ((uint32_t)last + TK - 1) / TK : 0;
+                r.request = c + lo;
+                mine = r.kt + kTileCost;
+            }
+            uint64_t all;
+            const uint64_t before = cost + block_scan(mine, sums, all) - mine;
+            if (t < (uint32_t)total && n_tiles + t < p.max_tiles) {
+                r.cost0_lo = (uint32_t)before;
+                r.cost0_hi = (uint32_t)(before >> 32);
+                p.w.tiles[n_tiles + t] = r;
+                if (n_tiles + t < kSearchTiles) cost0[n_tiles + t] = before;
+            }
+            cost += all;
+        }
+        n_tiles = min(n_tiles + (uint32_t)total, p.max_tiles);  // rows named twice may make more: these are left out
+        __syncthreads();
+    }
+    const uint64_t U = cost * a.s.kv_heads;
+    uint64_t G = U / (kLeastPart + kTileCost);
+    G = G < 1 ? 1 : G > p.max_parts ? p.max_parts : G;
+    if (tid == 0) p.w.head[0] = U ? (uint32_t)G : 0;
+    if (U == 0 || tid >= (uint32_t)G) return;
+    auto find = [&](uint64_t u, uint32_t& tile, uint32_t& g, uint32_t& off, uint32_t& kt) {  // the tile of unit u
+        uint32_t lo = 0, hi = n_tiles;
+        while (hi - lo > 1) {
+            const uint32_t mid = (lo + hi) >> 1;
+            const uint64_t at = mid < kSearchTiles ? cost0[mid] : cost0_of(p.w.tiles[mid]);
+            if (at * a.s.kv_heads <= u) lo = mid;
+            else hi = mid;
+        }
+        kt = p.w.tiles[lo].kt;
+        const uint64_t rest = u - cost0_of(p.w.tiles[lo]) * a.s.kv_heads;
+        tile = lo;
+        g = (uint32_t)(rest / (kt + kTileCost));
+        off = (uint32_t)(rest % (kt + kTileCost));
+        return u - off;  // its first unit
+    };
+    const uint64_t b0 = U * tid / G, b1 = U * (tid + 1) / G;
+    PartRec part;
+    uint32_t kt;
+    find(b0, part.tile, part.g, part.off, kt);
+    part.n_units = (uint32_t)(b1 - b0);
+    p.w.parts[tid] = part;
+    SplitRec s{~0u, 0, 0, 0};
+    uint32_t tile, g, off;
+    const uint64_t begin = find(b1 - 1, tile, g, off, kt);
+    if (off + 1 < kt && begin >= b0) {
+        s.tile = tile;
+        s.g = g;
+        s.last = (uint32_t)(((begin + kt) * G - 1) / U);  // the part of its last key tile
+    }
+    p.w.splits[tid] = s;
+}
+
+// ---- the tiles --------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ void tc_st32(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// A operand from tensor memory: 128 lanes, two bf16 a column
+__device__ __forceinline__ void tc_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// Descriptor of a [keys][64 values] tile read with the values as the operand's rows (MN-major, 128-byte swizzle): 64-value blocks
+// `block` bytes apart, groups of 8 keys 1024 bytes apart.
+__device__ __forceinline__ uint64_t smem_desc_mn_sw128(uint32_t saddr, uint32_t block) {
+    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | (uint64_t)(block >> 4) << 16 | (uint64_t)(1024u >> 4) << 32 | (uint64_t)1 << 46 |
+           (uint64_t)2 << 61;
+}
+__device__ __forceinline__ void tensor_copy_4d(uint32_t dst, const CUtensorMap* map, uint32_t x, uint32_t y, uint32_t z, uint32_t w,
+                                               uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_tx(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// Registers: whole groups of four warps may pass registers to one another, so two streams come with a third group. 384 threads start
+// with 168 each (64512); 2 x 128 x 208 + 128 x 88 are as many.
+constexpr uint32_t tc_threads(int streams) { return streams == 2 ? 384 : 192; }
+template <int STREAMS>
+__device__ __forceinline__ void split_registers(bool softmax) {
+    if (STREAMS != 2) return;
+    if (softmax) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+}
+
+// One piece of the walk through a part: key tiles [kb, ke) of (tile, g).
+struct Walk {
+    TileRec t;
+    uint32_t tile, g, off, left, kb, ke;
+    bool whole;
+};
+
+template <int STREAMS>
+__global__ void __launch_bounds__(tc_threads(STREAMS), 1)
+ragged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                 const __grid_constant__ CUtensorMap map_v, const __grid_constant__ TcParams p) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    __shared__ __align__(8) unsigned long long bars[13 + 2 * kMaxSlots];
+    __shared__ uint32_t tmem_slot;
+    __shared__ int abort_flag;
+    pdl_launch_dependents();
+    constexpr uint32_t LOADER = STREAMS * 4, ISSUER = LOADER + 1;
+    const RaggedArgs& a = p.a;
+    const GqaShape& s = a.s;
+    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const uint32_t base = ((uint32_t)__cvta_generic_to_shared(smem) + 1023u) & ~1023u;
+    const uint32_t bar32 = (uint32_t)__cvta_generic_to_shared(bars);
+    const uint32_t q_full = bar32, q_empty = bar32 + 8, v_clean = bar32 + 16;
+    auto s_full = [&](uint32_t i) { return bar32 + 8 * (3 + i); };
+    auto p_full = [&](uint32_t i) { return bar32 + 8 * (5 + i); };
+    auto pv_done = [&](uint32_t i) { return bar32 + 8 * (7 + i); };  // one stream only
+    auto o_full = [&](uint32_t i) { return bar32 + 8 * (9 + i); };
+    auto o_free = [&](uint32_t i) { return bar32 + 8 * (11 + i); };
+    auto full = [&](uint32_t i) { return bar32 + 8 * (13 + i); };
+    auto empty = [&](uint32_t i) { return bar32 + 8 * (13 + kMaxSlots + i); };
+    auto slot_at = [&](uint32_t i) { return base + p.slots_at + i * SLOT; };
+
+    if (tid == 0) {
+        mbar_init(q_full, 1);
+        mbar_init(q_empty, 1);
+        mbar_init(v_clean, 1);
+        for (uint32_t i = 0; i < 2; ++i) {
+            mbar_init(s_full(i), 1);
+            mbar_init(p_full(i), 4);
+            mbar_init(pv_done(i), 1);
+            mbar_init(o_full(i), 1);
+            mbar_init(o_free(i), 4);
+        }
+        for (uint32_t i = 0; i < p.n_slots; ++i) {
+            mbar_init(full(i), 1);
+            mbar_init(empty(i), 1);
+        }
+        abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == ISSUER) {
+        const uint32_t slot = (uint32_t)__cvta_generic_to_shared(&tmem_slot);
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(slot) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;  // S 0 | S 1 | O 0 (| O 1)
+    volatile int* ab = &abort_flag;
+    pdl_wait();
+
+    const uint32_t c = blockIdx.x;
+    const bool busy = c < p.w.head[0];
+    Walk w{};
+    if (busy) {
+        const PartRec part = p.w.parts[c];
+        w.tile = part.tile;
+        w.g = part.g;
+        w.off = part.off;
+        w.left = part.n_units;
+        w.t = p.w.tiles[w.tile];
+    }
+    // The next piece; the tile's record is the one that w.t holds when the walk enters it.
+    auto next = [&]() {
+        while (w.left) {
+            const uint32_t cost = w.t.kt + kTileCost, n = min(cost - w.off, w.left);
+            w.kb = w.off;
+            w.ke = min(w.t.kt, w.off + n);
+            w.left -= n;
+            w.off += n;
+            w.whole = w.kb == 0 && w.ke == w.t.kt;
+            if (w.kb < w.ke || (w.kb == 0 && w.t.kt == 0)) return true;
+            if (w.left) {  // only the constant was left of it
+                w.off = 0;
+                if (++w.g == s.kv_heads) {
+                    w.g = 0;
+                    w.t = p.w.tiles[++w.tile];
+                }
+            }
+        }
+        return false;
+    };
+    auto leave = [&]() {  // behind a piece
+        if (w.left) {
+            w.off = 0;
+            if (++w.g == s.kv_heads) {
+                w.g = 0;
+                w.t = p.w.tiles[++w.tile];
+            }
+        }
+    };
+
+    if (warp >= LOADER) {
+        split_registers<STREAMS>(false);
+        if (warp == LOADER) {
+            bool alive = true;
+            uint32_t n = 0, pieces = 0, cleaned = 0;  // slots asked for
+            auto enter = [&](uint32_t bytes) {  // the next slot, free
+                const uint32_t i = n % p.n_slots, use = n / p.n_slots;
+                if (use > 0) alive = alive && mbar_wait(empty(i), (use - 1) & 1u, ab, p.err);
+                alive = __all_sync(0xFFFFFFFFu, alive);
+                if (alive && lane == 0) mbar_arrive_tx(full(i), bytes);
+                __syncwarp();
+                if (alive) ++n;
+                return i;
+            };
+            // `rows` rows from key k0 on, `blocks` blocks of 64 columns (from block b0) to dst: copies of `box` rows, a lane each
+            auto copy = [&](const CUtensorMap* map, uint32_t dst, uint32_t k0, uint32_t rows, uint32_t box, uint32_t b0, uint32_t blocks, uint32_t bar) {
+                const uint32_t per = rows / box;
+                for (uint32_t i = lane; i < per * blocks; i += 32) {
+                    const uint32_t b = i / per, r = i % per * box, key = k0 + r;
+                    uint32_t y = w.t.first_row + key, z = 0;
+                    if (a.lens) {
+                        const uint32_t j = key >> a.shift;
+                        const uint32_t page = j < a.table_ld ? (uint32_t)__ldg(a.tables + (size_t)w.t.request * a.table_ld + j) : a.pages;
+                        z = page < a.pages ? page : a.pages;
+                        y = key & ((1u << a.shift) - 1);
+                    }
+                    tensor_copy_4d(dst + (b * rows + r) * 128, map, (b0 + b) * 64, w.g, y, z, bar);
+                }
+            };
+            asm volatile("fence.proxy.async.global;" ::: "memory");
+            while (alive && next()) {
+                if (w.kb < w.ke) {
+                    const uint32_t end = (uint32_t)(w.t.see0 + (int32_t)w.t.tokens - 1);  // keys that the tile sees
+                    auto keys = [&](uint32_t t) {
+                        for (uint32_t b = 0; b < p.dk && alive; ++b) {
+                            const uint32_t i = enter(SLOT);
+                            if (alive) copy(&map_k, slot_at(i), t * TK, TK, p.kbox, b, 1, full(i));
+                        }
+                    };
+                    auto values = [&](uint32_t t) {
+                        uint32_t at[8];
+                        for (uint32_t v = 0; v < p.vs && alive; ++v) {
+                            at[v & 7] = enter(p.vk * p.dv * 128);
+                            if (alive) copy(&map_v, slot_at(at[v & 7]), t * TK + v * p.vk, p.vk, p.vbox, 0, p.dv, full(at[v & 7]));
+                        }
+                        if (!alive || (t + 1) * TK <= end) return;
+                        for (uint32_t v = 0; v < p.vs && alive; ++v) {  // what lies behind the last key is no value
+                            const uint32_t k0 = t * TK + v * p.vk, keep = k0 >= end ? 0 : min(end - k0, p.vk), i = at[v & 7];
+                            if (keep == p.vk) continue;
+                            alive = mbar_wait(full(i), ((n - p.vs + v) / p.n_slots) & 1u, ab, p.err);
+                            alive = __all_sync(0xFFFFFFFFu, alive);
+                            for (uint32_t e = lane; alive && e < (p.vk - keep) * 8 * p.dv; e += 32) {
+                                const uint32_t b = e / ((p.vk - keep) * 8), rest = e % ((p.vk - keep) * 8);
+                                asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(slot_at(i) + (b * p.vk + keep) * 128 + rest * 16), "r"(0) : "memory");
+                            }
+                        }
+                        fence_proxy_async();
+                        __syncwarp();
+                        if (alive && lane == 0) mbar_arrive(v_clean);
+                        ++cleaned;
+                    };
+                    keys(w.kb);
+                    if (alive && pieces > 0) alive = __all_sync(0xFFFFFFFFu, mbar_wait(q_empty, (pieces - 1) & 1u, ab, p.err));
+                    if (alive && lane == 0) {
+                        mbar_arrive_tx(q_full, STREAMS * p.dk * p.rt * p.R * 128);
+                        for (uint32_t q = 0; q < STREAMS; ++q)
+                            for (uint32_t b = 0; b < p.dk; ++b)
+                                tensor_copy_4d(base + (q * p.dk + b) * SLOT, &map_q, b * 64, w.g * p.R, w.t.row0 + q * p.rt, 0, q_full);
+                    }
+                    __syncwarp();
+                    ++pieces;
+                    for (uint32_t t = w.kb; t < w.ke && alive; ++t) {
+                        if (STREAMS == 1 && t + 1 < w.ke) keys(t + 1);  // in the order in which the issuer wants them
+                        if (alive) values(t);
+                        if (STREAMS == 2 && t + 1 < w.ke && alive) keys(t + 1);
+                    }
+                }
+                leave();
+            }
+            if (!alive) {  // copies still in flight land before the CTA may retire
+                *ab = 1;
+                for (uint32_t back = 1; back <= p.n_slots && back <= n; ++back)
+                    for (uint32_t i = 0; i < kSpinLimit; ++i)
+                        if (mbar_try_wait(full((n - back) % p.n_slots), ((n - back) / p.n_slots) & 1u)) break;
+                for (uint32_t i = 0; pieces > 0 && i < kSpinLimit; ++i)
+                    if (mbar_try_wait(q_full, (pieces - 1) & 1u)) break;
+            }
+        } else if (warp == ISSUER) {
+            if (lane == 0) {
+                const uint32_t id_s = idesc_bf16(128, TK), id_o = idesc_bf16(128, s.vdimp) | (1u << 16);  // V: MN-major
+                bool alive = true;
+                uint32_t n = 0, pieces = 0, cleaned = 0, count = 0;  // slots consumed; count: tiles of a stream so far
+                auto slot_full = [&](uint32_t at) { return mbar_wait(full(at % p.n_slots), (at / p.n_slots) & 1u, ab, p.err); };
+                // scores of a stream against the keys in the slots from `at` on; release: the slots are free behind them
+                auto scores = [&](uint32_t q, uint32_t col, uint32_t at, bool wait, bool release) {
+                    for (uint32_t b = 0; b < p.dk; ++b) {
+                        if (wait && !slot_full(at + b)) return false;
+                        tc_fence_after();
+                        const uint64_t qd = smem_desc_sw128(base + (q * p.dk + b) * SLOT), kd = smem_desc_sw128(slot_at((at + b) % p.n_slots));
+                        const uint32_t steps = min(4u, s.dimp / 16 - b * 4);
+                        for (uint32_t k = 0; k < steps; ++k) tc_mma_f16(tmem + col, qd + 2 * k, kd + 2 * k, id_s, (b | k) != 0 ? 1u : 0u);
+                        if (release) tc_commit(empty((at + b) % p.n_slots));
+                    }
+                    return true;
+                };
+                auto product = [&](uint32_t o_col, uint32_t p_col, uint32_t at, bool wait, bool release, bool first) {
+                    for (uint32_t v = 0; v < p.vs; ++v) {
+                        if (wait && !slot_full(at + v)) return false;
+                        tc_fence_after();
+                        const uint64_t vd = smem_desc_mn_sw128(slot_at((at + v) % p.n_slots), p.vk * 128);
+                        for (uint32_t k = 0; k < p.vk / 16; ++k)
+                            tc_mma_ts(tmem + o_col, tmem + p_col + (v * p.vk / 16 + k) * 8, vd + (2048 >> 4) * k, id_o,
+                                      first && (v | k) == 0 ? 0u : 1u);
+                        if (release) tc_commit(empty((at + v) % p.n_slots));
+                    }
+                    return true;
+                };
+                while (alive && next()) {
+                    if (w.kb < w.ke) {
+                        const uint32_t end = (uint32_t)(w.t.see0 + (int32_t)w.t.tokens - 1);
+                        alive = mbar_wait(q_full, pieces & 1u, ab, p.err);
+                        const uint32_t nt = w.ke - w.kb;
+                        if (STREAMS == 2) {
+                            uint32_t k_at = n;
+                            for (uint32_t q = 0; q < 2 && alive; ++q) {
+                                alive = scores(q, q * TK, k_at, q == 0, q == 1);
+                                if (alive) tc_commit(s_full(q));
+                            }
+                            for (uint32_t t = 0; t < nt && alive; ++t) {
+                                const uint32_t v_at = k_at + p.dk, k_next = v_at + p.vs;
+                                const bool dirty = (w.kb + t + 1) * TK > end, more = t + 1 < nt;
+                                for (uint32_t q = 0; q < 2 && alive; ++q) {
+                                    if (dirty && q == 0) alive = mbar_wait(v_clean, cleaned++ & 1u, ab, p.err);
+                                    alive = alive && mbar_wait(p_full(q), (count + t) & 1u, ab, p.err);
+                                    if (alive && t == 0 && pieces > 0) alive = mbar_wait(o_free(q), (pieces - 1) & 1u, ab, p.err);
+                                    alive = alive && product(256 + q * 128, q * TK, v_at, q == 0, q == 1, t == 0);
+                                    if (!alive) break;
+                                    if (more) {
+                                        alive = scores(q, q * TK, k_next, q == 0, q == 1);
+                                        if (alive) tc_commit(s_full(q));
+                                        if (t + 2 == nt && q == 1) tc_commit(q_empty);
+                                    } else {
+                                        tc_commit(o_full(q));
+                                    }
+                                }
+                                k_at = k_next;
+                            }
+                            if (nt == 1 && alive) tc_commit(q_empty);
+                            n += nt * (p.dk + p.vs);
+                            count += nt;
+                        } else {
+                            alive = alive && scores(0, (count & 1u) * TK, n, true, true);
+                            n += p.dk;
+                            if (alive) {
+                                tc_commit(s_full(count & 1u));
+                                if (nt == 1) tc_commit(q_empty);
+                            }
+                            for (uint32_t t = 0; t < nt && alive; ++t) {
+                                const uint32_t b = (count + t) & 1u, use = (count + t) >> 1;
+                                if (t + 1 < nt) {
+                                    alive = scores(0, (b ^ 1u) * TK, n, true, true);
+                                    n += p.dk;
+                                    if (!alive) break;
+                                    tc_commit(s_full(b ^ 1u));
+                                    if (t + 2 == nt) tc_commit(q_empty);
+                                }
+                                if ((w.kb + t + 1) * TK > end) alive = mbar_wait(v_clean, cleaned++ & 1u, ab, p.err);
+                                alive = alive && mbar_wait(p_full(b), use & 1u, ab, p.err);
+                                if (alive && t == 0 && pieces > 0) alive = mbar_wait(o_free(0), (pieces - 1) & 1u, ab, p.err);
+                                alive = alive && product(256, b * TK, n, true, true, t == 0);
+                                n += p.vs;
+                                if (!alive) break;
+                                tc_commit(pv_done(b));
+                                if (t + 1 == nt) tc_commit(o_full(0));
+                            }
+                            count += nt;
+                        }
+                        ++pieces;
+                    }
+                    leave();
+                }
+                if (!alive) *ab = 1;
+            }
+            __syncwarp();
+        }
+    } else {
+        split_registers<STREAMS>(true);
+        const uint32_t q = warp >> 2, m = tid & 127, lanes = ((warp & 3) * 32u) << 16;
+        const uint32_t o_col = 256 + q * 128;
+        uint32_t count = 0, pieces = 0;
+        bool alive = true;
+        const float scale = p.scale2 > 0.0f ? p.scale2 : 1.0f;
+        while (alive && next()) {
+            const uint32_t token = q * p.rt + m / p.R, head = w.g * p.R + m % p.R;
+            const bool real = m < p.rt * p.R && token < w.t.tokens;
+            const int32_t see = real ? w.t.see0 + (int32_t)token : 0;
+            float mx_run = -INFINITY, l = 0.0f;
+            for (uint32_t t = w.kb; t < w.ke; ++t, ++count) {
+                const uint32_t b = STREAMS == 2 ? q : count & 1u, use = STREAMS == 2 ? count : count >> 1;
+                const uint32_t s_col = tmem + lanes + b * TK;
+                alive = __all_sync(0xFFFFFFFFu, mbar_wait(s_full(b), use & 1u, ab, p.err));
+                if (!alive) break;
+                tc_fence_after();
+                uint32_t sv[4][32];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) tc_ld32(s_col + i * 32, sv[i]);
+                tc_wait_ld();
+                if (p.scale2 <= 0.0f) {  // a negative scale turns the order round
+#pragma unroll
+                    for (int i = 0; i < 128; ++i) sv[i >> 5][i & 31] = __float_as_uint(__uint_as_float(sv[i >> 5][i & 31]) * p.scale2);
+                }
+                if (w.t.see0 < (int32_t)((t + 1) * TK)) {  // some row does not see all of the tile
+                    const int lim = see - (int)(t * TK);
+#pragma unroll
+                    for (int i = 0; i < 128; ++i)
+                        if (i >= lim) sv[i >> 5][i & 31] = 0xFF800000u;
+                }
+                float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int i = 0; i < 128; ++i) mx4[i & 3] = fmaxf(mx4[i & 3], __uint_as_float(sv[i >> 5][i & 31]));
+                // what lies in the tile behind the rows has no say in when the others are rescaled
+                const float mx = real ? fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * scale : -INFINITY;
+                if (t == w.kb) {
+                    mx_run = mx;
+                } else if (__any_sync(0xFFFFFFFFu, mx - mx_run > kRaise)) {
+                    const float to = fmaxf(mx_run, mx), f = mx_run == -INFINITY ? 1.0f : ex2(mx_run - to);
+                    if (STREAMS == 1) {  // O holds the tiles ahead of this one (with two streams the scores were issued behind it)
+                        alive = __all_sync(0xFFFFFFFFu, mbar_wait(pv_done((count - 1) & 1u), ((count - 1) >> 1) & 1u, ab, p.err));
+                        if (!alive) break;
+                        tc_fence_after();
+                    }
+#pragma unroll 1
+                    for (uint32_t col = 0; col < s.vdimp; col += 32) {
+                        uint32_t o[32];
+                        tc_ld32(tmem + lanes + o_col + col, o);
+                        tc_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                        tc_st32(tmem + lanes + o_col + col, o);
+                    }
+                    l *= f;
+                    mx_run = to;
+                }
+                const float shift = mx_run == -INFINITY ? 0.0f : mx_run;
+                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t pw[32];
+#pragma unroll
+                    for (int i = 0; i < 64; i += 2) {
+                        const int at = h * 64 + i;
+                        const float x = ex2(fmaf(__uint_as_float(sv[at >> 5][at & 31]), scale, -shift));
+                        const float y = ex2(fmaf(__uint_as_float(sv[at >> 5][(at & 31) + 1]), scale, -shift));
+                        pw[i >> 1] = pack2(x, y);
+                        sum[i & 2] += x;
+                        sum[(i & 2) + 1] += y;
+                    }
+                    tc_st32(s_col + h * 32, pw);
+                }
+                tc_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_full(b));
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            }
+            if (!alive) break;
+            if (w.kb < w.ke) {
+                alive = __all_sync(0xFFFFFFFFu, mbar_wait(o_full(STREAMS == 2 ? q : 0), pieces & 1u, ab, p.err));
+                if (!alive) break;
+                tc_fence_after();
+                ++pieces;
+            }
+            if (w.whole) {
+                bf16* row = static_cast<bf16*>(a.out) + (size_t)(w.t.row0 + token) * a.out_pitch;
+                bf16* out = row + (size_t)head * s.vdim;
+                const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+                const bool wide = (((uintptr_t)out) & 15u) == 0;
+#pragma unroll 1
+                for (uint32_t col = 0; col < s.vdim; col += 32) {
+                    uint32_t o[32];
+                    if (w.kb < w.ke) {
+                        tc_ld32(tmem + lanes + o_col + col, o);
+                        tc_wait_ld();
+                    }
+                    float x[32];
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) x[i] = l > 0.0f ? __uint_as_float(o[i]) * inv : 0.0f;
+                    if (real && wide && col + 32 <= s.vdim) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            reinterpret_cast<uint4*>(out + col)[i] = make_uint4(pack2(x[8 * i], x[8 * i + 1]), pack2(x[8 * i + 2], x[8 * i + 3]),
+                                                                                pack2(x[8 * i + 4], x[8 * i + 5]), pack2(x[8 * i + 6], x[8 * i + 7]));
+                    } else if (real) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (col + i < s.vdim) out[col + i] = __float2bfloat16_rn(x[i]);
+                    }
+                    __syncwarp();
+                }
+                if (real && head == 0)  // columns beyond the heads
+                    for (uint32_t i = s.heads * s.vdim; i < a.out_pitch; ++i) row[i] = __float2bfloat16_rn(0.0f);
+            } else {  // [vdimp + 2][rows]: values, maximum, sum; a tile's first piece goes to the second slot of its part
+                float* part = p.w.partial + (size_t)(2 * c + (w.kb == 0 ? 1 : 0)) * (s.vdimp + 2) * (STREAMS * 128) + tid;
+#pragma unroll 1
+                for (uint32_t col = 0; col < s.vdimp; col += 32) {
+                    uint32_t o[32];
+                    tc_ld32(tmem + lanes + o_col + col, o);
+                    tc_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        if (col + i < s.vdimp) part[(size_t)(col + i) * (STREAMS * 128)] = __uint_as_float(o[i]);
+                }
+                part[(size_t)s.vdimp * (STREAMS * 128)] = mx_run;
+                part[(size_t)(s.vdimp + 1) * (STREAMS * 128)] = l;
+            }
+            if (w.kb < w.ke) {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(o_free(q));
+            }
+            leave();
+        }
+        if (!alive) *ab = 1;
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (warp == ISSUER) {
+        if (abort_flag && lane == 0) {  // instructions in flight get a bounded chance to finish (gemm_bf16.cu)
+            mbar_init(v_clean, 1);
+            tc_commit(v_clean);
+            for (uint32_t i = 0; i < kSpinLimit; ++i)
+                if (mbar_try_wait(v_clean, 0)) break;
+        }
+        __syncwarp();
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    }
+}
+
+// The pieces of a tile, in the order of its keys: a block for 32 rows of the tile that begins in part blockIdx.x; a lane per row, eight
+// columns per warp and turn.
+template <int STREAMS>
+__global__ void __launch_bounds__(128)
+ragged_join_kernel(const __grid_constant__ TcParams p) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const RaggedArgs& a = p.a;
+    const GqaShape& s = a.s;
+    const uint32_t c = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.y * 32 + lane;
+    if (c >= p.w.head[0]) return;
+    const SplitRec sp = p.w.splits[c];
+    if (sp.tile == ~0u) return;
+    const TileRec t = p.w.tiles[sp.tile];
+    const uint32_t m = row & 127, token = (row >> 7) * p.rt + m / p.R, head = sp.g * p.R + m % p.R;
+    if (m >= p.rt * p.R || token >= t.tokens) return;
+    constexpr uint32_t ROWS = STREAMS * 128;
+    const size_t size = (size_t)(s.vdimp + 2) * ROWS;
+    auto piece = [&](uint32_t i) { return p.w.partial + (size_t)(i == c ? 2 * c + 1 : 2 * i) * size + row; };
+    float mx = -INFINITY, sum = 0.0f;
+    for (uint32_t i = c; i <= sp.last; ++i) mx = fmaxf(mx, piece(i)[(size_t)s.vdimp * ROWS]);
+    const float shift = mx == -INFINITY ? 0.0f : mx;
+    for (uint32_t i = c; i <= sp.last; ++i)
+        sum += exp2f(piece(i)[(size_t)s.vdimp * ROWS] - shift) * piece(i)[(size_t)(s.vdimp + 1) * ROWS];
+    const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+    bf16* out = static_cast<bf16*>(a.out) + (size_t)(t.row0 + token) * a.out_pitch;
+    for (uint32_t col = warp * 8; col < s.vdimp; col += 32) {
+        float acc[8] = {};
+        for (uint32_t i = c; i <= sp.last; ++i) {
+            const float* x = piece(i);
+            const float f = exp2f(x[(size_t)s.vdimp * ROWS] - shift);
+            if (f == 0.0f) continue;  // a piece of which the row sees nothing
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc[e] = fmaf(f, x[(size_t)(col + e) * ROWS], acc[e]);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (col + e < s.vdim) out[(size_t)head * s.vdim + col + e] = __float2bfloat16_rn(acc[e] * inv);
+    }
+    if (head == 0)
+        for (uint32_t i = s.heads * s.vdim + warp; i < a.out_pitch; i += 4) out[i] = __float2bfloat16_rn(0.0f);
+}
+
+int done(cudaError_t e) { return e == cudaSuccess ? ZQ_OK : cuda_fail(e); }
+
+int streams_of(const GqaShape& s) { return s.dimp <= 128 && s.vdimp <= 128 ? 2 : 1; }
+
+TcParams params_of(const RaggedArgs& a, size_t& bytes) {
+    TcParams p{};
+    const GqaShape& s = a.s;
+    const uint32_t streams = streams_of(s);
+    p.a = a;
+    p.R = s.heads / s.kv_heads;
+    p.rt = 128 / p.R;
+    p.scale2 = a.scale * kLog2e;
+    p.dk = (s.dimp + 63) / 64;
+    p.dv = (s.vdimp + 63) / 64;
+    p.vk = p.dv == 1 ? 128 : p.dv == 2 ? 64 : 32;
+    p.vs = TK / p.vk;
+    const uint32_t page = a.lens ? 1u << a.shift : TK;
+    p.kbox = page < TK ? page : TK;
+    p.vbox = page < p.vk ? page : p.vk;
+    p.slots_at = streams * p.dk * SLOT;
+    p.n_slots = (225 * 1024 - p.slots_at) / SLOT;
+    if (p.n_slots > kMaxSlots) p.n_slots = kMaxSlots;
+    p.max_parts = sm_count() < (int)kMaxParts ? sm_count() : kMaxParts;
+    const uint32_t tokens = streams * p.rt;
+    const size_t tiles = (size_t)a.rows / tokens + (a.requests < a.rows ? a.requests : a.rows) + 1;
+    p.max_tiles = (uint32_t)tiles;
+    char* at = static_cast<char*>(a.work);
+    auto take = [&](size_t n) {
+        char* r = at;
+        at += (n + 255) / 256 * 256;
+        return r;
+    };
+    p.w.head = reinterpret_cast<uint32_t*>(take(256));
+    p.w.parts = reinterpret_cast<PartRec*>(take(p.max_parts * sizeof(PartRec)));
+    p.w.splits = reinterpret_cast<SplitRec*>(take(p.max_parts * sizeof(SplitRec)));
+    p.w.tiles = reinterpret_cast<TileRec*>(take(tiles * sizeof(TileRec)));
+    p.w.partial = reinterpret_cast<float*>(take((size_t)p.max_parts * 2 * (s.vdimp + 2) * streams * 128 * sizeof(float)));
+    bytes = at - static_cast<char*>(a.work);
+    return p;
+}
+
+// Map over [outer][rows][heads][width] bf16: copies of `box` rows of 64 columns of `box_heads` heads, zeros beyond the edges.
+int map_4d(const void* base, uint64_t width, uint64_t heads, uint64_t rows, uint64_t outer, uint64_t ld, uint32_t box_heads, uint32_t box,
+           CUtensorMap* out) {
+    typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static EncodeFn encode = nullptr;
+    if (!encode) {
+        void* fn = nullptr;
+        cudaDriverEntryPointQueryResult qres;
+        ZQ_CUDA(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &qres));
+        if (!fn || qres != cudaDriverEntryPointSuccess) return ZQ_ERR_UNSUPPORTED;
+        encode = reinterpret_cast<EncodeFn>(fn);
+    }
+    const cuuint64_t dims[4] = {width, heads, rows, outer};
+    const cuuint64_t strides[3] = {width * 2, ld * 2, ld * 2 * rows};
+    const cuuint32_t boxes[4] = {64, box_heads, box, 1}, elem[4] = {1, 1, 1, 1};
+    const CUresult r = encode(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, boxes, elem,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? ZQ_OK : ZQ_ERR_UNSUPPORTED;
+}
+
+template <int STREAMS>
+int launch(TcParams& p, cudaStream_t st) {
+    const RaggedArgs& a = p.a;
+    const GqaShape& s = a.s;
+    CUtensorMap mq, mk, mv;
+    const uint64_t rows = a.lens ? 1ull << a.shift : a.rows, outer = a.lens ? a.pages : 1;
+    int rc = map_4d(a.q, s.dimp, s.heads, a.rows, 1, a.q_ld, p.R, p.rt, &mq);
+    if (rc == ZQ_OK) rc = map_4d(a.k, s.dimp, s.kv_heads, rows, outer, a.k_ld, 1, p.kbox, &mk);
+    if (rc == ZQ_OK) rc = map_4d(a.v, s.vdimp, s.kv_heads, rows, outer, a.v_ld, 1, p.vbox, &mv);
+    if (rc == ZQ_OK) rc = device_error_word(&p.err);
+    if (rc != ZQ_OK) return rc;
+    const uint32_t smem = p.slots_at + p.n_slots * SLOT + 1024;
+    ZQ_CUDA(cudaFuncSetAttribute(ragged_tc_kernel<STREAMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024));
+    rc = done(launch_pdl(ragged_prep_kernel, dim3(1), dim3(kPrepThreads), 0, st, p, STREAMS * p.rt));
+    if (rc == ZQ_OK) rc = done(launch_pdl(ragged_tc_kernel<STREAMS>, dim3(p.max_parts), dim3(tc_threads(STREAMS)), smem, st, mq, mk, mv, p));
+    if (rc == ZQ_OK) rc = done(launch_pdl(ragged_join_kernel<STREAMS>, dim3(p.max_parts, STREAMS * 4), dim3(128), 0, st, p));
+    return rc;
+}
+
+}  // namespace
+
+bool ragged_tc_takes(const RaggedArgs& a) { return a.s.dimp <= 256 && a.s.vdimp <= 256 && a.s.heads / a.s.kv_heads <= 128; }
+
+size_t ragged_tc_work_bytes(const RaggedArgs& a) {
+    size_t bytes;
+    params_of(a, bytes);
+    return bytes;
+}
+
+int launch_ragged_tc(const RaggedArgs& a, cudaStream_t st) {
+    size_t bytes;
+    TcParams p = params_of(a, bytes);
+    return streams_of(a.s) == 2 ? launch<2>(p, st) : launch<1>(p, st);
+}
+
+}  // namespace zq
