@@ -203,13 +203,37 @@ __device__ __forceinline__ void tc_st32(uint32_t taddr, const uint32_t* r) {
         : "memory");
 }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-// A operand from tensor memory: 128 lanes, two bf16 a column
-__device__ __forceinline__ void tc_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+// MMAs and commits of one lane (`lead`) of a warp that stays together: with its operands in uniform registers an MMA issues in a
+// few cycles, in a branch of one lane it takes over a hundred (each operand is moved to a uniform register again).
+__device__ __forceinline__ uint32_t elect_lane() {
+    uint32_t lead;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(lead));
+    return lead;
+}
+__device__ __forceinline__ void mma_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate, uint32_t lead) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
+        "{\n\t.reg .pred p, e;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-        ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        "setp.ne.b32 e, %5, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(lead)
+        : "memory");
+}
+// A operand from tensor memory: 128 lanes, two bf16 a column
+__device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate, uint32_t lead) {
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "setp.ne.b32 e, %5, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(lead)
+        : "memory");
+}
+__device__ __forceinline__ void commit(uint32_t bar, uint32_t lead) {
+    asm volatile(
+        "{\n\t.reg .pred e;\n\t"
+        "setp.ne.b32 e, %1, 0;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(lead)
         : "memory");
 }
 // Descriptor of a [keys][64 values] tile read with the values as the operand's rows (MN-major, 128-byte swizzle): 64-value blocks
@@ -439,92 +463,113 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                     if (mbar_try_wait(q_full, (pieces - 1) & 1u)) break;
             }
         } else if (warp == ISSUER) {
-            if (lane == 0) {
+            {
+                const uint32_t lead = elect_lane(), tm = __shfl_sync(0xFFFFFFFFu, tmem, 0);
+                auto wait_for = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, ab, p.err)) != 0; };
                 const uint32_t id_s = idesc_bf16(128, TK), id_o = idesc_bf16(128, s.vdimp) | (1u << 16);  // V: MN-major
                 bool alive = true;
-                uint32_t n = 0, pieces = 0, cleaned = 0, count = 0;  // slots consumed; count: tiles of a stream so far
-                auto slot_full = [&](uint32_t at) { return mbar_wait(full(at % p.n_slots), (at / p.n_slots) & 1u, ab, p.err); };
-                // scores of a stream against the keys in the slots from `at` on; release: the slots are free behind them
-                auto scores = [&](uint32_t q, uint32_t col, uint32_t at, bool wait, bool release) {
-                    for (uint32_t b = 0; b < p.dk; ++b) {
-                        if (wait && !slot_full(at + b)) return false;
+                uint32_t pieces = 0, cleaned = 0, count = 0;  // count: tiles of a stream so far
+                uint32_t slot = 0, turn = 0;                  // of the next keys or values; turn: parity of the ring's rounds
+                const uint64_t q_desc = smem_desc_sw128(base), k_desc = smem_desc_sw128(slot_at(0)),
+                               v_desc = smem_desc_mn_sw128(slot_at(0), p.vk * 128);
+                constexpr uint64_t kSlotDesc = SLOT >> 4;
+                const uint32_t steps_last = s.dimp / 16 - (p.dk - 1) * 4;
+                auto after = [&](uint32_t& at, uint32_t& round) {
+                    if (++at == p.n_slots) {
+                        at = 0;
+                        round ^= 1u;
+                    }
+                };
+                // Scores of a stream against the keys in the slots from (at, round) on; release: the slots are free behind them.
+                auto scores = [&](uint32_t q, uint32_t col, uint32_t& at, uint32_t& round, bool wait, bool release) {
+                    uint64_t qd = q_desc + q * p.dk * kSlotDesc;
+                    for (uint32_t b = 0; b < p.dk; ++b, qd += kSlotDesc) {
+                        if (wait && !wait_for(full(at), round)) return false;
                         tc_fence_after();
-                        const uint64_t qd = smem_desc_sw128(base + (q * p.dk + b) * SLOT), kd = smem_desc_sw128(slot_at((at + b) % p.n_slots));
-                        const uint32_t steps = min(4u, s.dimp / 16 - b * 4);
-                        for (uint32_t k = 0; k < steps; ++k) tc_mma_f16(tmem + col, qd + 2 * k, kd + 2 * k, id_s, (b | k) != 0 ? 1u : 0u);
-                        if (release) tc_commit(empty((at + b) % p.n_slots));
+                        const uint64_t kd = k_desc + at * kSlotDesc;
+                        const uint32_t steps = b + 1 < p.dk ? 4 : steps_last;
+                        if (steps == 4) {
+#pragma unroll
+                            for (uint32_t k = 0; k < 4; ++k) mma_ss(tm + col, qd + 2 * k, kd + 2 * k, id_s, (b | k) != 0 ? 1u : 0u, lead);
+                        } else {
+                            for (uint32_t k = 0; k < steps; ++k) mma_ss(tm + col, qd + 2 * k, kd + 2 * k, id_s, (b | k) != 0 ? 1u : 0u, lead);
+                        }
+                        if (release) commit(empty(at), lead);
+                        after(at, round);
                     }
                     return true;
                 };
-                auto product = [&](uint32_t o_col, uint32_t p_col, uint32_t at, bool wait, bool release, bool first) {
+                auto product = [&](uint32_t o_col, uint32_t p_col, uint32_t& at, uint32_t& round, bool wait, bool release, bool first) {
+                    uint32_t pa = tm + p_col, more = first ? 0u : 1u;
                     for (uint32_t v = 0; v < p.vs; ++v) {
-                        if (wait && !slot_full(at + v)) return false;
+                        if (wait && !wait_for(full(at), round)) return false;
                         tc_fence_after();
-                        const uint64_t vd = smem_desc_mn_sw128(slot_at((at + v) % p.n_slots), p.vk * 128);
-                        for (uint32_t k = 0; k < p.vk / 16; ++k)
-                            tc_mma_ts(tmem + o_col, tmem + p_col + (v * p.vk / 16 + k) * 8, vd + (2048 >> 4) * k, id_o,
-                                      first && (v | k) == 0 ? 0u : 1u);
-                        if (release) tc_commit(empty((at + v) % p.n_slots));
+                        uint64_t vd = v_desc + at * kSlotDesc;
+                        for (uint32_t k = 0; k < p.vk; k += 32) {
+#pragma unroll
+                            for (uint32_t e = 0; e < 2; ++e, pa += 8, vd += 2048 >> 4, more = 1) mma_ts(tm + o_col, pa, vd, id_o, more, lead);
+                        }
+                        if (release) commit(empty(at), lead);
+                        after(at, round);
                     }
                     return true;
                 };
                 while (alive && next()) {
                     if (w.kb < w.ke) {
-                        const uint32_t end = (uint32_t)(w.t.see0 + (int32_t)w.t.tokens - 1);
-                        alive = mbar_wait(q_full, pieces & 1u, ab, p.err);
-                        const uint32_t nt = w.ke - w.kb;
+                        const uint32_t end = __shfl_sync(0xFFFFFFFFu, (uint32_t)(w.t.see0 + (int32_t)w.t.tokens - 1), 0);
+                        const uint32_t kb = __shfl_sync(0xFFFFFFFFu, w.kb, 0);
+                        alive = wait_for(q_full, pieces & 1u);
+                        const uint32_t nt = __shfl_sync(0xFFFFFFFFu, w.ke - w.kb, 0);
                         if (STREAMS == 2) {
-                            uint32_t k_at = n;
                             for (uint32_t q = 0; q < 2 && alive; ++q) {
-                                alive = scores(q, q * TK, k_at, q == 0, q == 1);
-                                if (alive) tc_commit(s_full(q));
+                                uint32_t at = slot, round = turn;
+                                alive = scores(q, q * TK, at, round, q == 0, q == 1);
+                                if (alive) commit(s_full(q), lead);
+                                if (q == 1) slot = at, turn = round;
                             }
+                            if (nt == 1 && alive) commit(q_empty, lead);
                             for (uint32_t t = 0; t < nt && alive; ++t) {
-                                const uint32_t v_at = k_at + p.dk, k_next = v_at + p.vs;
-                                const bool dirty = (w.kb + t + 1) * TK > end, more = t + 1 < nt;
+                                const bool more = t + 1 < nt;
+                                if ((kb + t + 1) * TK > end) alive = wait_for(v_clean, cleaned++ & 1u);
+                                uint32_t at = slot, round = turn;
                                 for (uint32_t q = 0; q < 2 && alive; ++q) {
-                                    if (dirty && q == 0) alive = mbar_wait(v_clean, cleaned++ & 1u, ab, p.err);
-                                    alive = alive && mbar_wait(p_full(q), (count + t) & 1u, ab, p.err);
-                                    if (alive && t == 0 && pieces > 0) alive = mbar_wait(o_free(q), (pieces - 1) & 1u, ab, p.err);
-                                    alive = alive && product(256 + q * 128, q * TK, v_at, q == 0, q == 1, t == 0);
+                                    alive = wait_for(p_full(q), (count + t) & 1u);
+                                    if (alive && t == 0 && pieces > 0) alive = wait_for(o_free(q), (pieces - 1) & 1u);
+                                    at = slot, round = turn;
+                                    alive = alive && product(256 + q * 128, q * TK, at, round, q == 0, q == 1, t == 0);
                                     if (!alive) break;
                                     if (more) {
-                                        alive = scores(q, q * TK, k_next, q == 0, q == 1);
-                                        if (alive) tc_commit(s_full(q));
-                                        if (t + 2 == nt && q == 1) tc_commit(q_empty);
+                                        alive = scores(q, q * TK, at, round, q == 0, q == 1);
+                                        if (alive) commit(s_full(q), lead);
+                                        if (t + 2 == nt && q == 1) commit(q_empty, lead);
                                     } else {
-                                        tc_commit(o_full(q));
+                                        commit(o_full(q), lead);
                                     }
                                 }
-                                k_at = k_next;
+                                slot = at, turn = round;
                             }
-                            if (nt == 1 && alive) tc_commit(q_empty);
-                            n += nt * (p.dk + p.vs);
                             count += nt;
                         } else {
-                            alive = alive && scores(0, (count & 1u) * TK, n, true, true);
-                            n += p.dk;
+                            alive = alive && scores(0, (count & 1u) * TK, slot, turn, true, true);
                             if (alive) {
-                                tc_commit(s_full(count & 1u));
-                                if (nt == 1) tc_commit(q_empty);
+                                commit(s_full(count & 1u), lead);
+                                if (nt == 1) commit(q_empty, lead);
                             }
                             for (uint32_t t = 0; t < nt && alive; ++t) {
                                 const uint32_t b = (count + t) & 1u, use = (count + t) >> 1;
                                 if (t + 1 < nt) {
-                                    alive = scores(0, (b ^ 1u) * TK, n, true, true);
-                                    n += p.dk;
+                                    alive = scores(0, (b ^ 1u) * TK, slot, turn, true, true);
                                     if (!alive) break;
-                                    tc_commit(s_full(b ^ 1u));
-                                    if (t + 2 == nt) tc_commit(q_empty);
+                                    commit(s_full(b ^ 1u), lead);
+                                    if (t + 2 == nt) commit(q_empty, lead);
                                 }
-                                if ((w.kb + t + 1) * TK > end) alive = mbar_wait(v_clean, cleaned++ & 1u, ab, p.err);
-                                alive = alive && mbar_wait(p_full(b), use & 1u, ab, p.err);
-                                if (alive && t == 0 && pieces > 0) alive = mbar_wait(o_free(0), (pieces - 1) & 1u, ab, p.err);
-                                alive = alive && product(256, b * TK, n, true, true, t == 0);
-                                n += p.vs;
+                                if ((kb + t + 1) * TK > end) alive = wait_for(v_clean, cleaned++ & 1u);
+                                alive = alive && wait_for(p_full(b), use & 1u);
+                                if (alive && t == 0 && pieces > 0) alive = wait_for(o_free(0), (pieces - 1) & 1u);
+                                alive = alive && product(256, b * TK, slot, turn, true, true, t == 0);
                                 if (!alive) break;
-                                tc_commit(pv_done(b));
-                                if (t + 1 == nt) tc_commit(o_full(0));
+                                commit(pv_done(b), lead);
+                                if (t + 1 == nt) commit(o_full(0), lead);
                             }
                             count += nt;
                         }
@@ -679,7 +724,8 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     tc_fence_before();
     __syncthreads();
     if (warp == ISSUER) {
-        if (abort_flag && lane == 0) {  // instructions in flight get a bounded chance to finish (gemm_bf16.cu)
+        const uint32_t lead = elect_lane();  // the lane that issued
+        if (abort_flag && lead) {  // instructions in flight get a bounded chance to finish (gemm_bf16.cu)
             mbar_init(v_clean, 1);
             tc_commit(v_clean);
             for (uint32_t i = 0; i < kSpinLimit; ++i)
