@@ -279,7 +279,8 @@ struct Walk {
     bool whole;
 };
 
-template <int STREAMS>
+// DK, DV: blocks of 64 dimensions of a key and of a value, full ones; 0: as the parameters say.
+template <int STREAMS, int DK, int DV>
 __global__ void __launch_bounds__(tc_threads(STREAMS), 1)
 ragged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                  const __grid_constant__ CUtensorMap map_v, const __grid_constant__ TcParams p) {
@@ -303,6 +304,7 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     auto full = [&](uint32_t i) { return bar32 + 8 * (13 + i); };
     auto empty = [&](uint32_t i) { return bar32 + 8 * (13 + kMaxSlots + i); };
     auto slot_at = [&](uint32_t i) { return base + p.slots_at + i * SLOT; };
+    const uint32_t dk = DK ? DK : p.dk, dv = DV ? DV : p.dv, vk = DV ? (DV == 1 ? 128 : DV == 2 ? 64 : 32) : p.vk, vs = TK / vk;
 
     if (tid == 0) {
         mbar_init(q_full, 1);
@@ -379,77 +381,83 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         split_registers<STREAMS>(false);
         if (warp == LOADER) {
             bool alive = true;
-            uint32_t n = 0, pieces = 0, cleaned = 0;  // slots asked for
+            uint32_t pieces = 0, slot = 0, turn = 1, n = 0;  // turn: parity that a slot's first use finds
+            // A slot's copies, a lane each: rows of `box`, blocks of 64 columns.
+            const uint32_t k_boxes = TK / p.kbox, v_per = p.vk / p.vbox, v_boxes = v_per * dv;
+            const uint32_t k_row = lane % k_boxes * p.kbox, v_block = lane / v_per, v_row = lane % v_per * p.vbox;
+            const uint32_t in_page = (1u << a.shift) - 1;
             auto enter = [&](uint32_t bytes) {  // the next slot, free
-                const uint32_t i = n % p.n_slots, use = n / p.n_slots;
-                if (use > 0) alive = alive && mbar_wait(empty(i), (use - 1) & 1u, ab, p.err);
-                alive = __all_sync(0xFFFFFFFFu, alive);
-                if (alive && lane == 0) mbar_arrive_tx(full(i), bytes);
+                alive = alive && __all_sync(0xFFFFFFFFu, mbar_wait(empty(slot), turn, ab, p.err));
+                if (alive && lane == 0) mbar_arrive_tx(full(slot), bytes);
                 __syncwarp();
-                if (alive) ++n;
-                return i;
             };
-            // `rows` rows from key k0 on, `blocks` blocks of 64 columns (from block b0) to dst: copies of `box` rows, a lane each
-            auto copy = [&](const CUtensorMap* map, uint32_t dst, uint32_t k0, uint32_t rows, uint32_t box, uint32_t b0, uint32_t blocks, uint32_t bar) {
-                const uint32_t per = rows / box;
-                for (uint32_t i = lane; i < per * blocks; i += 32) {
-                    const uint32_t b = i / per, r = i % per * box, key = k0 + r;
-                    uint32_t y = w.t.first_row + key, z = 0;
-                    if (a.lens) {
-                        const uint32_t j = key >> a.shift;
-                        const uint32_t page = j < a.table_ld ? (uint32_t)__ldg(a.tables + (size_t)w.t.request * a.table_ld + j) : a.pages;
-                        z = page < a.pages ? page : a.pages;
-                        y = key & ((1u << a.shift) - 1);
-                    }
-                    tensor_copy_4d(dst + (b * rows + r) * 128, map, (b0 + b) * 64, w.g, y, z, bar);
+            auto after = [&]() {
+                if (alive) ++n;
+                if (++slot == p.n_slots) {
+                    slot = 0;
+                    turn ^= 1u;
                 }
+            };
+            // Pages of a tile's keys, 16 keys a lane; looked up a tile ahead. What is no page is one behind the last: zeros.
+            auto look_up = [&](uint32_t t) {
+                const uint32_t j = (t * TK + (lane & 7) * 16) >> a.shift;
+                const uint32_t page = a.lens && j < a.table_ld ? (uint32_t)__ldg(a.tables + (size_t)w.t.request * a.table_ld + j) : a.pages;
+                return min(page, a.pages);
+            };
+            auto copy = [&](const CUtensorMap* map, uint32_t dst, uint32_t key, uint32_t page, uint32_t col) {
+                tensor_copy_4d(dst, map, col, w.g, a.lens ? key & in_page : w.t.first_row + key, a.lens ? page : 0, full(slot));
             };
             asm volatile("fence.proxy.async.global;" ::: "memory");
             while (alive && next()) {
                 if (w.kb < w.ke) {
                     const uint32_t end = (uint32_t)(w.t.see0 + (int32_t)w.t.tokens - 1);  // keys that the tile sees
-                    auto keys = [&](uint32_t t) {
-                        for (uint32_t b = 0; b < p.dk && alive; ++b) {
-                            const uint32_t i = enter(SLOT);
-                            if (alive) copy(&map_k, slot_at(i), t * TK, TK, p.kbox, b, 1, full(i));
+                    uint32_t pages = look_up(w.kb), pages_after = 0;  // of the tile whose values, and of the one whose keys are next
+                    auto keys = [&](uint32_t t, uint32_t from) {
+                        const uint32_t page = __shfl_sync(0xFFFFFFFFu, from, k_row >> 4);
+                        for (uint32_t b = 0; b < dk && alive; ++b) {
+                            enter(SLOT);
+                            if (alive && lane < k_boxes) copy(&map_k, slot_at(slot) + k_row * 128, t * TK + k_row, page, b * 64);
+                            after();
                         }
                     };
-                    auto values = [&](uint32_t t) {
-                        uint32_t at[8];
-                        for (uint32_t v = 0; v < p.vs && alive; ++v) {
-                            at[v & 7] = enter(p.vk * p.dv * 128);
-                            if (alive) copy(&map_v, slot_at(at[v & 7]), t * TK + v * p.vk, p.vk, p.vbox, 0, p.dv, full(at[v & 7]));
-                        }
-                        if (!alive || (t + 1) * TK <= end) return;
-                        for (uint32_t v = 0; v < p.vs && alive; ++v) {  // what lies behind the last key is no value
-                            const uint32_t k0 = t * TK + v * p.vk, keep = k0 >= end ? 0 : min(end - k0, p.vk), i = at[v & 7];
-                            if (keep == p.vk) continue;
-                            alive = mbar_wait(full(i), ((n - p.vs + v) / p.n_slots) & 1u, ab, p.err);
-                            alive = __all_sync(0xFFFFFFFFu, alive);
-                            for (uint32_t e = lane; alive && e < (p.vk - keep) * 8 * p.dv; e += 32) {
-                                const uint32_t b = e / ((p.vk - keep) * 8), rest = e % ((p.vk - keep) * 8);
-                                asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(slot_at(i) + (b * p.vk + keep) * 128 + rest * 16), "r"(0) : "memory");
+                    auto values = [&](uint32_t t, uint32_t from) {
+                        const bool dirty = (t + 1) * TK > end;
+                        for (uint32_t v = 0; v < vs && alive; ++v) {
+                            const uint32_t page = __shfl_sync(0xFFFFFFFFu, from, (v * vk + v_row) >> 4), k0 = t * TK + v * vk;
+                            enter(vk * dv * 128);
+                            if (alive && lane < v_boxes) copy(&map_v, slot_at(slot) + (v_block * vk + v_row) * 128, k0 + v_row, page, v_block * 64);
+                            if (alive && dirty) {  // what lies behind the last key is no value
+                                const uint32_t keep = k0 >= end ? 0 : min(end - k0, vk), chunks = (vk - keep) * 8;
+                                alive = __all_sync(0xFFFFFFFFu, mbar_wait(full(slot), turn ^ 1u, ab, p.err));
+                                for (uint32_t b = 0; b < dv && alive; ++b)
+                                    for (uint32_t e = lane; e < chunks; e += 32)
+                                        asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(slot_at(slot) + (b * vk + keep) * 128 + e * 16), "r"(0)
+                                                     : "memory");
                             }
+                            after();
                         }
-                        fence_proxy_async();
-                        __syncwarp();
-                        if (alive && lane == 0) mbar_arrive(v_clean);
-                        ++cleaned;
+                        if (dirty) {
+                            fence_proxy_async();
+                            __syncwarp();
+                            if (alive && lane == 0) mbar_arrive(v_clean);
+                        }
                     };
-                    keys(w.kb);
+                    keys(w.kb, pages);
                     if (alive && pieces > 0) alive = __all_sync(0xFFFFFFFFu, mbar_wait(q_empty, (pieces - 1) & 1u, ab, p.err));
                     if (alive && lane == 0) {
-                        mbar_arrive_tx(q_full, STREAMS * p.dk * p.rt * p.R * 128);
+                        mbar_arrive_tx(q_full, STREAMS * dk * p.rt * p.R * 128);
                         for (uint32_t q = 0; q < STREAMS; ++q)
-                            for (uint32_t b = 0; b < p.dk; ++b)
-                                tensor_copy_4d(base + (q * p.dk + b) * SLOT, &map_q, b * 64, w.g * p.R, w.t.row0 + q * p.rt, 0, q_full);
+                            for (uint32_t b = 0; b < dk; ++b)
+                                tensor_copy_4d(base + (q * dk + b) * SLOT, &map_q, b * 64, w.g * p.R, w.t.row0 + q * p.rt, 0, q_full);
                     }
                     __syncwarp();
-                    ++pieces;
+                    if (alive) ++pieces;
                     for (uint32_t t = w.kb; t < w.ke && alive; ++t) {
-                        if (STREAMS == 1 && t + 1 < w.ke) keys(t + 1);  // in the order in which the issuer wants them
-                        if (alive) values(t);
-                        if (STREAMS == 2 && t + 1 < w.ke && alive) keys(t + 1);
+                        if (t + 1 < w.ke) pages_after = look_up(t + 1);
+                        if (STREAMS == 1 && t + 1 < w.ke) keys(t + 1, pages_after);  // in the order in which the issuer wants them
+                        if (alive) values(t, pages);
+                        if (STREAMS == 2 && t + 1 < w.ke && alive) keys(t + 1, pages_after);
+                        pages = pages_after;
                     }
                 }
                 leave();
@@ -471,9 +479,9 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 uint32_t pieces = 0, cleaned = 0, count = 0;  // count: tiles of a stream so far
                 uint32_t slot = 0, turn = 0;                  // of the next keys or values; turn: parity of the ring's rounds
                 const uint64_t q_desc = smem_desc_sw128(base), k_desc = smem_desc_sw128(slot_at(0)),
-                               v_desc = smem_desc_mn_sw128(slot_at(0), p.vk * 128);
+                               v_desc = smem_desc_mn_sw128(slot_at(0), vk * 128);
                 constexpr uint64_t kSlotDesc = SLOT >> 4;
-                const uint32_t steps_last = s.dimp / 16 - (p.dk - 1) * 4;
+                const uint32_t steps_last = DK ? 4 : s.dimp / 16 - (dk - 1) * 4;
                 auto after = [&](uint32_t& at, uint32_t& round) {
                     if (++at == p.n_slots) {
                         at = 0;
@@ -482,12 +490,13 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 };
                 // Scores of a stream against the keys in the slots from (at, round) on; release: the slots are free behind them.
                 auto scores = [&](uint32_t q, uint32_t col, uint32_t& at, uint32_t& round, bool wait, bool release) {
-                    uint64_t qd = q_desc + q * p.dk * kSlotDesc;
-                    for (uint32_t b = 0; b < p.dk; ++b, qd += kSlotDesc) {
+                    uint64_t qd = q_desc + q * dk * kSlotDesc;
+#pragma unroll
+                    for (uint32_t b = 0; b < dk; ++b, qd += kSlotDesc) {
                         if (wait && !wait_for(full(at), round)) return false;
                         tc_fence_after();
                         const uint64_t kd = k_desc + at * kSlotDesc;
-                        const uint32_t steps = b + 1 < p.dk ? 4 : steps_last;
+                        const uint32_t steps = b + 1 < dk ? 4 : steps_last;
                         if (steps == 4) {
 #pragma unroll
                             for (uint32_t k = 0; k < 4; ++k) mma_ss(tm + col, qd + 2 * k, kd + 2 * k, id_s, (b | k) != 0 ? 1u : 0u, lead);
@@ -501,11 +510,13 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 };
                 auto product = [&](uint32_t o_col, uint32_t p_col, uint32_t& at, uint32_t& round, bool wait, bool release, bool first) {
                     uint32_t pa = tm + p_col, more = first ? 0u : 1u;
-                    for (uint32_t v = 0; v < p.vs; ++v) {
+#pragma unroll
+                    for (uint32_t v = 0; v < vs; ++v) {
                         if (wait && !wait_for(full(at), round)) return false;
                         tc_fence_after();
                         uint64_t vd = v_desc + at * kSlotDesc;
-                        for (uint32_t k = 0; k < p.vk; k += 32) {
+#pragma unroll
+                        for (uint32_t k = 0; k < vk; k += 32) {
 #pragma unroll
                             for (uint32_t e = 0; e < 2; ++e, pa += 8, vd += 2048 >> 4, more = 1) mma_ts(tm + o_col, pa, vd, id_o, more, lead);
                         }
@@ -844,7 +855,7 @@ int map_4d(const void* base, uint64_t width, uint64_t heads, uint64_t rows, uint
     return r == CUDA_SUCCESS ? ZQ_OK : ZQ_ERR_UNSUPPORTED;
 }
 
-template <int STREAMS>
+template <int STREAMS, int DK, int DV>
 int launch(TcParams& p, cudaStream_t st) {
     const RaggedArgs& a = p.a;
     const GqaShape& s = a.s;
@@ -856,9 +867,9 @@ int launch(TcParams& p, cudaStream_t st) {
     if (rc == ZQ_OK) rc = device_error_word(&p.err);
     if (rc != ZQ_OK) return rc;
     const uint32_t smem = p.slots_at + p.n_slots * SLOT + 1024;
-    ZQ_CUDA(cudaFuncSetAttribute(ragged_tc_kernel<STREAMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024));
+    ZQ_CUDA(cudaFuncSetAttribute(ragged_tc_kernel<STREAMS, DK, DV>, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024));
     rc = done(launch_pdl(ragged_prep_kernel, dim3(1), dim3(kPrepThreads), 0, st, p, STREAMS * p.rt));
-    if (rc == ZQ_OK) rc = done(launch_pdl(ragged_tc_kernel<STREAMS>, dim3(p.max_parts), dim3(tc_threads(STREAMS)), smem, st, mq, mk, mv, p));
+    if (rc == ZQ_OK) rc = done(launch_pdl(ragged_tc_kernel<STREAMS, DK, DV>, dim3(p.max_parts), dim3(tc_threads(STREAMS)), smem, st, mq, mk, mv, p));
     if (rc == ZQ_OK) rc = done(launch_pdl(ragged_join_kernel<STREAMS>, dim3(p.max_parts, STREAMS * 4), dim3(128), 0, st, p));
     return rc;
 }
@@ -876,7 +887,9 @@ size_t ragged_tc_work_bytes(const RaggedArgs& a) {
 int launch_ragged_tc(const RaggedArgs& a, cudaStream_t st) {
     size_t bytes;
     TcParams p = params_of(a, bytes);
-    return streams_of(a.s) == 2 ? launch<2>(p, st) : launch<1>(p, st);
+    const uint32_t d = a.s.dimp == a.s.vdimp ? a.s.dimp : 0;
+    if (streams_of(a.s) == 2) return d == 64 ? launch<2, 1, 1>(p, st) : d == 128 ? launch<2, 2, 2>(p, st) : launch<2, 0, 0>(p, st);
+    return d == 256 ? launch<1, 4, 4>(p, st) : launch<1, 0, 0>(p, st);
 }
 
 }  // namespace zq
