@@ -8,14 +8,15 @@
 //               of keys: MN-major).
 // Up to 128 dimensions two such tiles of rows (STREAMS = 2) take turns on one stream of keys: the tensor cores work on one while the
 // other's softmax runs. Beyond that O takes half of tensor memory; one tile, two buffers of scores.
-// Keys and values come through one ring of 16 KB slots: a slot holds 64 dimensions of 128 keys, or all dimensions of 128 / VS keys
-// as values, brought in by tensor copies of a page's rows (or 128 packed rows). Pages that do not exist are coordinates outside the
+// Keys and values come through one ring of slots (16 KB up to 64 dimensions, else 32 KB): a slot holds the keys of a tile, or 128 of
+// their dimensions, or the values of a tile, or of 64 keys, brought in by tensor copies of a page's rows (or 128 packed rows). Pages that do not exist are coordinates outside the
 // tensor: zeros. Values behind the last key that the tile sees are overwritten with zeros, whatever the page holds there.
 //
 // Work is cut evenly: the tiles' key tiles (and a constant per tile), one behind the other, are shared out in equal contiguous parts,
 // one per SM. What a part has of a tile that it does not cover alone goes to a slot of partial sums; a third kernel joins these.
-// Roles: warps 0-3 (and 4-7 with two streams) softmax and results; then a warp that issues copies, and one that issues MMAs and owns
-// the tensor memory. Every wait is bounded, as in gemm_bf16.cu.
+// Roles: warps 0-3 (and 4-7 with two streams) softmax and results; then a warp that issues copies, and one per stream that issues its
+// MMAs (what a warp does besides, waits above all, costs more than the MMAs: one warp for both streams made the period of two tiles
+// 4400 cycles, of which their products are 2048). The first of them owns the tensor memory. Every wait is bounded, as in gemm_bf16.cu.
 #include "paged.h"
 #include "tc_common.cuh"
 
@@ -23,11 +24,11 @@ namespace zq {
 namespace {
 
 constexpr uint32_t TK = 128;                // keys of a tile
-constexpr uint32_t SLOT = 128 * 128;        // bytes of 128 keys x 64 dimensions
+constexpr uint32_t ATOM = 128 * 128;        // bytes of 128 keys (or rows) x 64 dimensions
 constexpr uint32_t kMaxSlots = 12;
 constexpr uint32_t kMaxParts = 160;         // CTAs
 constexpr float kRaise = 8.0f;              // powers of two that the maximum may lag behind
-constexpr uint32_t kTileCost = 1;           // what a tile costs besides its keys, in key tiles
+constexpr uint32_t kTileCost = 2;           // what a tile costs besides its keys, in key tiles
 constexpr uint32_t kLeastPart = 3;          // key tiles that a CTA is started for
 constexpr uint32_t kPrepThreads = 1024;
 constexpr uint32_t kSearchTiles = 4096;     // tiles whose costs the search keeps in shared memory
@@ -60,7 +61,7 @@ struct TcParams {
     uint32_t max_parts, max_tiles;
     float scale2;
     uint32_t dk, dv;           // 64-wide blocks of a key / value row
-    uint32_t vs, vk;           // slots of a tile's values, keys of such a slot
+    uint32_t slot, vk;         // bytes of a slot; keys of a slot of values
     uint32_t kbox, vbox;       // rows of a copy
     uint32_t n_slots, slots_at;
     unsigned int* err;
@@ -92,6 +93,7 @@ __device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t* sums, uint6
 
 __global__ void __launch_bounds__(kPrepThreads)
 ragged_prep_kernel(const __grid_constant__ TcParams p, uint32_t tile_tokens) {
+    static_assert(kMaxParts < kPrepThreads, "a thread per boundary");
     __shared__ uint64_t sums[32];
     __shared__ uint32_t first[kPrepThreads + 1];
     __shared__ uint32_t rows_of[kPrepThreads];
@@ -157,7 +159,7 @@ ragged_prep_kernel(const __grid_constant__ TcParams p, uint32_t tile_tokens) {
     uint64_t G = U / (kLeastPart + kTileCost);
     G = G < 1 ? 1 : G > p.max_parts ? p.max_parts : G;
     if (tid == 0) p.w.head[0] = U ? (uint32_t)G : 0;
-    if (U == 0 || tid >= (uint32_t)G) return;
+    if (U == 0) return;
     auto find = [&](uint64_t u, uint32_t& tile, uint32_t& g, uint32_t& off, uint32_t& kt) {  // the tile of unit u
         uint32_t lo = 0, hi = n_tiles;
         while (hi - lo > 1) {
@@ -173,9 +175,23 @@ ragged_prep_kernel(const __grid_constant__ TcParams p, uint32_t tile_tokens) {
         off = (uint32_t)(rest % (kt + kTileCost));
         return u - off;  // its first unit
     };
-    const uint64_t b0 = U * tid / G, b1 = U * (tid + 1) / G;
-    PartRec part;
+    // Equal parts, but for boundaries close to a tile's, which are moved there: a tile cut in two has two sums to store and to join.
+    __shared__ uint64_t bound[kMaxParts + 1];
+    const uint32_t snap = (uint32_t)min((uint64_t)8, U / G / 12);
+    PartRec part{};
     uint32_t kt;
+    if (tid <= (uint32_t)G) {
+        uint64_t u = U * tid / G;
+        if (tid > 0 && tid < (uint32_t)G) {
+            const uint64_t begin = find(u, part.tile, part.g, part.off, kt);
+            if (part.off <= snap) u = begin;
+            else if (kt + kTileCost - part.off <= snap) u = begin + kt + kTileCost;
+        }
+        bound[tid] = u;
+    }
+    __syncthreads();
+    if (tid >= (uint32_t)G) return;
+    const uint64_t b0 = bound[tid], b1 = bound[tid + 1];
     find(b0, part.tile, part.g, part.off, kt);
     part.n_units = (uint32_t)(b1 - b0);
     p.w.parts[tid] = part;
@@ -183,9 +199,13 @@ ragged_prep_kernel(const __grid_constant__ TcParams p, uint32_t tile_tokens) {
     uint32_t tile, g, off;
     const uint64_t begin = find(b1 - 1, tile, g, off, kt);
     if (off + 1 < kt && begin >= b0) {
+        const uint64_t end = begin + kt - 1;  // its last key tile
+        uint32_t last = (uint32_t)(((end + 1) * G - 1) / U);
+        while (bound[last] > end) --last;
+        while (bound[last + 1] <= end) ++last;
         s.tile = tile;
         s.g = g;
-        s.last = (uint32_t)(((begin + kt) * G - 1) / U);  // the part of its last key tile
+        s.last = last;
     }
     p.w.splits[tid] = s;
 }
@@ -252,6 +272,38 @@ __device__ __forceinline__ void tensor_copy_4d(uint32_t dst, const CUtensorMap* 
 __device__ __forceinline__ void mbar_arrive_tx(uint32_t bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
+__device__ __forceinline__ bf16 half_of(uint32_t two, int high) {
+    const unsigned short bits = (unsigned short)(high ? two >> 16 : two & 0xFFFFu);
+    return *reinterpret_cast<const bf16*>(&bits);
+}
+__device__ __forceinline__ void store32(bf16* out, const uint32_t* v) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(out), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]),
+                 "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
+using pair = unsigned long long;  // two f32 of neighbouring registers
+__device__ __forceinline__ pair pair_of(uint32_t a, uint32_t b) {
+    pair r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(a), "r"(b));
+    return r;
+}
+__device__ __forceinline__ pair pair_of(float a, float b) { return pair_of(__float_as_uint(a), __float_as_uint(b)); }
+__device__ __forceinline__ void split(pair v, uint32_t& a, uint32_t& b) { asm("mov.b64 {%0, %1}, %2;" : "=r"(a), "=r"(b) : "l"(v)); }
+__device__ __forceinline__ pair fma2(pair a, pair b, pair c) {
+    pair r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ pair add2(pair a, pair b) {
+    pair r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -261,6 +313,27 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&v);
 }
+
+// 2^x of two numbers up to 2^16 by multiply-adds: x = j + f with j the nearest integer (by adding 1.5 x 2^23, which leaves j in the low
+// bits), 2^f on [-1/2, 1/2] by the cubic of least relative error (7.5e-5, a thirtieth of the rounding to bf16 that follows), j added to the
+// exponent. Below 2^-125 the result is 2^-125: a hidden key's weight, then, which no sum notices.
+__device__ __forceinline__ void exp2_pair(pair x, uint32_t& a, uint32_t& b) {
+    uint32_t u, v;
+    split(x, u, v);
+    x = pair_of(fmaxf(__uint_as_float(u), -125.0f), fmaxf(__uint_as_float(v), -125.0f));
+    const pair t = add2(x, pair_of(12582912.0f, 12582912.0f)), j = add2(t, pair_of(-12582912.0f, -12582912.0f));
+    const pair f = fma2(j, pair_of(-1.0f, -1.0f), x);
+    pair y = fma2(f, pair_of(0.05517167f, 0.05517167f), pair_of(0.24261113f, 0.24261113f));
+    y = fma2(y, f, pair_of(0.69326097f, 0.69326097f));
+    y = fma2(y, f, pair_of(0.99992806f, 0.99992806f));
+    split(y, a, b);
+    split(t, u, v);
+    a += u << 23;
+    b += v << 23;
+}
+// Pairs of eight whose exponentials are made that way: the special-function unit gives a warp's 32 in eight cycles, so 128 keys of a row
+// would take it as long as the tensor cores take for both products.
+__device__ __forceinline__ constexpr bool by_products(int pair_index) { return (pair_index & 7) == 2 || (pair_index & 7) == 5 || (pair_index & 7) == 7; }
 
 // Registers: whole groups of four warps may pass registers to one another, so two streams come with a third group. 384 threads start
 // with 168 each (64512); 2 x 128 x 208 + 128 x 88 are as many.
@@ -274,7 +347,7 @@ __device__ __forceinline__ void split_registers(bool softmax) {
 
 // One piece of the walk through a part: key tiles [kb, ke) of (tile, g).
 struct Walk {
-    TileRec t;
+    TileRec t, ahead;  // the tile's record, and the next one's, requested a tile before it is needed
     uint32_t tile, g, off, left, kb, ke;
     bool whole;
 };
@@ -285,7 +358,7 @@ __global__ void __launch_bounds__(tc_threads(STREAMS), 1)
 ragged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                  const __grid_constant__ CUtensorMap map_v, const __grid_constant__ TcParams p) {
     extern __shared__ __align__(16) unsigned char smem[];
-    __shared__ __align__(8) unsigned long long bars[13 + 2 * kMaxSlots];
+    __shared__ __align__(8) unsigned long long bars[16 + 2 * kMaxSlots];
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag;
     pdl_launch_dependents();
@@ -295,23 +368,28 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t base = ((uint32_t)__cvta_generic_to_shared(smem) + 1023u) & ~1023u;
     const uint32_t bar32 = (uint32_t)__cvta_generic_to_shared(bars);
-    const uint32_t q_full = bar32, q_empty = bar32 + 8, v_clean = bar32 + 16;
+    const uint32_t q_full = bar32, q_empty = bar32 + 8;
+    auto v_clean = [&](uint32_t i) { return bar32 + 8 * (i ? 15 : 2); };  // the loader may be a piece ahead
     auto s_full = [&](uint32_t i) { return bar32 + 8 * (3 + i); };
     auto p_full = [&](uint32_t i) { return bar32 + 8 * (5 + i); };
     auto pv_done = [&](uint32_t i) { return bar32 + 8 * (7 + i); };  // one stream only
     auto o_full = [&](uint32_t i) { return bar32 + 8 * (9 + i); };
     auto o_free = [&](uint32_t i) { return bar32 + 8 * (11 + i); };
-    auto full = [&](uint32_t i) { return bar32 + 8 * (13 + i); };
-    auto empty = [&](uint32_t i) { return bar32 + 8 * (13 + kMaxSlots + i); };
+    auto p_half = [&](uint32_t i) { return bar32 + 8 * (13 + i); };
+    auto full = [&](uint32_t i) { return bar32 + 8 * (16 + i); };
+    auto empty = [&](uint32_t i) { return bar32 + 8 * (16 + kMaxSlots + i); };
+    const uint32_t dk = DK ? DK : p.dk, dv = DV ? DV : p.dv, vk = DV ? (DV <= 2 ? 128 : 64) : p.vk;
+    const uint32_t SLOT = DK && DV ? (DK == 1 && DV == 1 ? 1 : 2) * ATOM : p.slot, kb_slot = SLOT / ATOM;  // blocks of keys in a slot
+    const uint32_t ks = (dk + kb_slot - 1) / kb_slot, vs = TK / vk;                                       // slots of a tile's keys, values
     auto slot_at = [&](uint32_t i) { return base + p.slots_at + i * SLOT; };
-    const uint32_t dk = DK ? DK : p.dk, dv = DV ? DV : p.dv, vk = DV ? (DV == 1 ? 128 : DV == 2 ? 64 : 32) : p.vk, vs = TK / vk;
 
     if (tid == 0) {
         mbar_init(q_full, 1);
-        mbar_init(q_empty, 1);
-        mbar_init(v_clean, 1);
+        mbar_init(q_empty, STREAMS);
         for (uint32_t i = 0; i < 2; ++i) {
+            mbar_init(v_clean(i), 1);
             mbar_init(s_full(i), 1);
+            mbar_init(p_half(i), 4);
             mbar_init(p_full(i), 4);
             mbar_init(pv_done(i), 1);
             mbar_init(o_full(i), 1);
@@ -319,7 +397,7 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         }
         for (uint32_t i = 0; i < p.n_slots; ++i) {
             mbar_init(full(i), 1);
-            mbar_init(empty(i), 1);
+            mbar_init(empty(i), STREAMS);
         }
         abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -346,8 +424,19 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         w.off = part.off;
         w.left = part.n_units;
         w.t = p.w.tiles[w.tile];
+        w.ahead = p.w.tiles[min(w.tile + 1, p.max_tiles - 1)];
     }
-    // The next piece; the tile's record is the one that w.t holds when the walk enters it.
+    auto leave = [&]() {  // behind a piece
+        if (w.left) {
+            w.off = 0;
+            if (++w.g == s.kv_heads) {
+                w.g = 0;
+                ++w.tile;
+                w.t = w.ahead;
+                w.ahead = p.w.tiles[min(w.tile + 1, p.max_tiles - 1)];
+            }
+        }
+    };
     auto next = [&]() {
         while (w.left) {
             const uint32_t cost = w.t.kt + kTileCost, n = min(cost - w.off, w.left);
@@ -357,34 +446,19 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             w.off += n;
             w.whole = w.kb == 0 && w.ke == w.t.kt;
             if (w.kb < w.ke || (w.kb == 0 && w.t.kt == 0)) return true;
-            if (w.left) {  // only the constant was left of it
-                w.off = 0;
-                if (++w.g == s.kv_heads) {
-                    w.g = 0;
-                    w.t = p.w.tiles[++w.tile];
-                }
-            }
+            leave();  // only the constant was left of it
         }
         return false;
-    };
-    auto leave = [&]() {  // behind a piece
-        if (w.left) {
-            w.off = 0;
-            if (++w.g == s.kv_heads) {
-                w.g = 0;
-                w.t = p.w.tiles[++w.tile];
-            }
-        }
     };
 
     if (warp >= LOADER) {
         split_registers<STREAMS>(false);
         if (warp == LOADER) {
             bool alive = true;
-            uint32_t pieces = 0, slot = 0, turn = 1, n = 0;  // turn: parity that a slot's first use finds
+            uint32_t pieces = 0, slot = 0, turn = 1, n = 0, cleaned = 0;  // turn: parity that a slot's first use finds
             // A slot's copies, a lane each: rows of `box`, blocks of 64 columns.
-            const uint32_t k_boxes = TK / p.kbox, v_per = p.vk / p.vbox, v_boxes = v_per * dv;
-            const uint32_t k_row = lane % k_boxes * p.kbox, v_block = lane / v_per, v_row = lane % v_per * p.vbox;
+            const uint32_t k_per = TK / p.kbox, v_per = vk / p.vbox, v_boxes = v_per * dv;
+            const uint32_t k_block = lane / k_per, k_row = lane % k_per * p.kbox, v_block = lane / v_per, v_row = lane % v_per * p.vbox;
             const uint32_t in_page = (1u << a.shift) - 1;
             auto enter = [&](uint32_t bytes) {  // the next slot, free
                 alive = alive && __all_sync(0xFFFFFFFFu, mbar_wait(empty(slot), turn, ab, p.err));
@@ -414,9 +488,11 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                     uint32_t pages = look_up(w.kb), pages_after = 0;  // of the tile whose values, and of the one whose keys are next
                     auto keys = [&](uint32_t t, uint32_t from) {
                         const uint32_t page = __shfl_sync(0xFFFFFFFFu, from, k_row >> 4);
-                        for (uint32_t b = 0; b < dk && alive; ++b) {
-                            enter(SLOT);
-                            if (alive && lane < k_boxes) copy(&map_k, slot_at(slot) + k_row * 128, t * TK + k_row, page, b * 64);
+                        for (uint32_t b = 0; b < dk && alive; b += kb_slot) {
+                            const uint32_t blocks = min(kb_slot, dk - b);
+                            enter(blocks * ATOM);
+                            if (alive && k_block < blocks)
+                                copy(&map_k, slot_at(slot) + k_block * ATOM + k_row * 128, t * TK + k_row, page, (b + k_block) * 64);
                             after();
                         }
                     };
@@ -439,7 +515,8 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                         if (dirty) {
                             fence_proxy_async();
                             __syncwarp();
-                            if (alive && lane == 0) mbar_arrive(v_clean);
+                            if (alive && lane == 0) mbar_arrive(v_clean(cleaned++ & 1u));
+                            cleaned = __shfl_sync(0xFFFFFFFFu, cleaned, 0);
                         }
                     };
                     keys(w.kb, pages);
@@ -448,7 +525,7 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                         mbar_arrive_tx(q_full, STREAMS * dk * p.rt * p.R * 128);
                         for (uint32_t q = 0; q < STREAMS; ++q)
                             for (uint32_t b = 0; b < dk; ++b)
-                                tensor_copy_4d(base + (q * dk + b) * SLOT, &map_q, b * 64, w.g * p.R, w.t.row0 + q * p.rt, 0, q_full);
+                                tensor_copy_4d(base + (q * dk + b) * ATOM, &map_q, b * 64, w.g * p.R, w.t.row0 + q * p.rt, 0, q_full);
                     }
                     __syncwarp();
                     if (alive) ++pieces;
@@ -470,126 +547,107 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 for (uint32_t i = 0; pieces > 0 && i < kSpinLimit; ++i)
                     if (mbar_try_wait(q_full, (pieces - 1) & 1u)) break;
             }
-        } else if (warp == ISSUER) {
-            {
-                const uint32_t lead = elect_lane(), tm = __shfl_sync(0xFFFFFFFFu, tmem, 0);
-                auto wait_for = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, ab, p.err)) != 0; };
-                const uint32_t id_s = idesc_bf16(128, TK), id_o = idesc_bf16(128, s.vdimp) | (1u << 16);  // V: MN-major
-                bool alive = true;
-                uint32_t pieces = 0, cleaned = 0, count = 0;  // count: tiles of a stream so far
-                uint32_t slot = 0, turn = 0;                  // of the next keys or values; turn: parity of the ring's rounds
-                const uint64_t q_desc = smem_desc_sw128(base), k_desc = smem_desc_sw128(slot_at(0)),
-                               v_desc = smem_desc_mn_sw128(slot_at(0), vk * 128);
-                constexpr uint64_t kSlotDesc = SLOT >> 4;
-                const uint32_t steps_last = DK ? 4 : s.dimp / 16 - (dk - 1) * 4;
-                auto after = [&](uint32_t& at, uint32_t& round) {
-                    if (++at == p.n_slots) {
-                        at = 0;
-                        round ^= 1u;
-                    }
-                };
-                // Scores of a stream against the keys in the slots from (at, round) on; release: the slots are free behind them.
-                auto scores = [&](uint32_t q, uint32_t col, uint32_t& at, uint32_t& round, bool wait, bool release) {
-                    uint64_t qd = q_desc + q * dk * kSlotDesc;
+        } else if (warp < ISSUER + STREAMS) {
+            const uint32_t q = __shfl_sync(0xFFFFFFFFu, warp - ISSUER, 0), lead = elect_lane(), tm = __shfl_sync(0xFFFFFFFFu, tmem, 0);
+            auto wait_for = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, ab, p.err)) != 0; };
+            const uint32_t id_s = idesc_bf16(128, TK), id_o = idesc_bf16(128, s.vdimp) | (1u << 16);  // V: MN-major
+            bool alive = true;
+            uint32_t pieces = 0, cleaned = 0, count = 0;  // count: tiles so far
+            uint32_t slot = 0, turn = 0;                  // of the next keys or values; turn: parity of the ring's rounds
+            const uint64_t q_desc = smem_desc_sw128(base + q * dk * ATOM), k_desc = smem_desc_sw128(slot_at(0)),
+                           v_desc = smem_desc_mn_sw128(slot_at(0), vk * 128);
+            const uint64_t slot_desc = SLOT >> 4, atom_desc = ATOM >> 4;
+            const uint32_t steps_last = DK ? 4 : s.dimp / 16 - (dk - 1) * 4, o_col = 256 + q * 128;
+            auto after = [&]() {
+                commit(empty(slot), lead);  // free when both streams have done with it
+                if (++slot == p.n_slots) {
+                    slot = 0;
+                    turn ^= 1u;
+                }
+            };
+            // Scores against the keys in the next slots.
+            auto scores = [&](uint32_t col) {
+                uint64_t qd = q_desc;
 #pragma unroll
-                    for (uint32_t b = 0; b < dk; ++b, qd += kSlotDesc) {
-                        if (wait && !wait_for(full(at), round)) return false;
-                        tc_fence_after();
-                        const uint64_t kd = k_desc + at * kSlotDesc;
-                        const uint32_t steps = b + 1 < dk ? 4 : steps_last;
-                        if (steps == 4) {
+                for (uint32_t b0 = 0; b0 < dk; b0 += kb_slot) {
+                    if (!wait_for(full(slot), turn)) return false;
+                    tc_fence_after();
+                    uint64_t kd = k_desc + slot * slot_desc;
+#pragma unroll
+                    for (uint32_t b = b0; b < b0 + kb_slot; ++b, qd += atom_desc, kd += atom_desc) {
+                        if (b >= dk) break;
+                        if (DK || b + 1 < dk || steps_last == 4) {
 #pragma unroll
                             for (uint32_t k = 0; k < 4; ++k) mma_ss(tm + col, qd + 2 * k, kd + 2 * k, id_s, (b | k) != 0 ? 1u : 0u, lead);
                         } else {
-                            for (uint32_t k = 0; k < steps; ++k) mma_ss(tm + col, qd + 2 * k, kd + 2 * k, id_s, (b | k) != 0 ? 1u : 0u, lead);
+                            for (uint32_t k = 0; k < steps_last; ++k) mma_ss(tm + col, qd + 2 * k, kd + 2 * k, id_s, (b | k) != 0 ? 1u : 0u, lead);
                         }
-                        if (release) commit(empty(at), lead);
-                        after(at, round);
                     }
-                    return true;
-                };
-                auto product = [&](uint32_t o_col, uint32_t p_col, uint32_t& at, uint32_t& round, bool wait, bool release, bool first) {
-                    uint32_t pa = tm + p_col, more = first ? 0u : 1u;
-#pragma unroll
-                    for (uint32_t v = 0; v < vs; ++v) {
-                        if (wait && !wait_for(full(at), round)) return false;
-                        tc_fence_after();
-                        uint64_t vd = v_desc + at * kSlotDesc;
-#pragma unroll
-                        for (uint32_t k = 0; k < vk; k += 32) {
-#pragma unroll
-                            for (uint32_t e = 0; e < 2; ++e, pa += 8, vd += 2048 >> 4, more = 1) mma_ts(tm + o_col, pa, vd, id_o, more, lead);
-                        }
-                        if (release) commit(empty(at), lead);
-                        after(at, round);
-                    }
-                    return true;
-                };
-                while (alive && next()) {
-                    if (w.kb < w.ke) {
-                        const uint32_t end = __shfl_sync(0xFFFFFFFFu, (uint32_t)(w.t.see0 + (int32_t)w.t.tokens - 1), 0);
-                        const uint32_t kb = __shfl_sync(0xFFFFFFFFu, w.kb, 0);
-                        alive = wait_for(q_full, pieces & 1u);
-                        const uint32_t nt = __shfl_sync(0xFFFFFFFFu, w.ke - w.kb, 0);
-                        if (STREAMS == 2) {
-                            for (uint32_t q = 0; q < 2 && alive; ++q) {
-                                uint32_t at = slot, round = turn;
-                                alive = scores(q, q * TK, at, round, q == 0, q == 1);
-                                if (alive) commit(s_full(q), lead);
-                                if (q == 1) slot = at, turn = round;
-                            }
-                            if (nt == 1 && alive) commit(q_empty, lead);
-                            for (uint32_t t = 0; t < nt && alive; ++t) {
-                                const bool more = t + 1 < nt;
-                                if ((kb + t + 1) * TK > end) alive = wait_for(v_clean, cleaned++ & 1u);
-                                uint32_t at = slot, round = turn;
-                                for (uint32_t q = 0; q < 2 && alive; ++q) {
-                                    alive = wait_for(p_full(q), (count + t) & 1u);
-                                    if (alive && t == 0 && pieces > 0) alive = wait_for(o_free(q), (pieces - 1) & 1u);
-                                    at = slot, round = turn;
-                                    alive = alive && product(256 + q * 128, q * TK, at, round, q == 0, q == 1, t == 0);
-                                    if (!alive) break;
-                                    if (more) {
-                                        alive = scores(q, q * TK, at, round, q == 0, q == 1);
-                                        if (alive) commit(s_full(q), lead);
-                                        if (t + 2 == nt && q == 1) commit(q_empty, lead);
-                                    } else {
-                                        commit(o_full(q), lead);
-                                    }
-                                }
-                                slot = at, turn = round;
-                            }
-                            count += nt;
-                        } else {
-                            alive = alive && scores(0, (count & 1u) * TK, slot, turn, true, true);
-                            if (alive) {
-                                commit(s_full(count & 1u), lead);
-                                if (nt == 1) commit(q_empty, lead);
-                            }
-                            for (uint32_t t = 0; t < nt && alive; ++t) {
-                                const uint32_t b = (count + t) & 1u, use = (count + t) >> 1;
-                                if (t + 1 < nt) {
-                                    alive = scores(0, (b ^ 1u) * TK, slot, turn, true, true);
-                                    if (!alive) break;
-                                    commit(s_full(b ^ 1u), lead);
-                                    if (t + 2 == nt) commit(q_empty, lead);
-                                }
-                                if ((kb + t + 1) * TK > end) alive = wait_for(v_clean, cleaned++ & 1u);
-                                alive = alive && wait_for(p_full(b), use & 1u);
-                                if (alive && t == 0 && pieces > 0) alive = wait_for(o_free(0), (pieces - 1) & 1u);
-                                alive = alive && product(256, b * TK, slot, turn, true, true, t == 0);
-                                if (!alive) break;
-                                commit(pv_done(b), lead);
-                                if (t + 1 == nt) commit(o_full(0), lead);
-                            }
-                            count += nt;
-                        }
-                        ++pieces;
-                    }
-                    leave();
+                    after();
                 }
-                if (!alive) *ab = 1;
+                return true;
+            };
+            // O += P V, the second half of P when `rest` says so.
+            auto product = [&](uint32_t p_col, bool first, uint32_t rest, uint32_t parity) {
+                uint32_t pa = tm + p_col, more = first ? 0u : 1u;
+#pragma unroll
+                for (uint32_t v = 0; v < vs; ++v) {
+                    if (!wait_for(full(slot), turn)) return false;
+                    tc_fence_after();
+                    uint64_t vd = v_desc + slot * slot_desc;
+#pragma unroll
+                    for (uint32_t k = 0; k < vk; k += 64) {
+                        if (v * vk + k == TK / 2) {
+                            if (!wait_for(rest, parity)) return false;
+                            tc_fence_after();
+                        }
+#pragma unroll
+                        for (uint32_t e = 0; e < 4; ++e, pa += 8, vd += 2048 >> 4, more = 1) mma_ts(tm + o_col, pa, vd, id_o, more, lead);
+                    }
+                    after();
+                }
+                return true;
+            };
+            while (alive && next()) {
+                if (w.kb < w.ke) {
+                    const uint32_t end = __shfl_sync(0xFFFFFFFFu, (uint32_t)(w.t.see0 + (int32_t)w.t.tokens - 1), 0);
+                    const uint32_t kb = __shfl_sync(0xFFFFFFFFu, w.kb, 0), nt = __shfl_sync(0xFFFFFFFFu, w.ke - w.kb, 0);
+                    alive = wait_for(q_full, pieces & 1u);
+                    // buffer of scores, and its uses so far, of tile t of the piece
+                    auto buffer = [&](uint32_t t) { return STREAMS == 2 ? q : (count + t) & 1u; };
+                    auto use = [&](uint32_t t) { return STREAMS == 2 ? count + t : (count + t) >> 1; };
+                    alive = alive && scores(buffer(0) * TK);
+                    if (alive) {
+                        commit(s_full(buffer(0)), lead);
+                        if (nt == 1) commit(q_empty, lead);
+                    }
+                    for (uint32_t t = 0; t < nt && alive; ++t) {
+                        const uint32_t b = buffer(t), parity = use(t) & 1u;
+                        auto ahead = [&]() {  // the next tile's scores
+                            if (!scores(buffer(t + 1) * TK)) return false;
+                            commit(s_full(buffer(t + 1)), lead);
+                            if (t + 2 == nt) commit(q_empty, lead);
+                            return true;
+                        };
+                        if (STREAMS == 1 && t + 1 < nt) alive = ahead();
+                        if ((kb + t + 1) * TK > end) {
+                            alive = alive && wait_for(v_clean(cleaned & 1u), (cleaned >> 1) & 1u);
+                            ++cleaned;
+                        }
+                        alive = alive && wait_for(p_half(b), parity);
+                        if (alive && t == 0 && pieces > 0) alive = wait_for(o_free(q), (pieces - 1) & 1u);
+                        alive = alive && product(b * TK, t == 0, p_full(b), parity);
+                        if (!alive) break;
+                        if (STREAMS == 1) commit(pv_done(b), lead);
+                        if (t + 1 == nt) commit(o_full(q), lead);
+                        else if (STREAMS == 2) alive = ahead();
+                    }
+                    count += nt;
+                    ++pieces;
+                }
+                leave();
             }
+            if (!alive) *ab = 1;
             __syncwarp();
         }
     } else {
@@ -626,7 +684,8 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 }
                 float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int i = 0; i < 128; ++i) mx4[i & 3] = fmaxf(mx4[i & 3], __uint_as_float(sv[i >> 5][i & 31]));
+                for (int i = 0; i < 128; i += 2)
+                    mx4[(i >> 1) & 3] = max3(mx4[(i >> 1) & 3], __uint_as_float(sv[i >> 5][i & 31]), __uint_as_float(sv[i >> 5][(i & 31) + 1]));
                 // what lies in the tile behind the rows has no say in when the others are rescaled
                 const float mx = real ? fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * scale : -INFINITY;
                 if (t == w.kb) {
@@ -651,30 +710,41 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                     mx_run = to;
                 }
                 const float shift = mx_run == -INFINITY ? 0.0f : mx_run;
-                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                // A half of the keys at a time: the product of the first half runs under the exponentials of the second.
+                const pair scale_2 = pair_of(scale, scale), shift_2 = pair_of(-shift, -shift);
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     uint32_t pw[32];
 #pragma unroll
-                    for (int i = 0; i < 64; i += 2) {
-                        const int at = h * 64 + i;
-                        const float x = ex2(fmaf(__uint_as_float(sv[at >> 5][at & 31]), scale, -shift));
-                        const float y = ex2(fmaf(__uint_as_float(sv[at >> 5][(at & 31) + 1]), scale, -shift));
-                        pw[i >> 1] = pack2(x, y);
-                        sum[i & 2] += x;
-                        sum[(i & 2) + 1] += y;
+                    for (int i = 0; i < 32; ++i) {
+                        uint32_t &x = sv[h * 2 + (i >> 4)][(2 * i) & 31], &y = sv[h * 2 + (i >> 4)][((2 * i) & 31) + 1];
+                        const pair z = fma2(pair_of(x, y), scale_2, shift_2);
+                        if (by_products(i)) {
+                            exp2_pair(z, x, y);
+                        } else {
+                            uint32_t u, v;
+                            split(z, u, v);
+                            x = __float_as_uint(ex2(__uint_as_float(u)));
+                            y = __float_as_uint(ex2(__uint_as_float(v)));
+                        }
+                        pw[i] = pack2(__uint_as_float(x), __uint_as_float(y));
                     }
                     tc_st32(s_col + h * 32, pw);
+                    tc_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(h == 0 ? p_half(b) : p_full(b));
                 }
-                tc_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(p_full(b));
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                pair sum[2] = {0, 0};
+#pragma unroll
+                for (int i = 0; i < 128; i += 2) sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], pair_of(sv[i >> 5][i & 31], sv[i >> 5][(i & 31) + 1]));
+                uint32_t u, v;
+                split(add2(sum[0], sum[1]), u, v);
+                l += __uint_as_float(u) + __uint_as_float(v);
             }
             if (!alive) break;
             if (w.kb < w.ke) {
-                alive = __all_sync(0xFFFFFFFFu, mbar_wait(o_full(STREAMS == 2 ? q : 0), pieces & 1u, ab, p.err));
+                alive = __all_sync(0xFFFFFFFFu, mbar_wait(o_full(q), pieces & 1u, ab, p.err));
                 if (!alive) break;
                 tc_fence_after();
                 ++pieces;
@@ -682,8 +752,8 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             if (w.whole) {
                 bf16* row = static_cast<bf16*>(a.out) + (size_t)(w.t.row0 + token) * a.out_pitch;
                 bf16* out = row + (size_t)head * s.vdim;
-                const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-                const bool wide = (((uintptr_t)out) & 15u) == 0;
+                const float inv = mx_run > -INFINITY ? 1.0f / l : 0.0f;
+                const uint32_t even = (uint32_t)(uintptr_t)out & 31u;  // 32-byte stores where they may be: a sector each
 #pragma unroll 1
                 for (uint32_t col = 0; col < s.vdim; col += 32) {
                     uint32_t o[32];
@@ -691,18 +761,27 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                         tc_ld32(tmem + lanes + o_col + col, o);
                         tc_wait_ld();
                     }
-                    float x[32];
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) x[i] = l > 0.0f ? __uint_as_float(o[i]) * inv : 0.0f;
-                    if (real && wide && col + 32 <= s.vdim) {
+                    for (int i = 0; i < 32; ++i) o[i] = mx_run > -INFINITY ? __float_as_uint(__uint_as_float(o[i]) * inv) : 0u;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[i] = pack2(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1]));
+                    if (real && even == 0 && col + 32 <= s.vdim) {
+                        store32(out + col, o);
+                        store32(out + col + 16, o + 8);
+                    } else if (real && (even & 15u) == 0) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
-                            reinterpret_cast<uint4*>(out + col)[i] = make_uint4(pack2(x[8 * i], x[8 * i + 1]), pack2(x[8 * i + 2], x[8 * i + 3]),
-                                                                                pack2(x[8 * i + 4], x[8 * i + 5]), pack2(x[8 * i + 6], x[8 * i + 7]));
+                            if (col + 8 * i + 8 <= s.vdim) {
+                                *reinterpret_cast<uint4*>(out + col + 8 * i) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                            } else {
+#pragma unroll
+                                for (int e = 0; e < 8; ++e)
+                                    if (col + 8 * i + e < s.vdim) out[col + 8 * i + e] = half_of(o[4 * i + e / 2], e & 1);
+                            }
                     } else if (real) {
 #pragma unroll
                         for (int i = 0; i < 32; ++i)
-                            if (col + i < s.vdim) out[col + i] = __float2bfloat16_rn(x[i]);
+                            if (col + i < s.vdim) out[col + i] = half_of(o[i / 2], i & 1);
                     }
                     __syncwarp();
                 }
@@ -734,15 +813,17 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
 
     tc_fence_before();
     __syncthreads();
-    if (warp == ISSUER) {
-        const uint32_t lead = elect_lane();  // the lane that issued
-        if (abort_flag && lead) {  // instructions in flight get a bounded chance to finish (gemm_bf16.cu)
-            mbar_init(v_clean, 1);
-            tc_commit(v_clean);
+    if (abort_flag) {  // instructions in flight get a bounded chance to finish (gemm_bf16.cu)
+        if (warp >= ISSUER && warp < ISSUER + STREAMS && elect_lane()) {  // the lanes that issued
+            const uint32_t bar = v_clean(warp - ISSUER);
+            mbar_init(bar, 1);
+            tc_commit(bar);
             for (uint32_t i = 0; i < kSpinLimit; ++i)
-                if (mbar_try_wait(v_clean, 0)) break;
+                if (mbar_try_wait(bar, 0)) break;
         }
-        __syncwarp();
+        __syncthreads();
+    }
+    if (warp == ISSUER) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
     }
@@ -750,8 +831,9 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
 
 // The pieces of a tile, in the order of its keys: a block for 32 rows of the tile that begins in part blockIdx.x; a lane per row, eight
 // columns per warp and turn.
+constexpr uint32_t kJoinThreads = 256;
 template <int STREAMS>
-__global__ void __launch_bounds__(128)
+__global__ void __launch_bounds__(kJoinThreads)
 ragged_join_kernel(const __grid_constant__ TcParams p) {
     pdl_launch_dependents();
     pdl_wait();
@@ -765,30 +847,35 @@ ragged_join_kernel(const __grid_constant__ TcParams p) {
     const uint32_t m = row & 127, token = (row >> 7) * p.rt + m / p.R, head = sp.g * p.R + m % p.R;
     if (m >= p.rt * p.R || token >= t.tokens) return;
     constexpr uint32_t ROWS = STREAMS * 128;
-    const size_t size = (size_t)(s.vdimp + 2) * ROWS;
+    const size_t size = (size_t)(s.vdimp + 2) * ROWS, ml = (size_t)s.vdimp * ROWS;
     auto piece = [&](uint32_t i) { return p.w.partial + (size_t)(i == c ? 2 * c + 1 : 2 * i) * size + row; };
     float mx = -INFINITY, sum = 0.0f;
-    for (uint32_t i = c; i <= sp.last; ++i) mx = fmaxf(mx, piece(i)[(size_t)s.vdimp * ROWS]);
+#pragma unroll 4
+    for (uint32_t i = c; i <= sp.last; ++i) mx = fmaxf(mx, piece(i)[ml]);
     const float shift = mx == -INFINITY ? 0.0f : mx;
-    for (uint32_t i = c; i <= sp.last; ++i)
-        sum += exp2f(piece(i)[(size_t)s.vdimp * ROWS] - shift) * piece(i)[(size_t)(s.vdimp + 1) * ROWS];
-    const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+#pragma unroll 4
+    for (uint32_t i = c; i <= sp.last; ++i) sum += exp2f(piece(i)[ml] - shift) * piece(i)[ml + ROWS];
+    const float inv = mx > -INFINITY ? 1.0f / sum : 0.0f;
     bf16* out = static_cast<bf16*>(a.out) + (size_t)(t.row0 + token) * a.out_pitch;
-    for (uint32_t col = warp * 8; col < s.vdimp; col += 32) {
+    for (uint32_t col = warp * 8; col < s.vdimp; col += kJoinThreads / 4) {
         float acc[8] = {};
+#pragma unroll 2
         for (uint32_t i = c; i <= sp.last; ++i) {
             const float* x = piece(i);
-            const float f = exp2f(x[(size_t)s.vdimp * ROWS] - shift);
-            if (f == 0.0f) continue;  // a piece of which the row sees nothing
+            const float f = exp2f(x[ml] - shift);
+            float v[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) acc[e] = fmaf(f, x[(size_t)(col + e) * ROWS], acc[e]);
+            for (int e = 0; e < 8; ++e) v[e] = x[(size_t)(col + e) * ROWS];
+            if (f > 0.0f)  // not a piece of which the row sees nothing
+#pragma unroll
+                for (int e = 0; e < 8; ++e) acc[e] = fmaf(f, v[e], acc[e]);
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e)
             if (col + e < s.vdim) out[(size_t)head * s.vdim + col + e] = __float2bfloat16_rn(acc[e] * inv);
     }
     if (head == 0)
-        for (uint32_t i = s.heads * s.vdim + warp; i < a.out_pitch; i += 4) out[i] = __float2bfloat16_rn(0.0f);
+        for (uint32_t i = s.heads * s.vdim + warp; i < a.out_pitch; i += kJoinThreads / 32) out[i] = __float2bfloat16_rn(0.0f);
 }
 
 int done(cudaError_t e) { return e == cudaSuccess ? ZQ_OK : cuda_fail(e); }
@@ -805,13 +892,13 @@ TcParams params_of(const RaggedArgs& a, size_t& bytes) {
     p.scale2 = a.scale * kLog2e;
     p.dk = (s.dimp + 63) / 64;
     p.dv = (s.vdimp + 63) / 64;
-    p.vk = p.dv == 1 ? 128 : p.dv == 2 ? 64 : 32;
-    p.vs = TK / p.vk;
+    p.slot = (p.dk == 1 && p.dv == 1 ? 1 : 2) * ATOM;
+    p.vk = p.dv <= 2 ? 128 : 64;
     const uint32_t page = a.lens ? 1u << a.shift : TK;
     p.kbox = page < TK ? page : TK;
     p.vbox = page < p.vk ? page : p.vk;
-    p.slots_at = streams * p.dk * SLOT;
-    p.n_slots = (225 * 1024 - p.slots_at) / SLOT;
+    p.slots_at = streams * p.dk * ATOM;
+    p.n_slots = (225 * 1024 - p.slots_at) / p.slot;
     if (p.n_slots > kMaxSlots) p.n_slots = kMaxSlots;
     p.max_parts = sm_count() < (int)kMaxParts ? sm_count() : kMaxParts;
     const uint32_t tokens = streams * p.rt;
@@ -866,11 +953,11 @@ int launch(TcParams& p, cudaStream_t st) {
     if (rc == ZQ_OK) rc = map_4d(a.v, s.vdimp, s.kv_heads, rows, outer, a.v_ld, 1, p.vbox, &mv);
     if (rc == ZQ_OK) rc = device_error_word(&p.err);
     if (rc != ZQ_OK) return rc;
-    const uint32_t smem = p.slots_at + p.n_slots * SLOT + 1024;
+    const uint32_t smem = p.slots_at + p.n_slots * p.slot + 1024;
     ZQ_CUDA(cudaFuncSetAttribute(ragged_tc_kernel<STREAMS, DK, DV>, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024));
     rc = done(launch_pdl(ragged_prep_kernel, dim3(1), dim3(kPrepThreads), 0, st, p, STREAMS * p.rt));
     if (rc == ZQ_OK) rc = done(launch_pdl(ragged_tc_kernel<STREAMS, DK, DV>, dim3(p.max_parts), dim3(tc_threads(STREAMS)), smem, st, mq, mk, mv, p));
-    if (rc == ZQ_OK) rc = done(launch_pdl(ragged_join_kernel<STREAMS>, dim3(p.max_parts, STREAMS * 4), dim3(128), 0, st, p));
+    if (rc == ZQ_OK) rc = done(launch_pdl(ragged_join_kernel<STREAMS>, dim3(p.max_parts, STREAMS * 4), dim3(kJoinThreads), 0, st, p));
     return rc;
 }
 
