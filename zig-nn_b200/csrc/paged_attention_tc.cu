@@ -358,7 +358,7 @@ __global__ void __launch_bounds__(tc_threads(STREAMS), 1)
 ragged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                  const __grid_constant__ CUtensorMap map_v, const __grid_constant__ TcParams p) {
     extern __shared__ __align__(16) unsigned char smem[];
-    __shared__ __align__(8) unsigned long long bars[16 + 2 * kMaxSlots];
+    __shared__ __align__(8) unsigned long long bars[18 + 2 * kMaxSlots];
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag;
     pdl_launch_dependents();
@@ -376,8 +376,9 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     auto o_full = [&](uint32_t i) { return bar32 + 8 * (9 + i); };
     auto o_free = [&](uint32_t i) { return bar32 + 8 * (11 + i); };
     auto p_half = [&](uint32_t i) { return bar32 + 8 * (13 + i); };
-    auto full = [&](uint32_t i) { return bar32 + 8 * (16 + i); };
-    auto empty = [&](uint32_t i) { return bar32 + 8 * (16 + kMaxSlots + i); };
+    auto my_turn = [&](uint32_t i) { return bar32 + 8 * (16 + i); };  // of the issuers
+    auto full = [&](uint32_t i) { return bar32 + 8 * (18 + i); };
+    auto empty = [&](uint32_t i) { return bar32 + 8 * (18 + kMaxSlots + i); };
     const uint32_t dk = DK ? DK : p.dk, dv = DV ? DV : p.dv, vk = DV ? (DV <= 2 ? 128 : 64) : p.vk;
     const uint32_t SLOT = DK && DV ? (DK == 1 && DV == 1 ? 1 : 2) * ATOM : p.slot, kb_slot = SLOT / ATOM;  // blocks of keys in a slot
     const uint32_t ks = (dk + kb_slot - 1) / kb_slot, vs = TK / vk;                                       // slots of a tile's keys, values
@@ -388,6 +389,7 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         mbar_init(q_empty, STREAMS);
         for (uint32_t i = 0; i < 2; ++i) {
             mbar_init(v_clean(i), 1);
+            mbar_init(my_turn(i), 1);
             mbar_init(s_full(i), 1);
             mbar_init(p_half(i), 4);
             mbar_init(p_full(i), 4);
@@ -588,7 +590,7 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 return true;
             };
             // O += P V, the second half of P when `rest` says so.
-            auto product = [&](uint32_t p_col, bool first, uint32_t rest, uint32_t parity) {
+            auto product = [&](uint32_t p_col, bool first, uint32_t rest, uint32_t parity, uint32_t turn_parity) {
                 uint32_t pa = tm + p_col, more = first ? 0u : 1u;
 #pragma unroll
                 for (uint32_t v = 0; v < vs; ++v) {
@@ -598,7 +600,7 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
 #pragma unroll
                     for (uint32_t k = 0; k < vk; k += 64) {
                         if (v * vk + k == TK / 2) {
-                            if (!wait_for(rest, parity)) return false;
+                            if (!wait_for(rest, parity) || (STREAMS == 2 && !wait_for(my_turn(q), turn_parity))) return false;
                             tc_fence_after();
                         }
 #pragma unroll
@@ -636,11 +638,13 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                         }
                         alive = alive && wait_for(p_half(b), parity);
                         if (alive && t == 0 && pieces > 0) alive = wait_for(o_free(q), (pieces - 1) & 1u);
-                        alive = alive && product(b * TK, t == 0, p_full(b), parity);
+                        alive = alive && product(b * TK, t == 0, p_full(b), parity, (count + t + 1 - q) & 1u);
                         if (!alive) break;
                         if (STREAMS == 1) commit(pv_done(b), lead);
                         if (t + 1 == nt) commit(o_full(q), lead);
                         else if (STREAMS == 2) alive = ahead();
+                        if (STREAMS == 2 && lead) mbar_arrive(my_turn(1 - q));
+                        __syncwarp();
                     }
                     count += nt;
                     ++pieces;
