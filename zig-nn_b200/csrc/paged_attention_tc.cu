@@ -3,7 +3,7 @@
 //
 //   S = Q K^T   both operands K-major in shared memory (128-byte swizzle), S in tensor memory;
 //   softmax     one thread per row (its row is a tensor-memory lane), no exchange between threads; the running maximum is raised, and
-//               the output rescaled, only when it grows by more than 2^8: until then the weights are taken against the older maximum;
+//               the output rescaled, only when it grows by more than 2^16: until then the weights are taken against the older maximum;
 //   O += P V    P (bf16) is the A operand from tensor memory, where it overwrites its own scores; V as it lies in the cache (rows
 //               of keys: MN-major).
 // Up to 128 dimensions two such tiles of rows (STREAMS = 2) take turns on one stream of keys: the tensor cores work on one while the
@@ -27,7 +27,7 @@ constexpr uint32_t TK = 128;                // keys of a tile
 constexpr uint32_t ATOM = 128 * 128;        // bytes of 128 keys (or rows) x 64 dimensions
 constexpr uint32_t kMaxSlots = 12;
 constexpr uint32_t kMaxParts = 160;         // CTAs
-constexpr float kRaise = 8.0f;              // powers of two that the maximum may lag behind
+constexpr float kRaise = 16.0f;             // powers of two that the maximum may lag behind
 constexpr uint32_t kTileCost = 2;           // what a tile costs besides its keys, in key tiles
 constexpr uint32_t kLeastPart = 3;          // key tiles that a CTA is started for
 constexpr uint32_t kPrepThreads = 1024;
@@ -333,7 +333,34 @@ __device__ __forceinline__ void exp2_pair(pair x, uint32_t& a, uint32_t& b) {
 }
 // Pairs of eight whose exponentials are made that way: the special-function unit gives a warp's 32 in eight cycles, so 128 keys of a row
 // would take it as long as the tensor cores take for both products.
-__device__ __forceinline__ constexpr bool by_products(int pair_index) { return (pair_index & 7) == 2 || (pair_index & 7) == 5 || (pair_index & 7) == 7; }
+__device__ __forceinline__ constexpr bool by_products(int pair_index) { return (pair_index & 7) == 2; }
+
+__device__ __forceinline__ float max_of(const uint32_t (&sv)[4][32]) {
+    float m[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m[i] = fmaxf(__uint_as_float(sv[0][2 * i]), __uint_as_float(sv[0][2 * i + 1]));
+#pragma unroll
+    for (int i = 16; i < 128; i += 2) m[(i >> 1) & 7] = max3(m[(i >> 1) & 7], __uint_as_float(sv[i >> 5][i & 31]), __uint_as_float(sv[i >> 5][(i & 31) + 1]));
+    return max3(max3(m[0], m[1], m[2]), max3(m[3], m[4], m[5]), fmaxf(m[6], m[7]));
+}
+// x = 2^(x scale - shift) of 64 scores in place, and as bf16 two by two.
+__device__ __forceinline__ void weights(uint32_t (&x0)[32], uint32_t (&x1)[32], uint32_t (&pw)[32], float scale, float shift) {
+    const pair scale_2 = pair_of(scale, scale), shift_2 = pair_of(-shift, -shift);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+        uint32_t &x = i < 16 ? x0[(2 * i) & 31] : x1[(2 * i) & 31], &y = i < 16 ? x0[(2 * i + 1) & 31] : x1[(2 * i + 1) & 31];
+        const pair z = fma2(pair_of(x, y), scale_2, shift_2);
+        if (by_products(i)) {
+            exp2_pair(z, x, y);
+        } else {
+            uint32_t u, v;
+            split(z, u, v);
+            x = __float_as_uint(ex2(__uint_as_float(u)));
+            y = __float_as_uint(ex2(__uint_as_float(v)));
+        }
+        pw[i] = pack2(__uint_as_float(x), __uint_as_float(y));
+    }
+}
 
 // Registers: whole groups of four warps may pass registers to one another, so two streams come with a third group. 384 threads start
 // with 168 each (64512); 2 x 128 x 208 + 128 x 88 are as many.
@@ -560,21 +587,31 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                            v_desc = smem_desc_mn_sw128(slot_at(0), vk * 128);
             const uint64_t slot_desc = SLOT >> 4, atom_desc = ATOM >> 4;
             const uint32_t steps_last = DK ? 4 : s.dimp / 16 - (dk - 1) * 4, o_col = 256 + q * 128;
-            auto after = [&]() {
-                commit(empty(slot), lead);  // free when both streams have done with it
-                if (++slot == p.n_slots) {
-                    slot = 0;
-                    turn ^= 1u;
+            auto after = [&](uint32_t& at, uint32_t& round) {
+                if (++at == p.n_slots) {
+                    at = 0;
+                    round ^= 1u;
                 }
             };
-            // Scores against the keys in the next slots.
-            auto scores = [&](uint32_t col) {
+            // `n` slots from the next one on are there.
+            auto arrived = [&](uint32_t n) {
+                uint32_t at = slot, round = turn;
+                bool ok = true;
+#pragma unroll
+                for (uint32_t i = 0; i < n; ++i) {
+                    ok = ok && wait_for(full(at), round);
+                    after(at, round);
+                }
+                tc_fence_after();
+                return ok;
+            };
+            // Scores against the keys in the slots from `at` on, which have arrived.
+            auto scores = [&](uint32_t col, uint32_t at) {
                 uint64_t qd = q_desc;
+                uint32_t round = 0;
 #pragma unroll
                 for (uint32_t b0 = 0; b0 < dk; b0 += kb_slot) {
-                    if (!wait_for(full(slot), turn)) return false;
-                    tc_fence_after();
-                    uint64_t kd = k_desc + slot * slot_desc;
+                    uint64_t kd = k_desc + at * slot_desc;
 #pragma unroll
                     for (uint32_t b = b0; b < b0 + kb_slot; ++b, qd += atom_desc, kd += atom_desc) {
                         if (b >= dk) break;
@@ -585,30 +622,25 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                             for (uint32_t k = 0; k < steps_last; ++k) mma_ss(tm + col, qd + 2 * k, kd + 2 * k, id_s, (b | k) != 0 ? 1u : 0u, lead);
                         }
                     }
-                    after();
+                    after(at, round);
                 }
-                return true;
             };
-            // O += P V, the second half of P when `rest` says so.
-            auto product = [&](uint32_t p_col, bool first, uint32_t rest, uint32_t parity, uint32_t turn_parity) {
-                uint32_t pa = tm + p_col, more = first ? 0u : 1u;
+            // O += P V of 64 keys (half 0 or 1 of the tile), values in the slots from `at` on, which have arrived.
+            auto product = [&](uint32_t p_col, uint32_t half, bool first, uint32_t at) {
+                uint32_t round = 0, more = first && half == 0 ? 0u : 1u;
+                if (half == 1 && vs == 2) after(at, round);
+                uint32_t pa = tm + p_col + half * 32;
+                uint64_t vd = v_desc + at * slot_desc + (half == 1 && vs == 1 ? 4 * (2048 >> 4) : 0);
 #pragma unroll
-                for (uint32_t v = 0; v < vs; ++v) {
-                    if (!wait_for(full(slot), turn)) return false;
-                    tc_fence_after();
-                    uint64_t vd = v_desc + slot * slot_desc;
+                for (uint32_t e = 0; e < 4; ++e, pa += 8, vd += 2048 >> 4, more = 1) mma_ts(tm + o_col, pa, vd, id_o, more, lead);
+            };
+            // `n` slots from the next one on are free when both streams have done with them.
+            auto release = [&](uint32_t n) {
 #pragma unroll
-                    for (uint32_t k = 0; k < vk; k += 64) {
-                        if (v * vk + k == TK / 2) {
-                            if (!wait_for(rest, parity) || (STREAMS == 2 && !wait_for(my_turn(q), turn_parity))) return false;
-                            tc_fence_after();
-                        }
-#pragma unroll
-                        for (uint32_t e = 0; e < 4; ++e, pa += 8, vd += 2048 >> 4, more = 1) mma_ts(tm + o_col, pa, vd, id_o, more, lead);
-                    }
-                    after();
+                for (uint32_t i = 0; i < n; ++i) {
+                    commit(empty(slot), lead);
+                    after(slot, turn);
                 }
-                return true;
             };
             while (alive && next()) {
                 if (w.kb < w.ke) {
@@ -618,33 +650,54 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                     // buffer of scores, and its uses so far, of tile t of the piece
                     auto buffer = [&](uint32_t t) { return STREAMS == 2 ? q : (count + t) & 1u; };
                     auto use = [&](uint32_t t) { return STREAMS == 2 ? count + t : (count + t) >> 1; };
-                    alive = alive && scores(buffer(0) * TK);
+                    alive = alive && arrived(ks);
                     if (alive) {
+                        scores(buffer(0) * TK, slot);
                         commit(s_full(buffer(0)), lead);
                         if (nt == 1) commit(q_empty, lead);
+                        release(ks);
                     }
                     for (uint32_t t = 0; t < nt && alive; ++t) {
                         const uint32_t b = buffer(t), parity = use(t) & 1u;
-                        auto ahead = [&]() {  // the next tile's scores
-                            if (!scores(buffer(t + 1) * TK)) return false;
-                            commit(s_full(buffer(t + 1)), lead);
-                            if (t + 2 == nt) commit(q_empty, lead);
-                            return true;
-                        };
-                        if (STREAMS == 1 && t + 1 < nt) alive = ahead();
+                        if (STREAMS == 1) {
+                            if (t + 1 < nt) {  // the next tile's scores
+                                alive = arrived(ks);
+                                if (!alive) break;
+                                scores(buffer(t + 1) * TK, slot);
+                                commit(s_full(buffer(t + 1)), lead);
+                                if (t + 2 == nt) commit(q_empty, lead);
+                                release(ks);
+                            }
+                            alive = arrived(vs);
+                        } else {  // all that is waited for ahead of the weights
+                            alive = arrived(t + 1 < nt ? vs + ks : vs);
+                        }
                         if ((kb + t + 1) * TK > end) {
                             alive = alive && wait_for(v_clean(cleaned & 1u), (cleaned >> 1) & 1u);
                             ++cleaned;
                         }
-                        alive = alive && wait_for(p_half(b), parity);
                         if (alive && t == 0 && pieces > 0) alive = wait_for(o_free(q), (pieces - 1) & 1u);
-                        alive = alive && product(b * TK, t == 0, p_full(b), parity, (count + t + 1 - q) & 1u);
+                        alive = alive && wait_for(p_half(b), parity);
                         if (!alive) break;
+                        tc_fence_after();
+                        product(b * TK, 0, t == 0, slot);
+                        alive = wait_for(p_full(b), parity) && (STREAMS == 1 || wait_for(my_turn(q), (count + t + 1 - q) & 1u));
+                        if (!alive) break;
+                        tc_fence_after();
+                        product(b * TK, 1, false, slot);
                         if (STREAMS == 1) commit(pv_done(b), lead);
-                        if (t + 1 == nt) commit(o_full(q), lead);
-                        else if (STREAMS == 2) alive = ahead();
+                        if (t + 1 == nt) {
+                            commit(o_full(q), lead);
+                        } else if (STREAMS == 2) {
+                            uint32_t at = slot, round = turn;
+                            for (uint32_t i = 0; i < vs; ++i) after(at, round);
+                            scores(b * TK, at);
+                            commit(s_full(b), lead);
+                            if (t + 2 == nt) commit(q_empty, lead);
+                        }
                         if (STREAMS == 2 && lead) mbar_arrive(my_turn(1 - q));
                         __syncwarp();
+                        release(STREAMS == 2 && t + 1 < nt ? vs + ks : vs);
                     }
                     count += nt;
                     ++pieces;
@@ -672,78 +725,67 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 alive = __all_sync(0xFFFFFFFFu, mbar_wait(s_full(b), use & 1u, ab, p.err));
                 if (!alive) break;
                 tc_fence_after();
-                uint32_t sv[4][32];
+                uint32_t sv[4][32], pw[32];
+                float mx;
+                // Weights are taken against the maximum of the tiles ahead, and this tile's is found beside them: no chain from the scores
+                // over their maximum to the weights. A weight may then exceed 1, which changes nothing (f32 and bf16 reach 2^127), unless
+                // the maximum grows by more than 2^kRaise: then the output is rescaled and the tile begun again.
+                for (;;) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) tc_ld32(s_col + i * 32, sv[i]);
-                tc_wait_ld();
-                if (p.scale2 <= 0.0f) {  // a negative scale turns the order round
+                    for (int i = 0; i < 4; ++i) tc_ld32(s_col + i * 32, sv[i]);
+                    tc_wait_ld();
+                    if (p.scale2 <= 0.0f) {  // a negative scale turns the order round
 #pragma unroll
-                    for (int i = 0; i < 128; ++i) sv[i >> 5][i & 31] = __float_as_uint(__uint_as_float(sv[i >> 5][i & 31]) * p.scale2);
-                }
-                if (w.t.see0 < (int32_t)((t + 1) * TK)) {  // some row does not see all of the tile
-                    const int lim = see - (int)(t * TK);
-#pragma unroll
-                    for (int i = 0; i < 128; ++i)
-                        if (i >= lim) sv[i >> 5][i & 31] = 0xFF800000u;
-                }
-                float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                for (int i = 0; i < 128; i += 2)
-                    mx4[(i >> 1) & 3] = max3(mx4[(i >> 1) & 3], __uint_as_float(sv[i >> 5][i & 31]), __uint_as_float(sv[i >> 5][(i & 31) + 1]));
-                // what lies in the tile behind the rows has no say in when the others are rescaled
-                const float mx = real ? fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * scale : -INFINITY;
-                if (t == w.kb) {
-                    mx_run = mx;
-                } else if (__any_sync(0xFFFFFFFFu, mx - mx_run > kRaise)) {
-                    const float to = fmaxf(mx_run, mx), f = mx_run == -INFINITY ? 1.0f : ex2(mx_run - to);
-                    if (STREAMS == 1) {  // O holds the tiles ahead of this one (with two streams the scores were issued behind it)
-                        alive = __all_sync(0xFFFFFFFFu, mbar_wait(pv_done((count - 1) & 1u), ((count - 1) >> 1) & 1u, ab, p.err));
-                        if (!alive) break;
-                        tc_fence_after();
+                        for (int i = 0; i < 128; ++i) sv[i >> 5][i & 31] = __float_as_uint(__uint_as_float(sv[i >> 5][i & 31]) * p.scale2);
                     }
-#pragma unroll 1
-                    for (uint32_t col = 0; col < s.vdimp; col += 32) {
-                        uint32_t o[32];
-                        tc_ld32(tmem + lanes + o_col + col, o);
-                        tc_wait_ld();
+                    if (w.t.see0 < (int32_t)((t + 1) * TK)) {  // some row does not see all of the tile
+                        const int lim = see - (int)(t * TK);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                        tc_st32(tmem + lanes + o_col + col, o);
+                        for (int i = 0; i < 128; ++i)
+                            if (i >= lim) sv[i >> 5][i & 31] = 0xFF800000u;
+                    }
+                    const float shift = mx_run == -INFINITY ? 0.0f : mx_run;
+                    mx = max_of(sv);
+                    weights(sv[0], sv[1], pw, scale, shift);
+                    // what lies in the tile behind the rows has no say in when the others are rescaled
+                    mx = real ? mx * scale : -INFINITY;
+                    if (!__any_sync(0xFFFFFFFFu, mx > mx_run + kRaise)) break;
+                    const float to = fmaxf(mx_run, mx), f = mx_run == -INFINITY ? 0.0f : ex2(mx_run - to);
+                    if (t > w.kb) {
+                        if (STREAMS == 1) {  // O holds the tiles ahead of this one (with two streams the scores were issued behind it)
+                            alive = __all_sync(0xFFFFFFFFu, mbar_wait(pv_done((count - 1) & 1u), ((count - 1) >> 1) & 1u, ab, p.err));
+                            if (!alive) break;
+                            tc_fence_after();
+                        }
+#pragma unroll 1
+                        for (uint32_t col = 0; col < s.vdimp; col += 32) {
+                            uint32_t o[32];
+                            tc_ld32(tmem + lanes + o_col + col, o);
+                            tc_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                            tc_st32(tmem + lanes + o_col + col, o);
+                        }
                     }
                     l *= f;
                     mx_run = to;
                 }
-                const float shift = mx_run == -INFINITY ? 0.0f : mx_run;
+                if (!alive) break;
                 // A half of the keys at a time: the product of the first half runs under the exponentials of the second.
-                const pair scale_2 = pair_of(scale, scale), shift_2 = pair_of(-shift, -shift);
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    uint32_t pw[32];
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        uint32_t &x = sv[h * 2 + (i >> 4)][(2 * i) & 31], &y = sv[h * 2 + (i >> 4)][((2 * i) & 31) + 1];
-                        const pair z = fma2(pair_of(x, y), scale_2, shift_2);
-                        if (by_products(i)) {
-                            exp2_pair(z, x, y);
-                        } else {
-                            uint32_t u, v;
-                            split(z, u, v);
-                            x = __float_as_uint(ex2(__uint_as_float(u)));
-                            y = __float_as_uint(ex2(__uint_as_float(v)));
-                        }
-                        pw[i] = pack2(__uint_as_float(x), __uint_as_float(y));
-                    }
+                    if (h == 1) weights(sv[2], sv[3], pw, scale, mx_run == -INFINITY ? 0.0f : mx_run);
                     tc_st32(s_col + h * 32, pw);
                     tc_wait_st();
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(h == 0 ? p_half(b) : p_full(b));
                 }
-                pair sum[2] = {0, 0};
+                pair sum[4] = {0, 0, 0, 0};
 #pragma unroll
-                for (int i = 0; i < 128; i += 2) sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], pair_of(sv[i >> 5][i & 31], sv[i >> 5][(i & 31) + 1]));
+                for (int i = 0; i < 128; i += 2) sum[(i >> 1) & 3] = add2(sum[(i >> 1) & 3], pair_of(sv[i >> 5][i & 31], sv[i >> 5][(i & 31) + 1]));
                 uint32_t u, v;
-                split(add2(sum[0], sum[1]), u, v);
+                split(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), u, v);
                 l += __uint_as_float(u) + __uint_as_float(v);
             }
             if (!alive) break;
