@@ -1,4 +1,6 @@
 // Causal grouped-query attention of ragged rows over pages of keys and values, or over packed prompts; softmax in f32.
+//   * a few rows of each request (bf16): the packed rows as the 16 rows of mma.sync, a warp per range of keys;
+//   * more rows (bf16): paged_attention_tc.cu;
 //   * f32, and heads beyond 256 dimensions: tiles of 16 or 64 packed rows against tiles of keys, plain multiply-adds;
 //   * where a request's keys are cut into ranges, the ranges meet in a second small kernel.
 #include "paged_common.cuh"
@@ -191,6 +193,222 @@ ragged_plain_kernel(const __grid_constant__ RaggedCall call) {
     });
 }
 
+// ---- a few rows of each request, bf16 ---------------------------------------------------------------------------------------
+// A warp per item: up to 16 packed rows against its range of keys, 16 keys a step. The keys and values of a step are the warp's own:
+// cp.async into a ring of its own in shared memory, STAGES - 1 steps ahead, through the end of an item into the next one's, so that
+// the stream of keys and values never stops and no warp waits for another. What bounds it: that stream (per step 16 (D + V) values
+// against 2 D / 8 + 2 V / 8 MMAs).
+constexpr uint32_t kFewThreads = 128;
+
+template <int D, int STAGES>
+__global__ void __launch_bounds__(kFewThreads)
+ragged_few_kernel(const __grid_constant__ RaggedCall call) {
+    constexpr int S = D / 16;
+    extern __shared__ __align__(16) unsigned char smem[];
+    __shared__ uint32_t first[kFewThreads + 1];
+    __shared__ uint32_t sums[kFewThreads / 32];
+    pdl_launch_dependents();
+    pdl_wait();
+    const RaggedArgs& a = call.a;
+    const RaggedPlan& p = call.p;
+    const GqaShape& s = a.s;
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = gridDim.x * (kFewThreads / 32);
+    const uint32_t kpitch = (s.dimp + 8) * 2, vpitch = (s.vdimp + 8) * 2, k_bytes = 16 * kpitch, stage_bytes = k_bytes + 16 * vpitch;
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * STAGES * stage_bytes;
+    const bf16 *q = static_cast<const bf16*>(a.q), *kc = static_cast<const bf16*>(a.k), *vc = static_cast<const bf16*>(a.v);
+    const float scale2 = a.scale * kLog2e;
+
+    // 16 rows of one array -> shared memory, 16 bytes a lane and turn; zeros from row `rows` on
+    auto copy_rows = [&](uint32_t dst, uint32_t pitch, const bf16* base, size_t ld, size_t row0, uint32_t col, uint32_t dp, uint32_t rows) {
+        const uint32_t cpr = dp / 8, dr = 32 / cpr, dc = 32 % cpr;
+        uint32_t r = lane / cpr, c = lane % cpr;
+        const bf16* from = base + row0 * ld + col;
+#pragma unroll 4
+        for (uint32_t i = 0; i < cpr / 2; ++i) {
+            const bool ok = r < rows;
+            copy16(dst + r * pitch + c * 16, ok ? from + r * ld + c * 8 : base, ok);
+            r += dr;
+            c += dc;
+            if (c >= cpr) {
+                c -= cpr;
+                ++r;
+            }
+        }
+    };
+    uint32_t base = 0, next = blockIdx.x * (kFewThreads / 32) + warp;  // items of a CTA's warps are neighbours: heads of the same keys
+    for (uint32_t c = 0; c < a.requests; c += kFewThreads) {
+        const uint32_t total = count_items<kFewThreads>(a, p, c, first, sums);
+        // the producer's item and key, the consumer's item
+        uint32_t ahead = next, key = 0, filled = 0;
+        Item pi;
+        pi.k_end = 0;
+        bool more = false;  // the producer has an item with keys left
+        uint32_t page = 0;  // of the producer's next step
+        auto look_up = [&]() {
+            if (a.lens) page = (uint32_t)__ldg(a.tables + (size_t)pi.request * a.table_ld + (key >> a.shift));
+        };
+        auto advance = [&]() {  // to an item that has keys
+            more = false;
+            while (ahead < base + total) {
+                pi = item_at<kFewThreads>(a, p, c, first, ahead - base);
+                ahead += warps;
+                if (pi.k_begin < pi.k_end) {
+                    more = true;
+                    key = pi.k_begin;
+                    look_up();
+                    return;
+                }
+            }
+        };
+        auto produce = [&]() {
+            if (more) {
+                const uint32_t dst = ring + filled * stage_bytes;
+                const bool there = !a.lens || page < a.pages;
+                const size_t row0 = !there ? 0 : a.lens ? ((size_t)page << a.shift) + (key & ((1u << a.shift) - 1)) : (size_t)pi.row0 + key;
+                const uint32_t rows = there ? min(16u, pi.k_end - key) : 0;
+                copy_rows(dst, kpitch, kc, a.k_ld, row0, pi.g * s.dimp, s.dimp, rows);
+                copy_rows(dst + k_bytes, vpitch, vc, a.v_ld, row0, pi.g * s.vdimp, s.vdimp, rows);
+                filled = filled + 1 == STAGES ? 0 : filled + 1;
+                key += 16;
+                if (key >= pi.k_end) advance();
+                else look_up();
+            }
+            copy_commit();
+        };
+        advance();
+        for (int i = 0; i < STAGES - 1; ++i) produce();
+        uint32_t stage = 0;
+        for (; next < base + total; next += warps) {
+            const Item it = item_at<kFewThreads>(a, p, c, first, next - base);
+            uint32_t token[2], head[2];
+            bool real[2];
+            int32_t see[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                real[h] = row_of(p, it, (lane >> 2) + 8 * h, 16, token[h], head[h]);
+                see[h] = real[h] ? seen_by(it, token[h]) : 0;
+            }
+            uint32_t qf[S][4];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const bf16* row = q + (size_t)(it.row0 + (real[h] ? token[h] : 0)) * a.q_ld + (size_t)(it.g * p.R + (real[h] ? head[h] : 0)) * s.dimp;
+#pragma unroll
+                for (int k = 0; k < S; ++k) {
+                    const uint32_t col = k * 16 + (lane & 3) * 2;
+                    const bool in = real[h] && k * 16u < s.dimp;
+                    qf[k][h] = in ? __ldg(reinterpret_cast<const uint32_t*>(row + col)) : 0u;
+                    qf[k][h + 2] = in ? __ldg(reinterpret_cast<const uint32_t*>(row + col + 8)) : 0u;
+                }
+            }
+            float o[S * 2][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+#pragma unroll
+            for (int v = 0; v < S * 2; ++v)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[v][e] = 0.0f;
+            for (uint32_t k0 = it.k_begin; k0 < it.k_end; k0 += 16) {
+                copy_wait<STAGES - 2>();
+                __syncwarp();
+                const uint32_t kt = ring + stage * stage_bytes, vt = kt + k_bytes;
+                float z[2][4] = {};
+                const uint32_t k_addr = kt + (((lane >> 4) << 3) + (lane & 7)) * kpitch + ((lane >> 3) & 1) * 16;
+#pragma unroll
+                for (int k = 0; k < S; ++k) {
+                    if (k * 16u >= s.dimp) break;
+                    uint32_t b[4];
+                    ldmatrix4(b, k_addr + k * 32);
+                    mma_bf16(z[0], qf[k], b[0], b[1]);
+                    mma_bf16(z[1], qf[k], b[2], b[3]);
+                }
+                float mx[2] = {m[0], m[1]};
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int32_t at = (int32_t)k0 + n * 8 + (lane & 3) * 2 + (e & 1);
+                        z[n][e] = at < min(see[e >> 1], (int32_t)it.k_end) ? z[n][e] * scale2 : -INFINITY;
+                        mx[e >> 1] = fmaxf(mx[e >> 1], z[n][e]);
+                    }
+                float shift[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xFFFFFFFFu, mx[h], 1));
+                    mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xFFFFFFFFu, mx[h], 2));
+                    shift[h] = mx[h] == -INFINITY ? 0.0f : mx[h];
+                }
+                if (__any_sync(0xFFFFFFFFu, mx[0] > m[0] || mx[1] > m[1])) {
+                    const float f0 = exp2f(m[0] - shift[0]), f1 = exp2f(m[1] - shift[1]);
+                    l[0] *= f0;
+                    l[1] *= f1;
+#pragma unroll
+                    for (int v = 0; v < S * 2; ++v) {
+                        o[v][0] *= f0; o[v][1] *= f0; o[v][2] *= f1; o[v][3] *= f1;
+                    }
+                    m[0] = mx[0];
+                    m[1] = mx[1];
+                }
+                uint32_t pw[4];
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    const float x0 = exp2f(z[n][0] - shift[0]), x1 = exp2f(z[n][1] - shift[0]), y0 = exp2f(z[n][2] - shift[1]), y1 = exp2f(z[n][3] - shift[1]);
+                    l[0] += x0 + x1;  // this lane's share; the four lanes of a row meet at the end
+                    l[1] += y0 + y1;
+                    pw[2 * n] = pack_bf16(x0, x1);
+                    pw[2 * n + 1] = pack_bf16(y0, y1);
+                }
+                const uint32_t v_addr = vt + (((lane >> 3) & 1) * 8 + (lane & 7)) * vpitch + (lane >> 4) * 16;
+#pragma unroll
+                for (int v = 0; v < S; ++v) {
+                    if (v * 16u >= s.vdimp) break;
+                    uint32_t b[4];
+                    ldmatrix4_trans(b, v_addr + v * 32);
+                    mma_bf16(o[2 * v], pw, b[0], b[1]);
+                    mma_bf16(o[2 * v + 1], pw, b[2], b[3]);
+                }
+                __syncwarp();
+                stage = stage + 1 == STAGES ? 0 : stage + 1;
+                produce();
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                l[h] += __shfl_xor_sync(0xFFFFFFFFu, l[h], 1);
+                l[h] += __shfl_xor_sync(0xFFFFFFFFu, l[h], 2);
+                if (!real[h]) continue;
+                const uint32_t row = it.row0 + token[h], hd = it.g * p.R + head[h], col0 = (lane & 3) * 2;
+                if (it.ranges == 1) {
+                    bf16* out = static_cast<bf16*>(a.out) + (size_t)row * a.out_pitch;
+                    bf16* mine = out + (size_t)hd * s.vdim;
+                    const float inv = m[h] > -INFINITY ? 1.0f / l[h] : 0.0f;
+                    const bool even = s.vdim % 2 == 0;
+#pragma unroll
+                    for (int v = 0; v < S * 2; ++v) {
+                        const uint32_t col = v * 8 + col0;
+                        const float x = o[v][2 * h] * inv, y = o[v][2 * h + 1] * inv;
+                        if (even && col < s.vdim) {
+                            *reinterpret_cast<uint32_t*>(mine + col) = pack_bf16(x, y);
+                        } else {
+                            if (col < s.vdim) mine[col] = __float2bfloat16_rn(x);
+                            if (col + 1 < s.vdim) mine[col + 1] = __float2bfloat16_rn(y);
+                        }
+                    }
+                    if (hd == 0)
+                        for (uint32_t e = s.heads * s.vdim + (lane & 3); e < a.out_pitch; e += 4) out[e] = __float2bfloat16_rn(0.0f);
+                } else {
+                    const size_t at = ((size_t)row * s.heads + hd) * p.max_ranges + it.range;
+                    float* part = p.part + at * s.vdimp;
+#pragma unroll
+                    for (int v = 0; v < S * 2; ++v)
+                        if (v * 8 + col0 < s.vdimp) *reinterpret_cast<float2*>(part + v * 8 + col0) = make_float2(o[v][2 * h], o[v][2 * h + 1]);
+                    if ((lane & 3) == 0)
+                        *reinterpret_cast<float2*>(p.part + (size_t)a.rows * s.heads * p.max_ranges * s.vdimp + at * 2) = make_float2(m[h], l[h]);
+                }
+                if (p.max_ranges > 1 && hd == 0 && it.range == 0 && (lane & 3) == 0) p.n_ranges[row] = it.ranges;
+            }
+        }
+        copy_wait<0>();
+        base += total;
+    }
+}
+
 // The ranges of a row and head, a warp each: out = sum of their values, each brought to the common maximum, over their sums. Rows of
 // one range are written already; rows behind the last request have none.
 template <typename T>
@@ -288,6 +506,18 @@ int plain_any(const RaggedCall& c, uint32_t M, cudaStream_t st) {
     return v <= 64 ? plain<T, 64, 64, 1>(c, st) : v <= 128 ? plain<T, 64, 64, 2>(c, st) : plain<T, 64, 64, 4>(c, st);
 }
 
+template <int D, int STAGES>
+int few(const RaggedCall& c, cudaStream_t st) {
+    const size_t smem = (size_t)(kFewThreads / 32) * STAGES * 16 * (c.a.s.dimp + 8 + c.a.s.vdimp + 8) * 2;
+    ZQ_CUDA(cudaFuncSetAttribute(ragged_few_kernel<D, STAGES>, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024));
+    const uint32_t per_sm = smem <= 54 * 1024 ? 4 : smem <= 73 * 1024 ? 3 : smem <= 111 * 1024 ? 2 : 1;
+    return done(launch_pdl(ragged_few_kernel<D, STAGES>, dim3(per_sm * sm_count()), dim3(kFewThreads), smem, st, c));
+}
+int few_any(const RaggedCall& c, cudaStream_t st) {
+    const uint32_t d = c.a.s.dimp > c.a.s.vdimp ? c.a.s.dimp : c.a.s.vdimp;
+    return d <= 64 ? few<64, 4>(c, st) : d <= 128 ? few<128, 3>(c, st) : few<256, 3>(c, st);
+}
+
 }  // namespace
 
 size_t ragged_work_bytes(const RaggedArgs& a, bool f32) {
@@ -300,7 +530,8 @@ int launch_ragged_attention(const RaggedArgs& a, bool f32, cudaStream_t st) {
     const uint32_t M = tile_rows(a);
     if (!f32 && M == 64 && ragged_tc_takes(a)) return launch_ragged_tc(a, st);
     const RaggedCall c{a, plan_of(a, M)};
-    int rc = f32 ? plain_any<float>(c, M, st) : plain_any<bf16>(c, M, st);
+    const bool large = a.s.dimp > 256 || a.s.vdimp > 256;
+    int rc = f32 ? plain_any<float>(c, M, st) : M == 16 && !large ? few_any(c, st) : plain_any<bf16>(c, M, st);
     if (rc != ZQ_OK || c.p.max_ranges < 2) return rc;
     const dim3 grid(((uint64_t)a.rows * a.s.heads + 3) / 4);
     return done(f32 ? launch_pdl(ragged_combine_kernel<float>, grid, dim3(128), 0, st, c)

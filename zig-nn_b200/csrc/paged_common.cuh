@@ -40,68 +40,76 @@ __host__ __device__ inline uint32_t ranges_of(uint32_t len, uint32_t fill, uint3
     return (len + per - 1) / per;
 }
 
-// Calls body(item) for the items of this CTA: every gridDim.x-th. All threads take the same way. The requests are looked at as many at
-// once as the CTA has threads: a prefix sum over their counts of items, then a bisection per item.
+__device__ __forceinline__ void span_of(const RaggedArgs& a, uint32_t i, uint32_t& row0, uint32_t& n_rows, int32_t& len) {
+    const int32_t b = a.row_start[i], e = a.row_start[i + 1];
+    row0 = b < 0 ? 0 : min((uint32_t)b, a.rows);
+    const uint32_t end = e < 0 ? 0 : min((uint32_t)e, a.rows);
+    n_rows = end > row0 ? end - row0 : 0;
+    len = a.lens ? min(a.lens[i], (int32_t)a.capacity) : (int32_t)n_rows;
+}
+
+// The items of up to THREADS requests from `c` on, those of the requests before one another: their sum, and a prefix sum in `first`
+// (THREADS + 1 values; sums: one per warp), which item_at searches. All threads of the CTA take part.
+template <uint32_t THREADS>
+__device__ __forceinline__ uint32_t count_items(const RaggedArgs& a, const RaggedPlan& p, uint32_t c, uint32_t* first, uint32_t* sums) {
+    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    uint32_t scan = 0;
+    if (c + tid < a.requests) {
+        uint32_t row0, n_rows, per;
+        int32_t len;
+        span_of(a, c + tid, row0, n_rows, len);
+        scan = (n_rows + p.tokens - 1) / p.tokens * ranges_of(len > 0 ? len : 0, p.fill, p.most_keys, per) * a.s.kv_heads * p.head_tiles;
+    }
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+        const uint32_t o = __shfl_up_sync(0xFFFFFFFFu, scan, off);
+        if (lane >= (uint32_t)off) scan += o;
+    }
+    __syncthreads();
+    if (lane == 31) sums[warp] = scan;
+    __syncthreads();
+    for (uint32_t w = 0; w < warp; ++w) scan += sums[w];
+    first[tid + 1] = scan;
+    if (tid == 0) first[0] = 0;
+    __syncthreads();
+    return first[THREADS];
+}
+
+// Item x of those requests.
+template <uint32_t THREADS>
+__device__ __forceinline__ Item item_at(const RaggedArgs& a, const RaggedPlan& p, uint32_t c, const uint32_t* first, uint32_t x) {
+    uint32_t lo = 0, hi = THREADS;
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) >> 1;
+        if (first[mid] <= x) lo = mid;
+        else hi = mid;
+    }
+    Item it;
+    it.request = c + lo;
+    span_of(a, it.request, it.row0, it.n_rows, it.len);
+    uint32_t per, u = x - first[lo];
+    const uint32_t len = it.len > 0 ? it.len : 0;
+    it.ranges = ranges_of(len, p.fill, p.most_keys, per);
+    it.head_tile = p.head_tiles > 1 ? u % p.head_tiles : 0;
+    u /= p.head_tiles;
+    it.g = u % a.s.kv_heads;
+    u /= a.s.kv_heads;
+    it.range = u % it.ranges;
+    it.tile = u / it.ranges;
+    it.k_begin = it.range * per;
+    it.k_end = min(len, it.k_begin + per);
+    return it;
+}
+
+// Calls body(item) for the items of this CTA: every gridDim.x-th. All threads take the same way.
 template <uint32_t THREADS, typename Body>
 __device__ __forceinline__ void for_items(const RaggedArgs& a, const RaggedPlan& p, Body body) {
     __shared__ uint32_t first[THREADS + 1];
     __shared__ uint32_t sums[THREADS / 32];
-    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, per_unit = a.s.kv_heads * p.head_tiles;
     uint32_t next = blockIdx.x, base = 0;
-    auto span_of = [&](uint32_t i, uint32_t& row0, uint32_t& n_rows, int32_t& len) {
-        const int32_t b = a.row_start[i], e = a.row_start[i + 1];
-        row0 = b < 0 ? 0 : min((uint32_t)b, a.rows);
-        const uint32_t end = e < 0 ? 0 : min((uint32_t)e, a.rows);
-        n_rows = end > row0 ? end - row0 : 0;
-        len = a.lens ? min(a.lens[i], (int32_t)a.capacity) : (int32_t)n_rows;
-    };
     for (uint32_t c = 0; c < a.requests; c += THREADS) {
-        uint32_t count = 0;
-        if (c + tid < a.requests) {
-            uint32_t row0, n_rows, per;
-            int32_t len;
-            span_of(c + tid, row0, n_rows, len);
-            count = (n_rows + p.tokens - 1) / p.tokens * ranges_of(len > 0 ? len : 0, p.fill, p.most_keys, per) * per_unit;
-        }
-        uint32_t scan = count;
-#pragma unroll
-        for (int off = 1; off < 32; off <<= 1) {
-            const uint32_t o = __shfl_up_sync(0xFFFFFFFFu, scan, off);
-            if (lane >= (uint32_t)off) scan += o;
-        }
-        __syncthreads();
-        if (lane == 31) sums[warp] = scan;
-        __syncthreads();
-        for (uint32_t w = 0; w < warp; ++w) scan += sums[w];
-        first[tid + 1] = scan;
-        if (tid == 0) first[0] = 0;
-        __syncthreads();
-        const uint32_t total = first[THREADS];
-        while (next < base + total) {
-            const uint32_t x = next - base;
-            uint32_t lo = 0, hi = THREADS;
-            while (hi - lo > 1) {
-                const uint32_t mid = (lo + hi) >> 1;
-                if (first[mid] <= x) lo = mid;
-                else hi = mid;
-            }
-            Item it;
-            it.request = c + lo;
-            span_of(it.request, it.row0, it.n_rows, it.len);
-            uint32_t per, u = x - first[lo];
-            const uint32_t len = it.len > 0 ? it.len : 0;
-            it.ranges = ranges_of(len, p.fill, p.most_keys, per);
-            it.head_tile = u % p.head_tiles;
-            u /= p.head_tiles;
-            it.g = u % a.s.kv_heads;
-            u /= a.s.kv_heads;
-            it.range = u % it.ranges;
-            it.tile = u / it.ranges;
-            it.k_begin = it.range * per;
-            it.k_end = min(len, it.k_begin + per);
-            body(it);
-            next += gridDim.x;
-        }
+        const uint32_t total = count_items<THREADS>(a, p, c, first, sums);
+        for (; next < base + total; next += gridDim.x) body(item_at<THREADS>(a, p, c, first, next - base));
         base += total;
     }
 }
