@@ -200,20 +200,23 @@ ragged_plain_kernel(const __grid_constant__ RaggedCall call) {
 // against 2 D / 8 + 2 V / 8 MMAs).
 constexpr uint32_t kFewThreads = 128;
 
-template <int D, int STAGES>
+// FULL: keys and values have D dimensions, which spares the copies their counting.
+constexpr float kFewRaise = 16.0f;  // powers of two that the maximum may lag behind
+
+template <int D, int STAGES, bool FULL>
 __global__ void __launch_bounds__(kFewThreads)
 ragged_few_kernel(const __grid_constant__ RaggedCall call) {
     constexpr int S = D / 16;
     extern __shared__ __align__(16) unsigned char smem[];
-    __shared__ uint32_t first[kFewThreads + 1];
-    __shared__ uint32_t sums[kFewThreads / 32];
+    __shared__ Requests<kFewThreads> rq;
     pdl_launch_dependents();
     pdl_wait();
     const RaggedArgs& a = call.a;
     const RaggedPlan& p = call.p;
     const GqaShape& s = a.s;
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = gridDim.x * (kFewThreads / 32);
-    const uint32_t kpitch = (s.dimp + 8) * 2, vpitch = (s.vdimp + 8) * 2, k_bytes = 16 * kpitch, stage_bytes = k_bytes + 16 * vpitch;
+    const uint32_t dimp = FULL ? D : s.dimp, vdimp = FULL ? D : s.vdimp;
+    const uint32_t kpitch = (dimp + 8) * 2, vpitch = (vdimp + 8) * 2, k_bytes = 16 * kpitch, stage_bytes = k_bytes + 16 * vpitch;
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * STAGES * stage_bytes;
     const bf16 *q = static_cast<const bf16*>(a.q), *kc = static_cast<const bf16*>(a.k), *vc = static_cast<const bf16*>(a.v);
     const float scale2 = a.scale * kLog2e;
@@ -223,34 +226,45 @@ ragged_few_kernel(const __grid_constant__ RaggedCall call) {
         const uint32_t cpr = dp / 8, dr = 32 / cpr, dc = 32 % cpr;
         uint32_t r = lane / cpr, c = lane % cpr;
         const bf16* from = base + row0 * ld + col;
-#pragma unroll 4
-        for (uint32_t i = 0; i < cpr / 2; ++i) {
-            const bool ok = r < rows;
-            copy16(dst + r * pitch + c * 16, ok ? from + r * ld + c * 8 : base, ok);
-            r += dr;
-            c += dc;
-            if (c >= cpr) {
-                c -= cpr;
-                ++r;
+        if constexpr (FULL) {  // whole rows apart: D / 8 lanes a row (D = 256: a row)
+            from += (D == 256 ? 0 : r) * ld + c * 8;
+            dst += r * pitch + c * 16;
+            const size_t step = (D == 256 ? 1 : dr) * ld;
+            if (rows == 16) {
+#pragma unroll
+                for (uint32_t i = 0; i < D / 16; ++i, from += step, dst += dr * pitch) copy16(dst, from, true);
+            } else {
+#pragma unroll 1
+                for (uint32_t i = 0; i < D / 16; ++i, from += step, dst += dr * pitch, r += dr) copy16(dst, r < rows ? from : base, r < rows);
+            }
+        } else {
+#pragma unroll 1
+            for (uint32_t i = 0; i < cpr / 2; ++i) {
+                const bool ok = r < rows;
+                copy16(dst + r * pitch + c * 16, ok ? from + r * ld + c * 8 : base, ok);
+                r += dr;
+                c += dc;
+                if (c >= cpr) {
+                    c -= cpr;
+                    ++r;
+                }
             }
         }
     };
     uint32_t base = 0, next = blockIdx.x * (kFewThreads / 32) + warp;  // items of a CTA's warps are neighbours: heads of the same keys
     for (uint32_t c = 0; c < a.requests; c += kFewThreads) {
-        const uint32_t total = count_items<kFewThreads>(a, p, c, first, sums);
-        // the producer's item and key, the consumer's item
-        uint32_t ahead = next, key = 0, filled = 0;
+        const uint32_t total = count_items<kFewThreads>(a, p, c, rq);
+        // what the copies are at: an item, its next key, the page of that, the stage to fill
+        uint32_t ahead = next, key = 0, filled = 0, page = 0;
         Item pi;
-        pi.k_end = 0;
-        bool more = false;  // the producer has an item with keys left
-        uint32_t page = 0;  // of the producer's next step
+        bool more = false;  // there is such a key
         auto look_up = [&]() {
             if (a.lens) page = (uint32_t)__ldg(a.tables + (size_t)pi.request * a.table_ld + (key >> a.shift));
         };
         auto advance = [&]() {  // to an item that has keys
             more = false;
             while (ahead < base + total) {
-                pi = item_at<kFewThreads>(a, p, c, first, ahead - base);
+                pi = item_at<kFewThreads>(a, p, c, rq, ahead - base);
                 ahead += warps;
                 if (pi.k_begin < pi.k_end) {
                     more = true;
@@ -265,41 +279,43 @@ ragged_few_kernel(const __grid_constant__ RaggedCall call) {
                 const uint32_t dst = ring + filled * stage_bytes;
                 const bool there = !a.lens || page < a.pages;
                 const size_t row0 = !there ? 0 : a.lens ? ((size_t)page << a.shift) + (key & ((1u << a.shift) - 1)) : (size_t)pi.row0 + key;
-                const uint32_t rows = there ? min(16u, pi.k_end - key) : 0;
-                copy_rows(dst, kpitch, kc, a.k_ld, row0, pi.g * s.dimp, s.dimp, rows);
-                copy_rows(dst + k_bytes, vpitch, vc, a.v_ld, row0, pi.g * s.vdimp, s.vdimp, rows);
-                filled = filled + 1 == STAGES ? 0 : filled + 1;
+                const uint32_t rows = there ? min(16u, pi.k_end - key) : 0, g = pi.g;
                 key += 16;
+                if (key < pi.k_end) look_up();
+                copy_rows(dst, kpitch, kc, a.k_ld, row0, g * dimp, dimp, rows);
+                copy_rows(dst + k_bytes, vpitch, vc, a.v_ld, row0, g * vdimp, vdimp, rows);
+                filled = filled + 1 == STAGES ? 0 : filled + 1;
                 if (key >= pi.k_end) advance();
-                else look_up();
             }
             copy_commit();
         };
         advance();
         for (int i = 0; i < STAGES - 1; ++i) produce();
         uint32_t stage = 0;
-        for (; next < base + total; next += warps) {
-            const Item it = item_at<kFewThreads>(a, p, c, first, next - base);
-            uint32_t token[2], head[2];
-            bool real[2];
-            int32_t see[2];
+        Item it;
+        uint32_t token[2], head[2], qf[S][4];
+        bool real[2];
+        auto enter = [&]() {  // the item `next`: its rows' queries, requested ahead of the stores of the item before
+            it = item_at<kFewThreads>(a, p, c, rq, next - base);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 real[h] = row_of(p, it, (lane >> 2) + 8 * h, 16, token[h], head[h]);
-                see[h] = real[h] ? seen_by(it, token[h]) : 0;
-            }
-            uint32_t qf[S][4];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const bf16* row = q + (size_t)(it.row0 + (real[h] ? token[h] : 0)) * a.q_ld + (size_t)(it.g * p.R + (real[h] ? head[h] : 0)) * s.dimp;
+                const bf16* row = q + (size_t)(it.row0 + (real[h] ? token[h] : 0)) * a.q_ld + (size_t)(it.g * p.R + (real[h] ? head[h] : 0)) * dimp + (lane & 3) * 2;
 #pragma unroll
                 for (int k = 0; k < S; ++k) {
-                    const uint32_t col = k * 16 + (lane & 3) * 2;
-                    const bool in = real[h] && k * 16u < s.dimp;
-                    qf[k][h] = in ? __ldg(reinterpret_cast<const uint32_t*>(row + col)) : 0u;
-                    qf[k][h + 2] = in ? __ldg(reinterpret_cast<const uint32_t*>(row + col + 8)) : 0u;
+                    const bool in = real[h] && (FULL || k * 16u < dimp);
+                    qf[k][h] = in ? __ldg(reinterpret_cast<const uint32_t*>(row + k * 16)) : 0u;
+                    qf[k][h + 2] = in ? __ldg(reinterpret_cast<const uint32_t*>(row + k * 16 + 8)) : 0u;
                 }
             }
+        };
+        if (next < base + total) enter();
+        while (next < base + total) {
+            int32_t see[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) see[h] = real[h] ? min(seen_by(it, token[h]), (int32_t)it.k_end) : 0;
+            // keys that every real row sees
+            const int32_t all = min(seen_by(it, it.tile * p.tokens), (int32_t)it.k_end);
             float o[S * 2][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
 #pragma unroll
             for (int v = 0; v < S * 2; ++v)
@@ -309,43 +325,49 @@ ragged_few_kernel(const __grid_constant__ RaggedCall call) {
                 copy_wait<STAGES - 2>();
                 __syncwarp();
                 const uint32_t kt = ring + stage * stage_bytes, vt = kt + k_bytes;
-                float z[2][4] = {};
+                float z[2][4] = {}, y[2][4] = {};  // even and odd steps of the dimensions: two chains each
                 const uint32_t k_addr = kt + (((lane >> 4) << 3) + (lane & 7)) * kpitch + ((lane >> 3) & 1) * 16;
 #pragma unroll
                 for (int k = 0; k < S; ++k) {
-                    if (k * 16u >= s.dimp) break;
+                    if (!FULL && k * 16u >= dimp) break;
                     uint32_t b[4];
                     ldmatrix4(b, k_addr + k * 32);
-                    mma_bf16(z[0], qf[k], b[0], b[1]);
-                    mma_bf16(z[1], qf[k], b[2], b[3]);
+                    mma_bf16(k & 1 ? y[0] : z[0], qf[k], b[0], b[1]);
+                    mma_bf16(k & 1 ? y[1] : z[1], qf[k], b[2], b[3]);
                 }
-                float mx[2] = {m[0], m[1]};
+                float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
                 for (int n = 0; n < 2; ++n)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int32_t at = (int32_t)k0 + n * 8 + (lane & 3) * 2 + (e & 1);
-                        z[n][e] = at < min(see[e >> 1], (int32_t)it.k_end) ? z[n][e] * scale2 : -INFINITY;
-                        mx[e >> 1] = fmaxf(mx[e >> 1], z[n][e]);
-                    }
-                float shift[2];
+                    for (int e = 0; e < 4; ++e) z[n][e] = (z[n][e] + y[n][e]) * scale2;
+                if ((int32_t)k0 + 16 > all) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xFFFFFFFFu, mx[h], 1));
-                    mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xFFFFFFFFu, mx[h], 2));
-                    shift[h] = mx[h] == -INFINITY ? 0.0f : mx[h];
+                    for (int n = 0; n < 2; ++n)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if ((int32_t)(k0 + n * 8 + (lane & 3) * 2 + (e & 1)) >= see[e >> 1]) z[n][e] = -INFINITY;
                 }
-                if (__any_sync(0xFFFFFFFFu, mx[0] > m[0] || mx[1] > m[1])) {
-                    const float f0 = exp2f(m[0] - shift[0]), f1 = exp2f(m[1] - shift[1]);
-                    l[0] *= f0;
-                    l[1] *= f1;
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) mx[e >> 1] = fmaxf(mx[e >> 1], z[n][e]);
+                // The weights are taken against an older maximum while none exceeds it by more than 2^kFewRaise: no exchange in a step.
+                if (__any_sync(0xFFFFFFFFu, mx[0] > m[0] + kFewRaise || mx[1] > m[1] + kFewRaise)) {
+                    float f[2];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xFFFFFFFFu, mx[h], 1));
+                        mx[h] = fmaxf(fmaxf(mx[h], __shfl_xor_sync(0xFFFFFFFFu, mx[h], 2)), m[h]);
+                        f[h] = m[h] == -INFINITY ? 0.0f : exp2f(m[h] - mx[h]);
+                        m[h] = mx[h];
+                        l[h] *= f[h];
+                    }
 #pragma unroll
                     for (int v = 0; v < S * 2; ++v) {
-                        o[v][0] *= f0; o[v][1] *= f0; o[v][2] *= f1; o[v][3] *= f1;
+                        o[v][0] *= f[0]; o[v][1] *= f[0]; o[v][2] *= f[1]; o[v][3] *= f[1];
                     }
-                    m[0] = mx[0];
-                    m[1] = mx[1];
                 }
+                const float shift[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
                 uint32_t pw[4];
 #pragma unroll
                 for (int n = 0; n < 2; ++n) {
@@ -358,7 +380,7 @@ ragged_few_kernel(const __grid_constant__ RaggedCall call) {
                 const uint32_t v_addr = vt + (((lane >> 3) & 1) * 8 + (lane & 7)) * vpitch + (lane >> 4) * 16;
 #pragma unroll
                 for (int v = 0; v < S; ++v) {
-                    if (v * 16u >= s.vdimp) break;
+                    if (!FULL && v * 16u >= vdimp) break;
                     uint32_t b[4];
                     ldmatrix4_trans(b, v_addr + v * 32);
                     mma_bf16(o[2 * v], pw, b[0], b[1]);
@@ -368,13 +390,18 @@ ragged_few_kernel(const __grid_constant__ RaggedCall call) {
                 stage = stage + 1 == STAGES ? 0 : stage + 1;
                 produce();
             }
+            const Item was = it;
+            const uint32_t was_token[2] = {token[0], token[1]}, was_head[2] = {head[0], head[1]};
+            const bool was_real[2] = {real[0], real[1]};
+            next += warps;
+            if (next < base + total) enter();
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 l[h] += __shfl_xor_sync(0xFFFFFFFFu, l[h], 1);
                 l[h] += __shfl_xor_sync(0xFFFFFFFFu, l[h], 2);
-                if (!real[h]) continue;
-                const uint32_t row = it.row0 + token[h], hd = it.g * p.R + head[h], col0 = (lane & 3) * 2;
-                if (it.ranges == 1) {
+                if (!was_real[h]) continue;
+                const uint32_t row = was.row0 + was_token[h], hd = was.g * p.R + was_head[h], col0 = (lane & 3) * 2;
+                if (was.ranges == 1) {
                     bf16* out = static_cast<bf16*>(a.out) + (size_t)row * a.out_pitch;
                     bf16* mine = out + (size_t)hd * s.vdim;
                     const float inv = m[h] > -INFINITY ? 1.0f / l[h] : 0.0f;
@@ -393,15 +420,15 @@ ragged_few_kernel(const __grid_constant__ RaggedCall call) {
                     if (hd == 0)
                         for (uint32_t e = s.heads * s.vdim + (lane & 3); e < a.out_pitch; e += 4) out[e] = __float2bfloat16_rn(0.0f);
                 } else {
-                    const size_t at = ((size_t)row * s.heads + hd) * p.max_ranges + it.range;
-                    float* part = p.part + at * s.vdimp;
+                    const size_t at = ((size_t)row * s.heads + hd) * p.max_ranges + was.range;
+                    float* part = p.part + at * vdimp;
 #pragma unroll
                     for (int v = 0; v < S * 2; ++v)
-                        if (v * 8 + col0 < s.vdimp) *reinterpret_cast<float2*>(part + v * 8 + col0) = make_float2(o[v][2 * h], o[v][2 * h + 1]);
+                        if (FULL || v * 8 + col0 < vdimp) *reinterpret_cast<float2*>(part + v * 8 + col0) = make_float2(o[v][2 * h], o[v][2 * h + 1]);
                     if ((lane & 3) == 0)
-                        *reinterpret_cast<float2*>(p.part + (size_t)a.rows * s.heads * p.max_ranges * s.vdimp + at * 2) = make_float2(m[h], l[h]);
+                        *reinterpret_cast<float2*>(p.part + (size_t)a.rows * s.heads * p.max_ranges * vdimp + at * 2) = make_float2(m[h], l[h]);
                 }
-                if (p.max_ranges > 1 && hd == 0 && it.range == 0 && (lane & 3) == 0) p.n_ranges[row] = it.ranges;
+                if (p.max_ranges > 1 && hd == 0 && was.range == 0 && (lane & 3) == 0) p.n_ranges[row] = was.ranges;
             }
         }
         copy_wait<0>();
@@ -506,16 +533,21 @@ int plain_any(const RaggedCall& c, uint32_t M, cudaStream_t st) {
     return v <= 64 ? plain<T, 64, 64, 1>(c, st) : v <= 128 ? plain<T, 64, 64, 2>(c, st) : plain<T, 64, 64, 4>(c, st);
 }
 
-template <int D, int STAGES>
+template <int D, int STAGES, bool FULL>
 int few(const RaggedCall& c, cudaStream_t st) {
     const size_t smem = (size_t)(kFewThreads / 32) * STAGES * 16 * (c.a.s.dimp + 8 + c.a.s.vdimp + 8) * 2;
-    ZQ_CUDA(cudaFuncSetAttribute(ragged_few_kernel<D, STAGES>, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024));
-    const uint32_t per_sm = smem <= 54 * 1024 ? 4 : smem <= 73 * 1024 ? 3 : smem <= 111 * 1024 ? 2 : 1;
-    return done(launch_pdl(ragged_few_kernel<D, STAGES>, dim3(per_sm * sm_count()), dim3(kFewThreads), smem, st, c));
+    ZQ_CUDA(cudaFuncSetAttribute(ragged_few_kernel<D, STAGES, FULL>, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024));
+    const uint32_t per_sm = smem <= 51 * 1024 ? 4 : smem <= 70 * 1024 ? 3 : smem <= 108 * 1024 ? 2 : 1;
+    return done(launch_pdl(ragged_few_kernel<D, STAGES, FULL>, dim3(per_sm * sm_count()), dim3(kFewThreads), smem, st, c));
 }
 int few_any(const RaggedCall& c, cudaStream_t st) {
     const uint32_t d = c.a.s.dimp > c.a.s.vdimp ? c.a.s.dimp : c.a.s.vdimp;
-    return d <= 64 ? few<64, 4>(c, st) : d <= 128 ? few<128, 3>(c, st) : few<256, 3>(c, st);
+    if (c.a.s.dimp == c.a.s.vdimp) {
+        if (d == 64) return few<64, 3, true>(c, st);
+        if (d == 128) return few<128, 3, true>(c, st);
+        if (d == 256) return few<256, 3, true>(c, st);
+    }
+    return d <= 64 ? few<64, 3, false>(c, st) : d <= 128 ? few<128, 3, false>(c, st) : few<256, 3, false>(c, st);
 }
 
 }  // namespace
@@ -534,8 +566,8 @@ int launch_ragged_attention(const RaggedArgs& a, bool f32, cudaStream_t st) {
     int rc = f32 ? plain_any<float>(c, M, st) : M == 16 && !large ? few_any(c, st) : plain_any<bf16>(c, M, st);
     if (rc != ZQ_OK || c.p.max_ranges < 2) return rc;
     const dim3 grid(((uint64_t)a.rows * a.s.heads + 3) / 4);
-    return done(f32 ? launch_pdl(ragged_combine_kernel<float>, grid, dim3(128), 0, st, c)
-                    : launch_pdl(ragged_combine_kernel<bf16>, grid, dim3(128), 0, st, c));
+    return done(f32 ? launch_pdl_split(true, ragged_combine_kernel<float>, grid, dim3(128), 0, st, c)
+                    : launch_pdl_split(true, ragged_combine_kernel<bf16>, grid, dim3(128), 0, st, c));
 }
 
 }  // namespace zq

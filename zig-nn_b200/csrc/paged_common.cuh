@@ -48,17 +48,25 @@ __device__ __forceinline__ void span_of(const RaggedArgs& a, uint32_t i, uint32_
     len = a.lens ? min(a.lens[i], (int32_t)a.capacity) : (int32_t)n_rows;
 }
 
-// The items of up to THREADS requests from `c` on, those of the requests before one another: their sum, and a prefix sum in `first`
-// (THREADS + 1 values; sums: one per warp), which item_at searches. All threads of the CTA take part.
+// Up to THREADS requests from one on: their items before one another, and what item_at needs of each.
 template <uint32_t THREADS>
-__device__ __forceinline__ uint32_t count_items(const RaggedArgs& a, const RaggedPlan& p, uint32_t c, uint32_t* first, uint32_t* sums) {
+struct Requests {
+    uint32_t first[THREADS + 1];  // prefix sum of their items
+    uint32_t row0[THREADS], n_rows[THREADS], ranges[THREADS], per[THREADS];
+    int32_t len[THREADS];
+    uint32_t sums[THREADS / 32];
+};
+
+// Of the requests from `c` on, by all threads of the CTA: how many items they have.
+template <uint32_t THREADS>
+__device__ __forceinline__ uint32_t count_items(const RaggedArgs& a, const RaggedPlan& p, uint32_t c, Requests<THREADS>& q) {
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    uint32_t scan = 0;
+    uint32_t row0 = 0, n_rows = 0, per = kRangeKeys, ranges = 1, scan = 0;
+    int32_t len = 0;
     if (c + tid < a.requests) {
-        uint32_t row0, n_rows, per;
-        int32_t len;
         span_of(a, c + tid, row0, n_rows, len);
-        scan = (n_rows + p.tokens - 1) / p.tokens * ranges_of(len > 0 ? len : 0, p.fill, p.most_keys, per) * a.s.kv_heads * p.head_tiles;
+        ranges = ranges_of(len > 0 ? len : 0, p.fill, p.most_keys, per);
+        scan = (p.tokens > 1 ? (n_rows + p.tokens - 1) / p.tokens : n_rows) * ranges * a.s.kv_heads * p.head_tiles;
     }
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
@@ -66,50 +74,62 @@ __device__ __forceinline__ uint32_t count_items(const RaggedArgs& a, const Ragge
         if (lane >= (uint32_t)off) scan += o;
     }
     __syncthreads();
-    if (lane == 31) sums[warp] = scan;
+    if (lane == 31) q.sums[warp] = scan;
+    q.row0[tid] = row0;
+    q.n_rows[tid] = n_rows;
+    q.ranges[tid] = ranges;
+    q.per[tid] = per;
+    q.len[tid] = len;
     __syncthreads();
-    for (uint32_t w = 0; w < warp; ++w) scan += sums[w];
-    first[tid + 1] = scan;
-    if (tid == 0) first[0] = 0;
+    for (uint32_t w = 0; w < warp; ++w) scan += q.sums[w];
+    q.first[tid + 1] = scan;
+    if (tid == 0) q.first[0] = 0;
     __syncthreads();
-    return first[THREADS];
+    return q.first[THREADS];
 }
 
 // Item x of those requests.
 template <uint32_t THREADS>
-__device__ __forceinline__ Item item_at(const RaggedArgs& a, const RaggedPlan& p, uint32_t c, const uint32_t* first, uint32_t x) {
+__device__ __forceinline__ Item item_at(const RaggedArgs& a, const RaggedPlan& p, uint32_t c, const Requests<THREADS>& q, uint32_t x) {
     uint32_t lo = 0, hi = THREADS;
     while (hi - lo > 1) {
         const uint32_t mid = (lo + hi) >> 1;
-        if (first[mid] <= x) lo = mid;
+        if (q.first[mid] <= x) lo = mid;
         else hi = mid;
     }
     Item it;
     it.request = c + lo;
-    span_of(a, it.request, it.row0, it.n_rows, it.len);
-    uint32_t per, u = x - first[lo];
-    const uint32_t len = it.len > 0 ? it.len : 0;
-    it.ranges = ranges_of(len, p.fill, p.most_keys, per);
-    it.head_tile = p.head_tiles > 1 ? u % p.head_tiles : 0;
-    u /= p.head_tiles;
+    it.row0 = q.row0[lo];
+    it.n_rows = q.n_rows[lo];
+    it.len = q.len[lo];
+    it.ranges = q.ranges[lo];
+    uint32_t u = x - q.first[lo];
+    it.head_tile = 0;
+    if (p.head_tiles > 1) {
+        it.head_tile = u % p.head_tiles;
+        u /= p.head_tiles;
+    }
     it.g = u % a.s.kv_heads;
     u /= a.s.kv_heads;
-    it.range = u % it.ranges;
-    it.tile = u / it.ranges;
-    it.k_begin = it.range * per;
-    it.k_end = min(len, it.k_begin + per);
+    it.tile = 0;
+    if (it.n_rows > p.tokens) {
+        it.tile = u / it.ranges;
+        u -= it.tile * it.ranges;
+    }
+    it.range = u;
+    it.k_begin = u * q.per[lo];
+    it.k_end = min(it.len > 0 ? (uint32_t)it.len : 0u, it.k_begin + q.per[lo]);
     return it;
 }
 
 // Calls body(item) for the items of this CTA: every gridDim.x-th. All threads take the same way.
 template <uint32_t THREADS, typename Body>
 __device__ __forceinline__ void for_items(const RaggedArgs& a, const RaggedPlan& p, Body body) {
-    __shared__ uint32_t first[THREADS + 1];
-    __shared__ uint32_t sums[THREADS / 32];
+    __shared__ Requests<THREADS> q;
     uint32_t next = blockIdx.x, base = 0;
     for (uint32_t c = 0; c < a.requests; c += THREADS) {
-        const uint32_t total = count_items<THREADS>(a, p, c, first, sums);
-        for (; next < base + total; next += gridDim.x) body(item_at<THREADS>(a, p, c, first, next - base));
+        const uint32_t total = count_items<THREADS>(a, p, c, q);
+        for (; next < base + total; next += gridDim.x) body(item_at<THREADS>(a, p, c, q, next - base));
         base += total;
     }
 }
