@@ -583,17 +583,22 @@ class GqaCache:
 PLAN_PAGES, PLAN_TABLE, PLAN_ROWS, PLAN_INCONSISTENT = 1, 2, 4, 8
 
 
+_current_device = torch._C._cuda_getDevice
+
+
 def _int_rows(t, name, *shape):
     """t, a contiguous int32 tensor of that shape (-1: any) on the current device."""
-    if not (isinstance(t, torch.Tensor) and t.dtype == torch.int32 and t.is_cuda and t.is_contiguous() and t.dim() == len(shape)
-            and all(n in (-1, m) for n, m in zip(shape, t.shape))):
-        raise ValueError("%s: expected a contiguous int32 CUDA tensor of shape %s" % (name, list(shape)))
-    return _here(t, name)
+    if isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.is_contiguous():
+        have = t.shape
+        if have == shape or (len(have) == len(shape) and all(n == -1 or n == m for n, m in zip(shape, have))):
+            if t.get_device() == _current_device():
+                return t
+    raise ValueError("%s: expected a contiguous int32 tensor of shape %s on CUDA device %d" % (name, list(shape), _current_device()))
 
 
 def _here(t, name):
-    if t.get_device() != torch._C._cuda_getDevice():
-        raise ValueError("%s is on device %d, the current one is %d" % (name, t.get_device(), torch._C._cuda_getDevice()))
+    if t.get_device() != _current_device():
+        raise ValueError("%s is on device %d, the current one is %d" % (name, t.get_device(), _current_device()))
     return t
 
 

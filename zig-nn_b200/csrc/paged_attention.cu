@@ -3,6 +3,8 @@
 //   * more rows (bf16): paged_attention_tc.cu;
 //   * f32, and heads beyond 256 dimensions: tiles of 16 or 64 packed rows against tiles of keys, plain multiply-adds;
 //   * where a request's keys are cut into ranges, the ranges meet in a second small kernel.
+#include <atomic>
+
 #include "paged_common.cuh"
 #include "tile_common.cuh"
 
@@ -290,13 +292,11 @@ ragged_few_kernel(const __grid_constant__ RaggedCall call) {
             copy_commit();
         };
         advance();
-        for (int i = 0; i < STAGES - 1; ++i) produce();
-        uint32_t stage = 0;
-        Item it;
-        uint32_t token[2], head[2], qf[S][4];
-        bool real[2];
-        auto enter = [&]() {  // the item `next`: its rows' queries, requested ahead of the stores of the item before
-            it = item_at<kFewThreads>(a, p, c, rq, next - base);
+        uint32_t stage = 0, pending = 0;  // pending: steps asked for and not yet worked on
+        for (; next < base + total; next += warps) {
+            const Item it = item_at<kFewThreads>(a, p, c, rq, next - base);
+            uint32_t token[2], head[2], qf[S][4];
+            bool real[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 real[h] = row_of(p, it, (lane >> 2) + 8 * h, 16, token[h], head[h]);
@@ -308,9 +308,6 @@ ragged_few_kernel(const __grid_constant__ RaggedCall call) {
                     qf[k][h + 2] = in ? __ldg(reinterpret_cast<const uint32_t*>(row + k * 16 + 8)) : 0u;
                 }
             }
-        };
-        if (next < base + total) enter();
-        while (next < base + total) {
             int32_t see[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) see[h] = real[h] ? min(seen_by(it, token[h]), (int32_t)it.k_end) : 0;
@@ -321,7 +318,9 @@ ragged_few_kernel(const __grid_constant__ RaggedCall call) {
             for (int v = 0; v < S * 2; ++v)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[v][e] = 0.0f;
-            for (uint32_t k0 = it.k_begin; k0 < it.k_end; k0 += 16) {
+            for (uint32_t k0 = it.k_begin; k0 < it.k_end; k0 += 16, --pending) {
+#pragma unroll 1
+                for (; pending < STAGES - 1; ++pending) produce();
                 copy_wait<STAGES - 2>();
                 __syncwarp();
                 const uint32_t kt = ring + stage * stage_bytes, vt = kt + k_bytes;
@@ -388,20 +387,14 @@ ragged_few_kernel(const __grid_constant__ RaggedCall call) {
                 }
                 __syncwarp();
                 stage = stage + 1 == STAGES ? 0 : stage + 1;
-                produce();
             }
-            const Item was = it;
-            const uint32_t was_token[2] = {token[0], token[1]}, was_head[2] = {head[0], head[1]};
-            const bool was_real[2] = {real[0], real[1]};
-            next += warps;
-            if (next < base + total) enter();
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 l[h] += __shfl_xor_sync(0xFFFFFFFFu, l[h], 1);
                 l[h] += __shfl_xor_sync(0xFFFFFFFFu, l[h], 2);
-                if (!was_real[h]) continue;
-                const uint32_t row = was.row0 + was_token[h], hd = was.g * p.R + was_head[h], col0 = (lane & 3) * 2;
-                if (was.ranges == 1) {
+                if (!real[h]) continue;
+                const uint32_t row = it.row0 + token[h], hd = it.g * p.R + head[h], col0 = (lane & 3) * 2;
+                if (it.ranges == 1) {
                     bf16* out = static_cast<bf16*>(a.out) + (size_t)row * a.out_pitch;
                     bf16* mine = out + (size_t)hd * s.vdim;
                     const float inv = m[h] > -INFINITY ? 1.0f / l[h] : 0.0f;
@@ -420,7 +413,7 @@ ragged_few_kernel(const __grid_constant__ RaggedCall call) {
                     if (hd == 0)
                         for (uint32_t e = s.heads * s.vdim + (lane & 3); e < a.out_pitch; e += 4) out[e] = __float2bfloat16_rn(0.0f);
                 } else {
-                    const size_t at = ((size_t)row * s.heads + hd) * p.max_ranges + was.range;
+                    const size_t at = ((size_t)row * s.heads + hd) * p.max_ranges + it.range;
                     float* part = p.part + at * vdimp;
 #pragma unroll
                     for (int v = 0; v < S * 2; ++v)
@@ -428,7 +421,7 @@ ragged_few_kernel(const __grid_constant__ RaggedCall call) {
                     if ((lane & 3) == 0)
                         *reinterpret_cast<float2*>(p.part + (size_t)a.rows * s.heads * p.max_ranges * vdimp + at * 2) = make_float2(m[h], l[h]);
                 }
-                if (p.max_ranges > 1 && hd == 0 && was.range == 0 && (lane & 3) == 0) p.n_ranges[row] = was.ranges;
+                if (p.max_ranges > 1 && hd == 0 && it.range == 0 && (lane & 3) == 0) p.n_ranges[row] = it.ranges;
             }
         }
         copy_wait<0>();
@@ -437,7 +430,8 @@ ragged_few_kernel(const __grid_constant__ RaggedCall call) {
 }
 
 // The ranges of a row and head, a warp each: out = sum of their values, each brought to the common maximum, over their sums. Rows of
-// one range are written already; rows behind the last request have none.
+// one range are written already; rows behind the last request have none. A chain of loads is what it takes: how many ranges, their
+// maxima and sums (a lane each, 32 at a time), their values (eight at a time).
 template <typename T>
 __global__ void __launch_bounds__(128)
 ragged_combine_kernel(const __grid_constant__ RaggedCall call) {
@@ -447,32 +441,45 @@ ragged_combine_kernel(const __grid_constant__ RaggedCall call) {
     const RaggedPlan& p = call.p;
     const GqaShape& s = a.s;
     const uint32_t lane = threadIdx.x & 31, unit = blockIdx.x * 4 + (threadIdx.x >> 5), row = unit / s.heads, h = unit % s.heads;
-    if (row >= a.rows || (int32_t)row >= a.row_start[a.requests] || (int32_t)row < a.row_start[0]) return;
-    const uint32_t n = p.n_ranges[row];
-    if (n < 2) return;
+    if (row >= a.rows) return;
+    const int32_t begin = a.row_start[0], end = a.row_start[a.requests];
+    const uint32_t n = p.n_ranges[row];  // of a row that is none: whatever lies there
     const size_t at = (size_t)unit * p.max_ranges;
     const float* part = p.part + at * s.vdimp;
     const float2* ml = reinterpret_cast<const float2*>(p.part + (size_t)a.rows * s.heads * p.max_ranges * s.vdimp) + at;
-    float mx = -INFINITY;
-    for (uint32_t i = lane; i < n; i += 32) mx = fmaxf(mx, ml[i].x);
+    float2 mine = lane < p.max_ranges ? ml[lane] : make_float2(-INFINITY, 0.0f);
+    if ((int32_t)row >= end || (int32_t)row < begin || n < 2 || n > p.max_ranges) return;
+    if (lane >= n) mine = make_float2(-INFINITY, 0.0f);
+    float mx = mine.x;
+    for (uint32_t i = lane + 32; i < n; i += 32) mx = fmaxf(mx, ml[i].x);
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, off));
     const float shift = mx == -INFINITY ? 0.0f : mx;
-    float sum = 0.0f;
-    for (uint32_t i = lane; i < n; i += 32) sum += exp2f(ml[i].x - shift) * ml[i].y;
+    float sum = exp2f(mine.x - shift) * mine.y;
+    for (uint32_t i = lane + 32; i < n; i += 32) sum += exp2f(ml[i].x - shift) * ml[i].y;
     sum = warp_sum_f(sum);
-    const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+    const float inv = mx > -INFINITY ? 1.0f / sum : 0.0f;
     T* out = static_cast<T*>(a.out) + (size_t)row * a.out_pitch;
-    for (uint32_t c = lane * 4; c < s.vdimp; c += 128) {
+    for (uint32_t c0 = 0; c0 < s.vdimp; c0 += 128) {
+        const uint32_t c = c0 + lane * 4;
         float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
-        for (uint32_t i = 0; i < n; ++i) {
-            const float4 v = *reinterpret_cast<const float4*>(part + (size_t)i * s.vdimp + c);
-            const float f = exp2f(ml[i].x - shift);
-            acc.x = fmaf(f, v.x, acc.x);
-            acc.y = fmaf(f, v.y, acc.y);
-            acc.z = fmaf(f, v.z, acc.z);
-            acc.w = fmaf(f, v.w, acc.w);
+        for (uint32_t i0 = 0; i0 < n; i0 += 32) {  // lane i has the factor of range i0 + i
+            const float f32 = i0 + lane < n ? exp2f((i0 ? ml[i0 + lane].x : mine.x) - shift) : 0.0f;
+            for (uint32_t i1 = 0; i1 < 32 && i0 + i1 < n; i1 += 8) {
+                float4 v[8];
+#pragma unroll
+                for (uint32_t e = 0; e < 8; ++e)
+                    v[e] = i0 + i1 + e < n && c < s.vdimp ? *reinterpret_cast<const float4*>(part + (size_t)(i0 + i1 + e) * s.vdimp + c)
+                                                         : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                for (uint32_t e = 0; e < 8; ++e) {
+                    const float f = __shfl_sync(0xFFFFFFFFu, f32, i1 + e);
+                    acc.x = fmaf(f, v[e].x, acc.x);
+                    acc.y = fmaf(f, v[e].y, acc.y);
+                    acc.z = fmaf(f, v[e].z, acc.z);
+                    acc.w = fmaf(f, v[e].w, acc.w);
+                }
+            }
         }
         const float o[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
 #pragma unroll
@@ -484,6 +491,18 @@ ragged_combine_kernel(const __grid_constant__ RaggedCall call) {
 }
 
 int done(cudaError_t e) { return e == cudaSuccess ? ZQ_OK : cuda_fail(e); }
+
+// The most shared memory that a kernel may ask for, set on each device at its first launch there.
+template <typename K>
+int allow_shared(K kernel, std::atomic<uint64_t>& devices) {
+    int device = 0;
+    ZQ_CUDA(cudaGetDevice(&device));
+    const uint64_t bit = 1ull << (device & 63);
+    if (devices.load(std::memory_order_relaxed) & bit) return ZQ_OK;
+    ZQ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024));
+    devices.fetch_or(bit, std::memory_order_relaxed);
+    return ZQ_OK;
+}
 
 // Rows of a tile: 64 where requests bring more packed rows than the small tile has, on the mean.
 uint32_t tile_rows(const RaggedArgs& a) {
@@ -521,7 +540,9 @@ template <typename T, int M, int N, int VC>
 int plain(const RaggedCall& c, cudaStream_t st) {
     const GqaShape& s = c.a.s;
     const size_t smem = ((size_t)(M + N) * (s.dimp + 4) + (size_t)N * s.vdimp + (size_t)M * (N + 4)) * 4;
-    ZQ_CUDA(cudaFuncSetAttribute(ragged_plain_kernel<T, M, N, VC>, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024));
+    static std::atomic<uint64_t> devices{0};
+    const int rc = allow_shared(ragged_plain_kernel<T, M, N, VC>, devices);
+    if (rc != ZQ_OK) return rc;
     const uint32_t per_sm = smem <= 72 * 1024 ? 3 : smem <= 110 * 1024 ? 2 : 1;
     return done(launch_pdl(ragged_plain_kernel<T, M, N, VC>, dim3(per_sm * sm_count()), dim3(kPlainThreads), smem, st, c));
 }
@@ -536,7 +557,9 @@ int plain_any(const RaggedCall& c, uint32_t M, cudaStream_t st) {
 template <int D, int STAGES, bool FULL>
 int few(const RaggedCall& c, cudaStream_t st) {
     const size_t smem = (size_t)(kFewThreads / 32) * STAGES * 16 * (c.a.s.dimp + 8 + c.a.s.vdimp + 8) * 2;
-    ZQ_CUDA(cudaFuncSetAttribute(ragged_few_kernel<D, STAGES, FULL>, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024));
+    static std::atomic<uint64_t> devices{0};
+    const int rc = allow_shared(ragged_few_kernel<D, STAGES, FULL>, devices);
+    if (rc != ZQ_OK) return rc;
     const uint32_t per_sm = smem <= 51 * 1024 ? 4 : smem <= 70 * 1024 ? 3 : smem <= 108 * 1024 ? 2 : 1;
     return done(launch_pdl(ragged_few_kernel<D, STAGES, FULL>, dim3(per_sm * sm_count()), dim3(kFewThreads), smem, st, c));
 }

@@ -10,7 +10,7 @@
 namespace zq {
 namespace {
 
-constexpr uint32_t kRangeKeys = 64;  // ranges are whole multiples of this
+constexpr uint32_t kRangeKeys = 32;  // ranges are whole multiples of this
 
 struct RaggedPlan {
     uint32_t R, tokens, head_tiles;  // query heads per key head; tokens and tiles of heads of a row tile
