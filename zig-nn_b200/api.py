@@ -627,10 +627,13 @@ def page_plan(new, lens, tables, free, span, page_size, rows, in_place=False):
     _int_rows(span, "span", 2)
     if rows < 0:
         raise ValueError("rows %d" % rows)
-    p = PagePlan()
-    p.lens, p.span = (lens, span) if in_place else (torch.empty_like(lens), torch.empty_like(span))
-    p.row_start, p.status = new.new_empty(requests + 1), new.new_empty(1)
-    p.pos, p.places = new.new_empty(rows), new.new_empty(rows)
+    p, even = PagePlan(), (rows + 3) // 4 * 4
+    # one allocation for all that comes back; pos and places on 16-byte boundaries
+    sizes = [even, even, requests + 1, 1] + ([] if in_place else [requests, 2])
+    p.pos, p.places, p.row_start, p.status, *after = torch.empty(sum(sizes), dtype=torch.int32, device=new.device).split(sizes)
+    p.lens, p.span = after or (lens, span)
+    if even != rows:
+        p.pos, p.places = p.pos[:rows], p.places[:rows]
     shape = S.Pages(free.shape[0], page_size, requests, tables.shape[1])
     rc = _lib.load().zq_page_plan(C.byref(shape), new.data_ptr(), lens.data_ptr(), p.lens.data_ptr(), tables.data_ptr(),
                                   free.data_ptr(), span.data_ptr(), p.span.data_ptr(), p.row_start.data_ptr(), p.pos.data_ptr(),

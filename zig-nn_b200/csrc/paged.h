@@ -25,9 +25,9 @@ struct PagedWriteArgs {
     float* v_first;
     void *q, *kc, *vc;
     const int32_t *pos, *places;
-    uint32_t n_places;  // places of the cache
+    uint32_t n_places, rows;  // places of the cache
 };
-int launch_paged_write(const PagedWriteArgs& a, uint32_t rows, bool f32, cudaStream_t st);
+int launch_paged_write(const PagedWriteArgs& a, bool f32, cudaStream_t st);
 
 // ---- attention of ragged rows (paged_attention.cu, paged_attention_tc.cu) ----------------------------------------------
 // Rows row_start[i] .. row_start[i + 1] - 1 are the last tokens of request i. Over pages: it holds lens[i] tokens, token t in place

@@ -96,7 +96,8 @@ int zq_paged_cache_write(const zq_gqa* g, const zq_pages* p, const float* d_qkv,
     a.pos = d_pos;
     a.places = d_places;
     a.n_places = p->pages * p->page_size;
-    return launch_paged_write(a, rows, is_f32(precision), as_stream(stream));
+    a.rows = rows;
+    return launch_paged_write(a, is_f32(precision), as_stream(stream));
 }
 
 size_t zq_paged_work_bytes(const zq_gqa* g, const zq_pages* p, uint32_t rows, int precision) {

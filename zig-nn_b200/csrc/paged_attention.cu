@@ -1,7 +1,8 @@
 // Causal grouped-query attention of ragged rows over pages of keys and values, or over packed prompts; softmax in f32.
-//   * a few rows of each request (bf16): the packed rows as the 16 rows of mma.sync, a warp per range of keys;
+//   * a few rows of each request: a warp per range of keys, the packed rows as the 16 rows of mma.sync (bf16) or by plain
+//     multiply-adds (f32);
 //   * more rows (bf16): paged_attention_tc.cu;
-//   * f32, and heads beyond 256 dimensions: tiles of 16 or 64 packed rows against tiles of keys, plain multiply-adds;
+//   * more rows (f32), and heads beyond 256 dimensions: tiles of 16 or 64 packed rows against tiles of keys, plain multiply-adds;
 //   * where a request's keys are cut into ranges, the ranges meet in a second small kernel.
 #include <atomic>
 
@@ -195,16 +196,123 @@ ragged_plain_kernel(const __grid_constant__ RaggedCall call) {
     });
 }
 
-// ---- a few rows of each request, bf16 ---------------------------------------------------------------------------------------
+// ---- a few rows of each request -------------------------------------------------------------------------------------------------
 // A warp per item: up to 16 packed rows against its range of keys, 16 keys a step. The keys and values of a step are the warp's own:
-// cp.async into a ring of its own in shared memory, STAGES - 1 steps ahead, through the end of an item into the next one's, so that
-// the stream of keys and values never stops and no warp waits for another. What bounds it: that stream (per step 16 (D + V) values
-// against 2 D / 8 + 2 V / 8 MMAs).
-constexpr uint32_t kFewThreads = 128;
-
-// FULL: keys and values have D dimensions, which spares the copies their counting.
+// cp.async into a ring of its own in shared memory, some steps ahead, through the end of an item into the next one's, so that
+// the stream of keys and values never stops and no warp waits for another. What bounds it: that stream. (B200, 64 requests of 500 to
+// 16384 tokens, 8 key heads of 128, 32 heads, bf16: 1.14 GB in 204 us, 5.6 TB/s; 4 warps an SM with five stages each took 538 us,
+// 8 with two 441 us, by an earlier build of 314 us with three.)
 constexpr float kFewRaise = 16.0f;  // powers of two that the maximum may lag behind
 
+// The copies of a warp's steps. FULL: keys and values have D dimensions, which spares the copies their counting.
+template <typename T, int D, int STAGES, bool FULL, uint32_t THREADS>
+struct KeyStream {
+    const RaggedArgs& a;
+    const RaggedPlan& p;
+    const Requests<THREADS>& rq;
+    const uint32_t dimp, vdimp, kpitch, vpitch, k_bytes, stage_bytes, ring, warps;
+    // an item, its next key, the page of that, the stage to fill; whether there is such a key; items from `ahead` on are to come
+    uint32_t c, base, end, ahead, key, filled = 0, page = 0;
+    Item it;
+    bool more = false;
+
+    __device__ __forceinline__ KeyStream(const RaggedCall& call, const Requests<THREADS>& q, uint32_t shared)
+        : a(call.a), p(call.p), rq(q), dimp(FULL ? D : a.s.dimp), vdimp(FULL ? D : a.s.vdimp), kpitch(dimp * sizeof(T) + 16),
+          vpitch(vdimp * sizeof(T) + 16), k_bytes(16 * kpitch), stage_bytes(16 * (kpitch + vpitch)),
+          ring(shared + (threadIdx.x >> 5) * STAGES * stage_bytes), warps(gridDim.x * (THREADS / 32)) {}
+
+    __device__ __forceinline__ void look_up() {
+        if (a.lens) page = (uint32_t)__ldg(a.tables + (size_t)it.request * a.table_ld + (key >> a.shift));
+    }
+    __device__ __forceinline__ void advance() {  // to an item that has keys
+        more = false;
+        while (ahead < end) {
+            it = item_at<THREADS>(a, p, c, rq, ahead - base);
+            ahead += warps;
+            if (it.k_begin < it.k_end) {
+                more = true;
+                key = it.k_begin;
+                look_up();
+                return;
+            }
+        }
+    }
+    // The items base ... end - 1 of the requests from c0 on, of which the warp's first is `next`.
+    __device__ __forceinline__ void enter(uint32_t c0, uint32_t first, uint32_t total, uint32_t next) {
+        c = c0;
+        base = first;
+        end = first + total;
+        ahead = next;
+        advance();
+    }
+    // 16 rows of one array, 16 bytes a lane and turn; zeros from row `rows` on
+    __device__ __forceinline__ void copy_rows(uint32_t dst, uint32_t pitch, const T* array, size_t ld, size_t row0, uint32_t col, uint32_t dp, uint32_t rows) {
+        constexpr uint32_t E = 16 / sizeof(T);
+        const uint32_t lane = threadIdx.x & 31, cpr = dp / E;
+        const T* from = array + row0 * ld + col;
+        if constexpr (FULL) {
+            constexpr uint32_t C = D / E, PER = C < 32 ? C : 32, DR = 32 / PER, TURNS = C / PER;  // lanes of a row, rows of a turn, turns of a row
+            uint32_t r = lane / PER;
+            from += r * ld + lane % PER * E;
+            dst += r * pitch + lane % PER * 16;
+            const size_t step = DR * ld;
+            if (rows == 16) {
+#pragma unroll
+                for (uint32_t i = 0; i < 16 / DR; ++i, from += step, dst += DR * pitch)
+#pragma unroll
+                    for (uint32_t t = 0; t < TURNS; ++t) copy16(dst + t * 512, from + t * 32 * E, true);
+            } else {
+#pragma unroll 1
+                for (uint32_t i = 0; i < 16 / DR; ++i, from += step, dst += DR * pitch, r += DR)
+#pragma unroll 1
+                    for (uint32_t t = 0; t < TURNS; ++t) copy16(dst + t * 512, r < rows ? from + t * 32 * E : array, r < rows);
+            }
+        } else {
+            uint32_t r = lane / cpr, c16 = lane % cpr;
+#pragma unroll 1
+            for (uint32_t i = 0; i < cpr / 2; ++i) {
+                const bool ok = r < rows;
+                copy16(dst + r * pitch + c16 * 16, ok ? from + r * ld + c16 * E : array, ok);
+                for (c16 += 32; c16 >= cpr; c16 -= cpr) ++r;
+            }
+        }
+    }
+    __device__ __forceinline__ void produce() {
+        if (more) {
+            const uint32_t dst = ring + filled * stage_bytes;
+            const bool there = !a.lens || page < a.pages;
+            const size_t row0 = !there ? 0 : a.lens ? ((size_t)page << a.shift) + (key & ((1u << a.shift) - 1)) : (size_t)it.row0 + key;
+            const uint32_t rows = there ? min(16u, it.k_end - key) : 0, g = it.g;
+            key += 16;
+            if (key < it.k_end) look_up();
+            copy_rows(dst, kpitch, static_cast<const T*>(a.k), a.k_ld, row0, g * dimp, dimp, rows);
+            copy_rows(dst + k_bytes, vpitch, static_cast<const T*>(a.v), a.v_ld, row0, g * vdimp, vdimp, rows);
+            filled = filled + 1 == STAGES ? 0 : filled + 1;
+            if (key >= it.k_end) advance();
+        }
+        copy_commit();
+    }
+};
+
+// Where the result of a row goes: a row of one range to the output, else to its range's place among the sums.
+struct RowOut {
+    uint32_t row, head;
+    float* part;  // null: the output
+    float2* ml;
+};
+__device__ __forceinline__ RowOut row_out(const RaggedArgs& a, const RaggedPlan& p, const Item& it, uint32_t token, uint32_t head) {
+    RowOut o{it.row0 + token, it.g * p.R + head, nullptr, nullptr};
+    if (it.ranges > 1) {
+        const size_t at = ((size_t)o.row * a.s.heads + o.head) * p.max_ranges + it.range;
+        o.part = p.part + at * a.s.vdimp;
+        o.ml = reinterpret_cast<float2*>(p.part + (size_t)a.rows * a.s.heads * p.max_ranges * a.s.vdimp) + at;
+    }
+    return o;
+}
+
+constexpr uint32_t kFewThreads = 128;
+
+// bf16: the packed rows are the 16 rows of mma.sync. A step costs a warp 2 D / 16 + 2 V / 16 MMAs of about 15 cycles.
 template <int D, int STAGES, bool FULL>
 __global__ void __launch_bounds__(kFewThreads)
 ragged_few_kernel(const __grid_constant__ RaggedCall call) {
@@ -216,84 +324,18 @@ ragged_few_kernel(const __grid_constant__ RaggedCall call) {
     const RaggedArgs& a = call.a;
     const RaggedPlan& p = call.p;
     const GqaShape& s = a.s;
-    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = gridDim.x * (kFewThreads / 32);
-    const uint32_t dimp = FULL ? D : s.dimp, vdimp = FULL ? D : s.vdimp;
-    const uint32_t kpitch = (dimp + 8) * 2, vpitch = (vdimp + 8) * 2, k_bytes = 16 * kpitch, stage_bytes = k_bytes + 16 * vpitch;
-    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * STAGES * stage_bytes;
-    const bf16 *q = static_cast<const bf16*>(a.q), *kc = static_cast<const bf16*>(a.k), *vc = static_cast<const bf16*>(a.v);
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    KeyStream<bf16, D, STAGES, FULL, kFewThreads> keys(call, rq, (uint32_t)__cvta_generic_to_shared(smem));
+    const uint32_t dimp = keys.dimp, vdimp = keys.vdimp, kpitch = keys.kpitch, vpitch = keys.vpitch;
+    const bf16* q = static_cast<const bf16*>(a.q);
     const float scale2 = a.scale * kLog2e;
-
-    // 16 rows of one array -> shared memory, 16 bytes a lane and turn; zeros from row `rows` on
-    auto copy_rows = [&](uint32_t dst, uint32_t pitch, const bf16* base, size_t ld, size_t row0, uint32_t col, uint32_t dp, uint32_t rows) {
-        const uint32_t cpr = dp / 8, dr = 32 / cpr, dc = 32 % cpr;
-        uint32_t r = lane / cpr, c = lane % cpr;
-        const bf16* from = base + row0 * ld + col;
-        if constexpr (FULL) {  // whole rows apart: D / 8 lanes a row (D = 256: a row)
-            from += (D == 256 ? 0 : r) * ld + c * 8;
-            dst += r * pitch + c * 16;
-            const size_t step = (D == 256 ? 1 : dr) * ld;
-            if (rows == 16) {
-#pragma unroll
-                for (uint32_t i = 0; i < D / 16; ++i, from += step, dst += dr * pitch) copy16(dst, from, true);
-            } else {
-#pragma unroll 1
-                for (uint32_t i = 0; i < D / 16; ++i, from += step, dst += dr * pitch, r += dr) copy16(dst, r < rows ? from : base, r < rows);
-            }
-        } else {
-#pragma unroll 1
-            for (uint32_t i = 0; i < cpr / 2; ++i) {
-                const bool ok = r < rows;
-                copy16(dst + r * pitch + c * 16, ok ? from + r * ld + c * 8 : base, ok);
-                r += dr;
-                c += dc;
-                if (c >= cpr) {
-                    c -= cpr;
-                    ++r;
-                }
-            }
-        }
-    };
     uint32_t base = 0, next = blockIdx.x * (kFewThreads / 32) + warp;  // items of a CTA's warps are neighbours: heads of the same keys
+    uint32_t stage = 0, pending = 0;                                   // pending: steps asked for and not yet worked on
     for (uint32_t c = 0; c < a.requests; c += kFewThreads) {
         const uint32_t total = count_items<kFewThreads>(a, p, c, rq);
-        // what the copies are at: an item, its next key, the page of that, the stage to fill
-        uint32_t ahead = next, key = 0, filled = 0, page = 0;
-        Item pi;
-        bool more = false;  // there is such a key
-        auto look_up = [&]() {
-            if (a.lens) page = (uint32_t)__ldg(a.tables + (size_t)pi.request * a.table_ld + (key >> a.shift));
-        };
-        auto advance = [&]() {  // to an item that has keys
-            more = false;
-            while (ahead < base + total) {
-                pi = item_at<kFewThreads>(a, p, c, rq, ahead - base);
-                ahead += warps;
-                if (pi.k_begin < pi.k_end) {
-                    more = true;
-                    key = pi.k_begin;
-                    look_up();
-                    return;
-                }
-            }
-        };
-        auto produce = [&]() {
-            if (more) {
-                const uint32_t dst = ring + filled * stage_bytes;
-                const bool there = !a.lens || page < a.pages;
-                const size_t row0 = !there ? 0 : a.lens ? ((size_t)page << a.shift) + (key & ((1u << a.shift) - 1)) : (size_t)pi.row0 + key;
-                const uint32_t rows = there ? min(16u, pi.k_end - key) : 0, g = pi.g;
-                key += 16;
-                if (key < pi.k_end) look_up();
-                copy_rows(dst, kpitch, kc, a.k_ld, row0, g * dimp, dimp, rows);
-                copy_rows(dst + k_bytes, vpitch, vc, a.v_ld, row0, g * vdimp, vdimp, rows);
-                filled = filled + 1 == STAGES ? 0 : filled + 1;
-                if (key >= pi.k_end) advance();
-            }
-            copy_commit();
-        };
-        advance();
-        uint32_t stage = 0, pending = 0;  // pending: steps asked for and not yet worked on
-        for (; next < base + total; next += warps) {
+        keys.enter(c, base, total, next);
+        pending = 0;
+        for (; next < base + total; next += keys.warps) {
             const Item it = item_at<kFewThreads>(a, p, c, rq, next - base);
             uint32_t token[2], head[2], qf[S][4];
             bool real[2];
@@ -320,10 +362,10 @@ ragged_few_kernel(const __grid_constant__ RaggedCall call) {
                 for (int e = 0; e < 4; ++e) o[v][e] = 0.0f;
             for (uint32_t k0 = it.k_begin; k0 < it.k_end; k0 += 16, --pending) {
 #pragma unroll 1
-                for (; pending < STAGES - 1; ++pending) produce();
+                for (; pending < STAGES - 1; ++pending) keys.produce();  // STAGES in flight: 211 us in place of 207
                 copy_wait<STAGES - 2>();
                 __syncwarp();
-                const uint32_t kt = ring + stage * stage_bytes, vt = kt + k_bytes;
+                const uint32_t kt = keys.ring + stage * keys.stage_bytes, vt = kt + keys.k_bytes;
                 float z[2][4] = {}, y[2][4] = {};  // even and odd steps of the dimensions: two chains each
                 const uint32_t k_addr = kt + (((lane >> 4) << 3) + (lane & 7)) * kpitch + ((lane >> 3) & 1) * 16;
 #pragma unroll
@@ -393,10 +435,11 @@ ragged_few_kernel(const __grid_constant__ RaggedCall call) {
                 l[h] += __shfl_xor_sync(0xFFFFFFFFu, l[h], 1);
                 l[h] += __shfl_xor_sync(0xFFFFFFFFu, l[h], 2);
                 if (!real[h]) continue;
-                const uint32_t row = it.row0 + token[h], hd = it.g * p.R + head[h], col0 = (lane & 3) * 2;
-                if (it.ranges == 1) {
-                    bf16* out = static_cast<bf16*>(a.out) + (size_t)row * a.out_pitch;
-                    bf16* mine = out + (size_t)hd * s.vdim;
+                const RowOut to = row_out(a, p, it, token[h], head[h]);
+                const uint32_t col0 = (lane & 3) * 2;
+                if (!to.part) {
+                    bf16* out = static_cast<bf16*>(a.out) + (size_t)to.row * a.out_pitch;
+                    bf16* mine = out + (size_t)to.head * s.vdim;
                     const float inv = m[h] > -INFINITY ? 1.0f / l[h] : 0.0f;
                     const bool even = s.vdim % 2 == 0;
 #pragma unroll
@@ -410,18 +453,182 @@ ragged_few_kernel(const __grid_constant__ RaggedCall call) {
                             if (col + 1 < s.vdim) mine[col + 1] = __float2bfloat16_rn(y);
                         }
                     }
-                    if (hd == 0)
+                    if (to.head == 0)
                         for (uint32_t e = s.heads * s.vdim + (lane & 3); e < a.out_pitch; e += 4) out[e] = __float2bfloat16_rn(0.0f);
                 } else {
-                    const size_t at = ((size_t)row * s.heads + hd) * p.max_ranges + it.range;
-                    float* part = p.part + at * vdimp;
 #pragma unroll
                     for (int v = 0; v < S * 2; ++v)
-                        if (FULL || v * 8 + col0 < vdimp) *reinterpret_cast<float2*>(part + v * 8 + col0) = make_float2(o[v][2 * h], o[v][2 * h + 1]);
-                    if ((lane & 3) == 0)
-                        *reinterpret_cast<float2*>(p.part + (size_t)a.rows * s.heads * p.max_ranges * vdimp + at * 2) = make_float2(m[h], l[h]);
+                        if (FULL || v * 8 + col0 < vdimp) *reinterpret_cast<float2*>(to.part + v * 8 + col0) = make_float2(o[v][2 * h], o[v][2 * h + 1]);
+                    if ((lane & 3) == 0) *to.ml = make_float2(m[h], l[h]);
                 }
-                if (p.max_ranges > 1 && hd == 0 && it.range == 0 && (lane & 3) == 0) p.n_ranges[row] = it.ranges;
+                if (p.max_ranges > 1 && to.head == 0 && it.range == 0 && (lane & 3) == 0) p.n_ranges[to.row] = it.ranges;
+            }
+        }
+        copy_wait<0>();
+        base += total;
+    }
+}
+
+// f32: plain multiply-adds from shared memory, up to four packed rows. Scores: a lane has one of the 16 keys and half of the
+// dimensions, the rows' queries come as broadcasts; values: a lane has four columns (of 64 columns the half-warps take every other
+// key), the weights come as broadcasts.
+constexpr uint32_t kFewRowsF32 = 4;
+
+template <int D, int STAGES, bool FULL, uint32_t THREADS>
+__global__ void __launch_bounds__(THREADS)
+ragged_few_f32_kernel(const __grid_constant__ RaggedCall call) {
+    constexpr int VN = D <= 128 ? 1 : D / 128;  // columns of a lane: 4 VN
+    constexpr uint32_t HALVES = D == 64 ? 2 : 1;
+    extern __shared__ __align__(16) unsigned char smem[];
+    __shared__ Requests<THREADS> rq;
+    pdl_launch_dependents();
+    pdl_wait();
+    const RaggedArgs& a = call.a;
+    const RaggedPlan& p = call.p;
+    const GqaShape& s = a.s;
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    KeyStream<float, D, STAGES, FULL, THREADS> keys(call, rq, (uint32_t)__cvta_generic_to_shared(smem));
+    const uint32_t dimp = keys.dimp, vdimp = keys.vdimp, kp = keys.kpitch / 4, vp = keys.vpitch / 4;
+    float* Q = reinterpret_cast<float*>(smem + (THREADS / 32) * STAGES * keys.stage_bytes) + warp * (4 * dimp + 64);  // [4][dimp]
+    float* P = Q + 4 * dimp;                                                                                         // [16 keys][4]
+    const float* q = static_cast<const float*>(a.q);
+    const float scale2 = a.scale * kLog2e;
+    const uint32_t my_key = lane & 15, side = lane >> 4;  // of the scores; a lane looks after rows 2 side + 0, 1 of its key
+    const uint32_t v_first = HALVES == 2 ? lane >> 4 : 0, v_lane = HALVES == 2 ? lane & 15 : lane;
+    uint32_t base = 0, next = blockIdx.x * (THREADS / 32) + warp, stage = 0, pending = 0;
+    for (uint32_t c = 0; c < a.requests; c += THREADS) {
+        const uint32_t total = count_items<THREADS>(a, p, c, rq);
+        keys.enter(c, base, total, next);
+        pending = 0;
+        for (; next < base + total; next += keys.warps) {
+            const Item it = item_at<THREADS>(a, p, c, rq, next - base);
+            __syncwarp();
+#pragma unroll
+            for (uint32_t r = 0; r < 4; ++r) {
+                uint32_t token, head;
+                const bool ok = row_of(p, it, r, 4, token, head);
+                const float* from = q + (size_t)(it.row0 + (ok ? token : 0)) * a.q_ld + (size_t)(it.g * p.R + (ok ? head : 0)) * dimp;
+                for (uint32_t d = lane * 4; d < dimp; d += 128)
+                    store4(Q + r * dimp + d, ok ? __ldg(reinterpret_cast<const float4*>(from + d)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f));
+            }
+            float o[4][4 * VN], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+            int32_t see[2];
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int e = 0; e < 4 * VN; ++e) o[r][e] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                uint32_t token, head;
+                see[i] = row_of(p, it, side * 2 + i, 4, token, head) ? min(seen_by(it, token), (int32_t)it.k_end) : 0;
+            }
+            __syncwarp();
+            for (uint32_t k0 = it.k_begin; k0 < it.k_end; k0 += 16, --pending) {
+#pragma unroll 1
+                for (; pending < STAGES; ++pending) keys.produce();
+                copy_wait<STAGES - 1>();
+                __syncwarp();
+                const float* K = reinterpret_cast<const float*>(smem + (warp * STAGES + stage) * keys.stage_bytes);
+                const float* V = K + keys.k_bytes / 4;
+                const float *k_row = K + my_key * kp + side * (dimp / 2), *q_row = Q + side * (dimp / 2);
+                float z[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 8
+                for (uint32_t d = 0; d < dimp / 2; d += 4) {
+                    const float4 x = *reinterpret_cast<const float4*>(k_row + d);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float4 y = *reinterpret_cast<const float4*>(q_row + r * dimp + d);
+                        z[r] = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, z[r]))));
+                    }
+                }
+#pragma unroll
+                for (int r = 0; r < 4; ++r) z[r] += __shfl_xor_sync(0xFFFFFFFFu, z[r], 16);
+                float x[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) x[e] = (int32_t)(k0 + my_key) < see[e] ? (side ? z[2 + e] : z[e]) * scale2 : -INFINITY;
+                // against an older maximum while none exceeds it by more than 2^kFewRaise
+                if (__any_sync(0xFFFFFFFFu, x[0] > m[0] + kFewRaise || x[1] > m[1] + kFewRaise)) {
+                    float f[2];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float mx = x[e];
+#pragma unroll
+                        for (int off = 8; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, off));
+                        mx = fmaxf(mx, m[e]);
+                        f[e] = m[e] == -INFINITY ? 0.0f : exp2f(m[e] - mx);
+                        m[e] = mx;
+                        l[e] *= f[e];
+                    }
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float fr = __shfl_sync(0xFFFFFFFFu, f[r & 1], (r >> 1) * 16);
+#pragma unroll
+                        for (int e = 0; e < 4 * VN; ++e) o[r][e] *= fr;
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    x[e] = exp2f(x[e] - (m[e] == -INFINITY ? 0.0f : m[e]));
+                    l[e] += x[e];
+                }
+                *reinterpret_cast<float2*>(P + my_key * 4 + side * 2) = make_float2(x[0], x[1]);
+                __syncwarp();
+#pragma unroll
+                for (int n = 0; n < VN; ++n) {
+                    const uint32_t col = v_lane * 4 + n * 128;
+                    if (col < vdimp) {
+#pragma unroll
+                        for (uint32_t k = 0; k < 16; k += HALVES) {
+                            const float4 v = *reinterpret_cast<const float4*>(V + (k + v_first) * vp + col);
+                            const float4 w = *reinterpret_cast<const float4*>(P + (k + v_first) * 4);
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) {
+                                const float y = r == 0 ? w.x : r == 1 ? w.y : r == 2 ? w.z : w.w;
+                                o[r][4 * n] = fmaf(y, v.x, o[r][4 * n]);
+                                o[r][4 * n + 1] = fmaf(y, v.y, o[r][4 * n + 1]);
+                                o[r][4 * n + 2] = fmaf(y, v.z, o[r][4 * n + 2]);
+                                o[r][4 * n + 3] = fmaf(y, v.w, o[r][4 * n + 3]);
+                            }
+                        }
+                    }
+                }
+                __syncwarp();
+                stage = stage + 1 == STAGES ? 0 : stage + 1;
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int off = 8; off > 0; off >>= 1) l[i] += __shfl_xor_sync(0xFFFFFFFFu, l[i], off);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float mr = __shfl_sync(0xFFFFFFFFu, m[r & 1], (r >> 1) * 16), lr = __shfl_sync(0xFFFFFFFFu, l[r & 1], (r >> 1) * 16);
+                if (HALVES == 2) {
+#pragma unroll
+                    for (int e = 0; e < 4 * VN; ++e) o[r][e] += __shfl_xor_sync(0xFFFFFFFFu, o[r][e], 16);
+                }
+                uint32_t token, head;
+                if (!row_of(p, it, r, 4, token, head)) continue;
+                const RowOut to = row_out(a, p, it, token, head);
+                if (v_first == 0) {
+                    if (!to.part) {
+                        float* out = static_cast<float*>(a.out) + (size_t)to.row * a.out_pitch;
+                        const float inv = mr > -INFINITY ? 1.0f / lr : 0.0f;
+#pragma unroll
+                        for (int n = 0; n < VN; ++n)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                if (v_lane * 4 + n * 128 + e < s.vdim) out[(size_t)to.head * s.vdim + v_lane * 4 + n * 128 + e] = o[r][4 * n + e] * inv;
+                        if (to.head == 0)
+                            for (uint32_t e = s.heads * s.vdim + v_lane; e < a.out_pitch; e += 32 / HALVES) out[e] = 0.0f;
+                    } else {
+#pragma unroll
+                        for (int n = 0; n < VN; ++n)
+                            if (v_lane * 4 + n * 128 < vdimp)
+                                store4(to.part + v_lane * 4 + n * 128, make_float4(o[r][4 * n], o[r][4 * n + 1], o[r][4 * n + 2], o[r][4 * n + 3]));
+                        if (lane == 0) *to.ml = make_float2(mr, lr);
+                    }
+                }
+                if (p.max_ranges > 1 && to.head == 0 && it.range == 0 && lane == 0) p.n_ranges[to.row] = it.ranges;
             }
         }
         copy_wait<0>();
@@ -504,30 +711,36 @@ int allow_shared(K kernel, std::atomic<uint64_t>& devices) {
     return ZQ_OK;
 }
 
-// Rows of a tile: 64 where requests bring more packed rows than the small tile has, on the mean.
-uint32_t tile_rows(const RaggedArgs& a) {
-    const uint32_t R = a.s.heads / a.s.kv_heads;
-    return (a.s.dimp > 256 || a.s.vdimp > 256 || (uint64_t)a.rows * R <= (uint64_t)16 * a.requests) ? 16 : 64;
+bool large(const GqaShape& s) { return s.dimp > 256 || s.vdimp > 256; }
+
+// Rows of a tile: 64 (or the tensor cores' tiles) where requests bring more packed rows than the small tile has, on the mean.
+uint32_t tile_rows(const RaggedArgs& a, bool f32) {
+    const uint64_t rows = (uint64_t)a.rows * (a.s.heads / a.s.kv_heads);
+    if (large(a.s)) return 16;
+    if (f32) return rows <= 2ull * kFewRowsF32 * a.requests ? kFewRowsF32 : 64;
+    return rows <= 16ull * a.requests ? 16 : 64;
 }
 
-// Ranges: as many as fill the SMs twice while the host sees too few units of work; beyond that no range longer than 512 keys, so that
-// requests of different lengths share the SMs evenly, or as much longer as keeps the sums of the ranges within 2^19 rows.
-RaggedPlan plan_of(const RaggedArgs& a, uint32_t M) {
+// Ranges of a request's keys. As many as give each of the GPU's workers (a warp, or a CTA of the larger tile) one while the host sees
+// fewer units of work than that, but no more than sqrt(0.4 keys): a range less costs a worker 16 keys (0.5 us), a range more costs the
+// join 0.08 us. Beyond that no range longer than 512 keys, so that requests of different lengths share the GPU evenly (one decode step
+// of 64 requests: 256 keys 228 us, 512 214, 1024 224), or as much longer as keeps the sums of the ranges within 2^19 rows.
+RaggedPlan plan_of(const RaggedArgs& a, uint32_t M, bool f32) {
     RaggedPlan p{};
     p.R = a.s.heads / a.s.kv_heads;
     p.tokens = p.R <= M ? M / p.R : 1;
     p.head_tiles = p.R <= M ? 1 : (p.R + M - 1) / M;
-    const uint64_t tiles = (uint64_t)a.rows / p.tokens + (a.requests < a.rows ? a.requests : a.rows);
-    const uint64_t units = (tiles ? tiles : 1) * a.s.kv_heads * p.head_tiles;
-    const uint64_t fill = 2ull * sm_count() / units;
+    const uint64_t per_tile = a.s.kv_heads * p.head_tiles, some = a.requests < a.rows ? a.requests : a.rows;  // requests with rows at most
+    const uint64_t packed = ((uint64_t)a.rows + p.tokens - 1) / p.tokens, least_units = (packed > some ? packed : some) * per_tile;
+    const bool wide = a.s.dimp > 128 || a.s.vdimp > 128, narrow = a.s.dimp <= 64 && a.s.vdimp <= 64;
+    const uint64_t per_sm = large(a.s) || M == 64 ? 1 : f32 ? (wide ? 3 : narrow ? 8 : 4) : (wide ? 4 : narrow ? 12 : 8);
+    const uint64_t fill = per_sm * sm_count() / (least_units ? least_units : 1);
     p.fill = fill < 1 ? 1 : (uint32_t)fill;
     uint64_t most = 512;
-    while (most < a.capacity && units * ((a.capacity + most - 1) / most) * M > (1ull << 19)) most *= 2;
+    const uint64_t most_units = (packed + some) * per_tile;
+    while (most < a.capacity && most_units * ((a.capacity + most - 1) / most) * M > (1ull << 19)) most *= 2;
     p.most_keys = (uint32_t)most;
-    const uint32_t blocks = (a.capacity + kRangeKeys - 1) / kRangeKeys, least = (a.capacity + p.most_keys - 1) / p.most_keys;
-    p.max_ranges = blocks < p.fill ? blocks : p.fill;
-    if (p.max_ranges < least) p.max_ranges = least;
-    if (p.max_ranges < 1) p.max_ranges = 1;
+    p.max_ranges = ranges_wanted(a.capacity, p.fill, p.most_keys);
     p.part = static_cast<float*>(a.work);
     p.n_ranges = reinterpret_cast<uint32_t*>(p.part + (size_t)a.rows * a.s.heads * p.max_ranges * (a.s.vdimp + 2));
     return p;
@@ -554,39 +767,53 @@ int plain_any(const RaggedCall& c, uint32_t M, cudaStream_t st) {
     return v <= 64 ? plain<T, 64, 64, 1>(c, st) : v <= 128 ? plain<T, 64, 64, 2>(c, st) : plain<T, 64, 64, 4>(c, st);
 }
 
-template <int D, int STAGES, bool FULL>
-int few(const RaggedCall& c, cudaStream_t st) {
-    const size_t smem = (size_t)(kFewThreads / 32) * STAGES * 16 * (c.a.s.dimp + 8 + c.a.s.vdimp + 8) * 2;
+// CTAs of an SM by shared memory; the kernels have some 4 KB of their own.
+uint32_t few_per_sm(size_t smem) { return smem <= 51 * 1024 ? 4 : smem <= 70 * 1024 ? 3 : smem <= 108 * 1024 ? 2 : 1; }
+
+template <int D, bool FULL>
+int few_bf16(const RaggedCall& c, cudaStream_t st) {
+    constexpr int STAGES = 3;
+    const size_t smem = (kFewThreads / 32) * STAGES * 16 * ((c.a.s.dimp + c.a.s.vdimp) * 2 + 32);
     static std::atomic<uint64_t> devices{0};
     const int rc = allow_shared(ragged_few_kernel<D, STAGES, FULL>, devices);
     if (rc != ZQ_OK) return rc;
-    const uint32_t per_sm = smem <= 51 * 1024 ? 4 : smem <= 70 * 1024 ? 3 : smem <= 108 * 1024 ? 2 : 1;
-    return done(launch_pdl(ragged_few_kernel<D, STAGES, FULL>, dim3(per_sm * sm_count()), dim3(kFewThreads), smem, st, c));
+    return done(launch_pdl(ragged_few_kernel<D, STAGES, FULL>, dim3(few_per_sm(smem) * sm_count()), dim3(kFewThreads), smem, st, c));
 }
-int few_any(const RaggedCall& c, cudaStream_t st) {
-    const uint32_t d = c.a.s.dimp > c.a.s.vdimp ? c.a.s.dimp : c.a.s.vdimp;
-    if (c.a.s.dimp == c.a.s.vdimp) {
-        if (d == 64) return few<64, 3, true>(c, st);
-        if (d == 128) return few<128, 3, true>(c, st);
-        if (d == 256) return few<256, 3, true>(c, st);
+template <int D, bool FULL>
+int few_f32(const RaggedCall& c, cudaStream_t st) {
+    constexpr int STAGES = D <= 128 ? 3 : 2;
+    constexpr uint32_t THREADS = D <= 128 ? 128 : 96;  // what an SM holds
+    const size_t smem = (THREADS / 32) * (STAGES * 16 * ((c.a.s.dimp + c.a.s.vdimp) * 4 + 32) + (4 * c.a.s.dimp + 64) * 4);
+    static std::atomic<uint64_t> devices{0};
+    const int rc = allow_shared(ragged_few_f32_kernel<D, STAGES, FULL, THREADS>, devices);
+    if (rc != ZQ_OK) return rc;
+    return done(launch_pdl(ragged_few_f32_kernel<D, STAGES, FULL, THREADS>, dim3(few_per_sm(smem) * sm_count()), dim3(THREADS), smem, st, c));
+}
+int few_any(const RaggedCall& c, bool f32, cudaStream_t st) {
+    const uint32_t k = c.a.s.dimp, v = c.a.s.vdimp, d = k > v ? k : v;
+    if (k == v) {
+        if (d == 64) return f32 ? few_f32<64, true>(c, st) : few_bf16<64, true>(c, st);
+        if (d == 128) return f32 ? few_f32<128, true>(c, st) : few_bf16<128, true>(c, st);
+        if (d == 256) return f32 ? few_f32<256, true>(c, st) : few_bf16<256, true>(c, st);
     }
-    return d <= 64 ? few<64, 3, false>(c, st) : d <= 128 ? few<128, 3, false>(c, st) : few<256, 3, false>(c, st);
+    if (d <= 64) return f32 ? few_f32<64, false>(c, st) : few_bf16<64, false>(c, st);
+    if (d <= 128) return f32 ? few_f32<128, false>(c, st) : few_bf16<128, false>(c, st);
+    return f32 ? few_f32<256, false>(c, st) : few_bf16<256, false>(c, st);
 }
 
 }  // namespace
 
 size_t ragged_work_bytes(const RaggedArgs& a, bool f32) {
-    const uint32_t M = tile_rows(a);
-    return !f32 && M == 64 && ragged_tc_takes(a) ? ragged_tc_work_bytes(a) : plan_bytes(a, plan_of(a, M));
+    const uint32_t M = tile_rows(a, f32);
+    return !f32 && M == 64 && ragged_tc_takes(a) ? ragged_tc_work_bytes(a) : plan_bytes(a, plan_of(a, M, f32));
 }
 
 int launch_ragged_attention(const RaggedArgs& a, bool f32, cudaStream_t st) {
     if (a.rows == 0 || a.requests == 0) return ZQ_OK;
-    const uint32_t M = tile_rows(a);
+    const uint32_t M = tile_rows(a, f32);
     if (!f32 && M == 64 && ragged_tc_takes(a)) return launch_ragged_tc(a, st);
-    const RaggedCall c{a, plan_of(a, M)};
-    const bool large = a.s.dimp > 256 || a.s.vdimp > 256;
-    int rc = f32 ? plain_any<float>(c, M, st) : M == 16 && !large ? few_any(c, st) : plain_any<bf16>(c, M, st);
+    const RaggedCall c{a, plan_of(a, M, f32)};
+    const int rc = M <= 16 && !large(a.s) ? few_any(c, f32, st) : f32 ? plain_any<float>(c, M, st) : plain_any<bf16>(c, M, st);
     if (rc != ZQ_OK || c.p.max_ranges < 2) return rc;
     const dim3 grid(((uint64_t)a.rows * a.s.heads + 3) / 4);
     return done(f32 ? launch_pdl_split(true, ragged_combine_kernel<float>, grid, dim3(128), 0, st, c)

@@ -10,7 +10,7 @@
 namespace zq {
 namespace {
 
-constexpr uint32_t kRangeKeys = 32;  // ranges are whole multiples of this
+constexpr uint32_t kRangeKeys = 16;  // ranges are whole multiples of this
 
 struct RaggedPlan {
     uint32_t R, tokens, head_tiles;  // query heads per key head; tokens and tiles of heads of a row tile
@@ -27,17 +27,20 @@ struct Item {
     uint32_t k_begin, k_end;  // keys of the range
 };
 
+// Ranges that `len` keys are cut into at most: never fewer for more keys.
+__host__ __device__ inline uint32_t ranges_wanted(uint32_t len, uint32_t fill, uint32_t most_keys) {
+    uint32_t n = (len + kRangeKeys - 1) / kRangeKeys;
+    const uint32_t worth = (uint32_t)sqrtf(0.4f * (float)len), least = (len + most_keys - 1) / most_keys;
+    n = n < fill ? n : fill;
+    n = n < worth ? n : worth;
+    n = n > least ? n : least;
+    return n < 1 ? 1 : n;
+}
+// How many they are cut into, and how long these are.
 __host__ __device__ inline uint32_t ranges_of(uint32_t len, uint32_t fill, uint32_t most_keys, uint32_t& per) {
-    const uint32_t blocks = (len + kRangeKeys - 1) / kRangeKeys;
-    if (blocks == 0) {
-        per = kRangeKeys;
-        return 1;
-    }
-    uint32_t n = blocks < fill ? blocks : fill;
-    const uint32_t least = (len + most_keys - 1) / most_keys;
-    if (n < least) n = least;
-    per = (blocks + n - 1) / n * kRangeKeys;
-    return (len + per - 1) / per;
+    const uint32_t blocks = (len + kRangeKeys - 1) / kRangeKeys, n = ranges_wanted(len, fill, most_keys);
+    per = blocks > n ? (blocks + n - 1) / n * kRangeKeys : kRangeKeys;
+    return len ? (len + per - 1) / per : 1;
 }
 
 __device__ __forceinline__ void span_of(const RaggedArgs& a, uint32_t i, uint32_t& row0, uint32_t& n_rows, int32_t& len) {

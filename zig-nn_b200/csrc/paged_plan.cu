@@ -193,6 +193,97 @@ paged_write_kernel(const __grid_constant__ PagedWriteArgs a) {
     }
 }
 
+__device__ __forceinline__ void store_four(float* o, float4 v) { *reinterpret_cast<float4*>(o) = v; }
+__device__ __forceinline__ void store_four(bf16* o, float4 v) {
+    const __nv_bfloat162 x = __floats2bfloat162_rn(v.x, v.y), y = __floats2bfloat162_rn(v.z, v.w);
+    *reinterpret_cast<uint2*>(o) = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+}
+
+// The same where heads are whole groups of four values, up to 128 N of them: N accesses of 16 bytes a lane and head, HEADS heads of a row
+// requested together. What bounds it: the rows' bytes.
+template <typename TA, int N, int HEADS>
+__global__ void __launch_bounds__(128)
+paged_write_vec_kernel(const __grid_constant__ PagedWriteArgs a, uint32_t groups) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const GqaShape& s = a.s;
+    const uint32_t lane = threadIdx.x & 31, unit = blockIdx.x * 4 + (threadIdx.x >> 5), r = unit / groups, first_item = unit % groups * HEADS;
+    if (r >= a.rows) return;
+    const uint32_t n_qk = s.heads + s.kv_heads, n_items = n_qk + s.kv_heads;
+    const float* row = a.qkv + (size_t)r * (n_qk * s.dim + s.kv_heads * s.vdim);
+    const uint32_t place = (uint32_t)a.places[r], pos = (uint32_t)a.pos[r];
+    const bool kept = place < a.n_places;
+    float4 x[HEADS][N];
+#pragma unroll
+    for (int i = 0; i < HEADS; ++i) {
+        const uint32_t item = first_item + i;
+        const bool is_v = item >= n_qk;
+        const float* from = is_v ? row + (size_t)n_qk * s.dim + (size_t)(item - n_qk) * s.vdim : row + (size_t)item * s.dim;
+        const uint32_t dim = is_v ? s.vdim : s.dim;
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const uint32_t c = lane * 4 + n * 128;
+            x[i][n] = item < n_items && c < dim ? __ldcs(reinterpret_cast<const float4*>(from + c)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+    }
+    float ss[HEADS];
+#pragma unroll
+    for (int i = 0; i < HEADS; ++i) {
+        ss[i] = 0.0f;
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+            ss[i] = fmaf(x[i][n].x, x[i][n].x, fmaf(x[i][n].y, x[i][n].y, fmaf(x[i][n].z, x[i][n].z, fmaf(x[i][n].w, x[i][n].w, ss[i]))));
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1)
+#pragma unroll
+        for (int i = 0; i < HEADS; ++i) ss[i] += __shfl_xor_sync(0xFFFFFFFFu, ss[i], off);
+    const float temperature = first_item < s.heads ? query_temperature(pos, a.temp_coef, a.temp_every) : 1.0f;
+#pragma unroll
+    for (int i = 0; i < HEADS; ++i) {
+        const uint32_t item = first_item + i;
+        if (item >= n_items) break;
+        if (item < n_qk) {
+            const bool is_q = item < s.heads;
+            if (!is_q && !kept) continue;
+            const float f = 1.0f / sqrtf(ss[i] / (float)s.dim + a.eps) * (is_q ? temperature : 1.0f);
+            const float* w = is_q ? a.q_norm : a.k_norm;
+            TA* o = is_q ? static_cast<TA*>(a.q) + ((size_t)r * s.heads + item) * s.dimp
+                         : static_cast<TA*>(a.kc) + ((size_t)place * s.kv_heads + (item - s.heads)) * s.dimp;
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                const uint32_t c = lane * 4 + n * 128;
+                if (c >= s.dimp) continue;
+                float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (c < s.dim) {
+                    y.x = x[i][n].x * f * w[c];
+                    y.y = x[i][n].y * f * w[c + 1];
+                    y.z = x[i][n].z * f * w[c + 2];
+                    y.w = x[i][n].w * f * w[c + 3];
+                }
+                store_four(o + c, y);
+            }
+        } else {
+            const uint32_t g = item - n_qk;
+            float* first = a.v_first ? a.v_first + ((size_t)r * s.kv_heads + g) * s.vdim : nullptr;
+            TA* o = static_cast<TA*>(a.vc) + ((size_t)place * s.kv_heads + g) * s.vdimp;
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                const uint32_t c = lane * 4 + n * 128;
+                if (c >= s.vdimp) continue;
+                float4 y = x[i][n];
+                if (c < s.vdim) {
+                    y.x = mixed_value(y.x, a.vmix, first, c);
+                    y.y = mixed_value(y.y, a.vmix, first, c + 1);
+                    y.z = mixed_value(y.z, a.vmix, first, c + 2);
+                    y.w = mixed_value(y.w, a.vmix, first, c + 3);
+                }
+                if (kept) store_four(o + c, y);
+            }
+        }
+    }
+}
+
 int done(cudaError_t e) { return e == cudaSuccess ? ZQ_OK : cuda_fail(e); }
 
 }  // namespace
@@ -219,11 +310,34 @@ int launch_page_plan(const PagePlanArgs& a, cudaStream_t st) {
     return done(cudaLaunchKernelEx(&cfg, page_plan_kernel, a));
 }
 
-int launch_paged_write(const PagedWriteArgs& a, uint32_t rows, bool f32, cudaStream_t st) {
-    if (rows == 0) return ZQ_OK;
-    const dim3 grid(rows, (a.s.heads + 2 * a.s.kv_heads + 3) / 4);
-    return done(f32 ? launch_pdl(paged_write_kernel<float>, grid, dim3(128), 0, st, a)
-                    : launch_pdl(paged_write_kernel<bf16>, grid, dim3(128), 0, st, a));
+namespace {
+
+template <typename TA, int N>
+int write_vec(const PagedWriteArgs& a, cudaStream_t st) {
+    const uint32_t items = a.s.heads + 2 * a.s.kv_heads;
+    auto go = [&](auto kernel, uint32_t heads) {
+        const uint32_t groups = (items + heads - 1) / heads;
+        return done(launch_pdl(kernel, dim3((uint32_t)(((uint64_t)a.rows * groups + 3) / 4)), dim3(128), 0, st, a, groups));
+    };
+    // four heads a warp where that leaves each SM a dozen warps
+    return (uint64_t)a.rows * items >= 48ull * sm_count() ? go(paged_write_vec_kernel<TA, N, 4>, 4) : go(paged_write_vec_kernel<TA, N, 1>, 1);
+}
+template <typename TA>
+int write_any(const PagedWriteArgs& a, cudaStream_t st) {
+    const GqaShape& s = a.s;
+    const bool fours = s.dim % 4 == 0 && s.vdim % 4 == 0 && ((uintptr_t)a.qkv & 15u) == 0 && ((uintptr_t)a.q & 15u) == 0 &&
+                       ((uintptr_t)a.kc & 15u) == 0 && ((uintptr_t)a.vc & 15u) == 0;
+    const uint32_t d = s.dimp > s.vdimp ? s.dimp : s.vdimp;
+    if (fours && d <= 128) return write_vec<TA, 1>(a, st);
+    if (fours && d <= 256) return write_vec<TA, 2>(a, st);
+    return done(launch_pdl(paged_write_kernel<TA>, dim3(a.rows, (s.heads + 2 * s.kv_heads + 3) / 4), dim3(128), 0, st, a));
+}
+
+}  // namespace
+
+int launch_paged_write(const PagedWriteArgs& a, bool f32, cudaStream_t st) {
+    if (a.rows == 0) return ZQ_OK;
+    return f32 ? write_any<float>(a, st) : write_any<bf16>(a, st);
 }
 
 }  // namespace zq
