@@ -723,7 +723,7 @@ uint32_t tile_rows(const RaggedArgs& a, bool f32) {
 
 // Ranges of a request's keys. As many as give each of the GPU's workers (a warp, or a CTA of the larger tile) one while the host sees
 // fewer units of work than that, but no more than sqrt(0.4 keys): a range less costs a worker 16 keys (0.5 us), a range more costs the
-// join 0.08 us. Beyond that no range longer than 512 keys, so that requests of different lengths share the GPU evenly (one decode step
+// join 0.08 us. (The larger tile: eight times as many, since its items differ in what they see.) Beyond that no range longer than 512 keys, so that requests of different lengths share the GPU evenly (one decode step
 // of 64 requests: 256 keys 228 us, 512 214, 1024 224), or as much longer as keeps the sums of the ranges within 2^19 rows.
 RaggedPlan plan_of(const RaggedArgs& a, uint32_t M, bool f32) {
     RaggedPlan p{};
@@ -733,14 +733,15 @@ RaggedPlan plan_of(const RaggedArgs& a, uint32_t M, bool f32) {
     const uint64_t per_tile = a.s.kv_heads * p.head_tiles, some = a.requests < a.rows ? a.requests : a.rows;  // requests with rows at most
     const uint64_t packed = ((uint64_t)a.rows + p.tokens - 1) / p.tokens, least_units = (packed > some ? packed : some) * per_tile;
     const bool wide = a.s.dimp > 128 || a.s.vdimp > 128, narrow = a.s.dimp <= 64 && a.s.vdimp <= 64;
-    const uint64_t per_sm = large(a.s) || M == 64 ? 1 : f32 ? (wide ? 3 : narrow ? 8 : 4) : (wide ? 4 : narrow ? 12 : 8);
+    p.block = M == 64 ? 64 : 16;  // the steps of the kernels
+    const uint64_t per_sm = M == 64 ? 8 : large(a.s) ? 2 : f32 ? (wide ? 3 : narrow ? 8 : 4) : (wide ? 4 : narrow ? 12 : 8);
     const uint64_t fill = per_sm * sm_count() / (least_units ? least_units : 1);
     p.fill = fill < 1 ? 1 : (uint32_t)fill;
     uint64_t most = 512;
     const uint64_t most_units = (packed + some) * per_tile;
     while (most < a.capacity && most_units * ((a.capacity + most - 1) / most) * M > (1ull << 19)) most *= 2;
     p.most_keys = (uint32_t)most;
-    p.max_ranges = ranges_wanted(a.capacity, p.fill, p.most_keys);
+    p.max_ranges = ranges_wanted(a.capacity, p.block, p.fill, p.most_keys);
     p.part = static_cast<float*>(a.work);
     p.n_ranges = reinterpret_cast<uint32_t*>(p.part + (size_t)a.rows * a.s.heads * p.max_ranges * (a.s.vdimp + 2));
     return p;

@@ -10,11 +10,9 @@
 namespace zq {
 namespace {
 
-constexpr uint32_t kRangeKeys = 16;  // ranges are whole multiples of this
-
 struct RaggedPlan {
     uint32_t R, tokens, head_tiles;  // query heads per key head; tokens and tiles of heads of a row tile
-    uint32_t fill, most_keys;        // ranges that fill the GPU; keys of a range at most
+    uint32_t block, fill, most_keys;  // ranges are whole blocks of keys; ranges that fill the GPU; keys of a range at most
     uint32_t max_ranges;
     float* part;                     // [rows][heads][max_ranges][vdimp], then [rows][heads][max_ranges][2]: maximum, sum
     uint32_t* n_ranges;              // [rows]
@@ -28,8 +26,8 @@ struct Item {
 };
 
 // Ranges that `len` keys are cut into at most: never fewer for more keys.
-__host__ __device__ inline uint32_t ranges_wanted(uint32_t len, uint32_t fill, uint32_t most_keys) {
-    uint32_t n = (len + kRangeKeys - 1) / kRangeKeys;
+__host__ __device__ inline uint32_t ranges_wanted(uint32_t len, uint32_t block, uint32_t fill, uint32_t most_keys) {
+    uint32_t n = (len + block - 1) / block;
     const uint32_t worth = (uint32_t)sqrtf(0.4f * (float)len), least = (len + most_keys - 1) / most_keys;
     n = n < fill ? n : fill;
     n = n < worth ? n : worth;
@@ -37,9 +35,9 @@ __host__ __device__ inline uint32_t ranges_wanted(uint32_t len, uint32_t fill, u
     return n < 1 ? 1 : n;
 }
 // How many they are cut into, and how long these are.
-__host__ __device__ inline uint32_t ranges_of(uint32_t len, uint32_t fill, uint32_t most_keys, uint32_t& per) {
-    const uint32_t blocks = (len + kRangeKeys - 1) / kRangeKeys, n = ranges_wanted(len, fill, most_keys);
-    per = blocks > n ? (blocks + n - 1) / n * kRangeKeys : kRangeKeys;
+__host__ __device__ inline uint32_t ranges_of(uint32_t len, uint32_t block, uint32_t fill, uint32_t most_keys, uint32_t& per) {
+    const uint32_t blocks = (len + block - 1) / block, n = ranges_wanted(len, block, fill, most_keys);
+    per = blocks > n ? (blocks + n - 1) / n * block : block;
     return len ? (len + per - 1) / per : 1;
 }
 
@@ -64,11 +62,11 @@ struct Requests {
 template <uint32_t THREADS>
 __device__ __forceinline__ uint32_t count_items(const RaggedArgs& a, const RaggedPlan& p, uint32_t c, Requests<THREADS>& q) {
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    uint32_t row0 = 0, n_rows = 0, per = kRangeKeys, ranges = 1, scan = 0;
+    uint32_t row0 = 0, n_rows = 0, per = 1, ranges = 1, scan = 0;
     int32_t len = 0;
     if (c + tid < a.requests) {
         span_of(a, c + tid, row0, n_rows, len);
-        ranges = ranges_of(len > 0 ? len : 0, p.fill, p.most_keys, per);
+        ranges = ranges_of(len > 0 ? len : 0, p.block, p.fill, p.most_keys, per);
         scan = (p.tokens > 1 ? (n_rows + p.tokens - 1) / p.tokens : n_rows) * ranges * a.s.kv_heads * p.head_tiles;
     }
 #pragma unroll
