@@ -35,7 +35,8 @@ __device__ __forceinline__ void stage4(float* dst, const bf16* src, bool ok) {
 // M rows x N keys at a time, 16 x 16 threads: thread (ty, tx) has rows ty * RPT ... of the scores and of the output, keys tx + 16 j of
 // the scores, values tx * 4 + 64 c ... of the output. S = Q K^T from shared memory, the online softmax in registers (a row's 16
 // threads are half a warp), P through shared memory, O += P V. The next keys travel under the values' product, the values under the
-// scores.
+// scores. What bounds it: the issue of instructions; two products per multiply-add (even and odd dimensions of a score, neighbouring
+// columns of the output), copies whose rows and columns a thread knows from the start.
 template <typename T, int M, int N, int VC>
 __global__ void __launch_bounds__(kPlainThreads)
 ragged_plain_kernel(const __grid_constant__ RaggedCall call) {
@@ -50,6 +51,9 @@ ragged_plain_kernel(const __grid_constant__ RaggedCall call) {
     float *Q = smf, *K = Q + M * qp, *V = K + N * qp, *P = V + N * vp;
     const T *q = static_cast<const T*>(a.q), *kc = static_cast<const T*>(a.k), *vc = static_cast<const T*>(a.v);
     const float scale2 = a.scale * kLog2e;
+    // of the copies: four columns, the first row, rows apart (threads that are over have none)
+    const uint32_t k_per = s.dimp / 4, k_step = kPlainThreads / k_per, k_row = tid / k_per < k_step ? tid / k_per : M + N, k_col = tid % k_per * 4;
+    const uint32_t v_per = s.vdimp / 4, v_step = kPlainThreads / v_per, v_row = tid / v_per < v_step ? tid / v_per : M + N, v_col = tid % v_per * 4;
     for_items<kPlainThreads>(a, p, [&](const Item& it) {
         const uint32_t k_first = it.k_begin;
         uint32_t k_end = it.k_end;
@@ -59,21 +63,22 @@ ragged_plain_kernel(const __grid_constant__ RaggedCall call) {
             k_end = see <= 0 ? k_first : min(k_end, (uint32_t)see);
         }
         __syncthreads();  // the item before has been read
-        for (uint32_t i = tid; i < M * (s.dimp / 4); i += kPlainThreads) {
-            const uint32_t m = i / (s.dimp / 4), c = i % (s.dimp / 4) * 4;
+        for (uint32_t m = k_row; m < M; m += k_step) {
             uint32_t token, head;
             const bool ok = row_of(p, it, m, M, token, head);
-            stage4(Q + m * qp + c, q + (ok ? (size_t)(it.row0 + token) * a.q_ld + (size_t)(it.g * p.R + head) * s.dimp + c : 0), ok);
+            stage4(Q + m * qp + k_col, q + (ok ? (size_t)(it.row0 + token) * a.q_ld + (size_t)(it.g * p.R + head) * s.dimp + k_col : 0), ok);
         }
-        auto stage = [&](float* dst, const T* base, size_t ld, uint32_t pitch, uint32_t dp, uint32_t k0) {
-            for (uint32_t i = tid; i < N * (dp / 4); i += kPlainThreads) {
-                const uint32_t n = i / (dp / 4), c = i % (dp / 4) * 4, key = k0 + n;
-                const T* row = key < k_end ? token_row(a, it, base, ld, key) : nullptr;
-                stage4(dst + n * pitch + c, row ? row + (size_t)it.g * dp + c : base, row != nullptr);
+        auto stage = [&](float* dst, const T* base, size_t ld, uint32_t pitch, uint32_t dp, uint32_t first, uint32_t step, uint32_t col, uint32_t k0) {
+            for (uint32_t n = first; n < N; n += step) {
+                const T* row = k0 + n < k_end ? token_row(a, it, base, ld, k0 + n) : nullptr;
+                stage4(dst + n * pitch + col, row ? row + (size_t)it.g * dp + col : base, row != nullptr);
             }
             copy_commit();
         };
-        float o[RPT][VC][4], m[RPT], l[RPT];
+        auto stage_k = [&](uint32_t k0) { stage(K, kc, a.k_ld, qp, s.dimp, k_row, k_step, k_col, k0); };
+        auto stage_v = [&](uint32_t k0) { stage(V, vc, a.v_ld, vp, s.vdimp, v_row, v_step, v_col, k0); };
+        pair o[RPT][VC][2];
+        float m[RPT], l[RPT];
         int32_t see[RPT];
 #pragma unroll
         for (int r = 0; r < RPT; ++r) {
@@ -82,32 +87,39 @@ ragged_plain_kernel(const __grid_constant__ RaggedCall call) {
             m[r] = -INFINITY;
             l[r] = 0.0f;
 #pragma unroll
-            for (int c = 0; c < VC; ++c)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[r][c][e] = 0.0f;
+            for (int c = 0; c < VC; ++c) o[r][c][0] = o[r][c][1] = 0;
         }
-        if (k_first < k_end) stage(K, kc, a.k_ld, qp, s.dimp, k_first);
+        if (k_first < k_end) stage_k(k_first);
         for (uint32_t k0 = k_first; k0 < k_end; k0 += N) {
-            stage(V, vc, a.v_ld, vp, s.vdimp, k0);
+            stage_v(k0);
             copy_wait<1>();
             __syncthreads();
+            pair z2[RPT][CPT];
+#pragma unroll
+            for (int r = 0; r < RPT; ++r)
+#pragma unroll
+                for (int j = 0; j < CPT; ++j) z2[r][j] = 0;
+#pragma unroll 2
+            for (uint32_t d = 0; d < s.dimp; d += 4) {
+                ulonglong2 x[RPT], y[CPT];
+#pragma unroll
+                for (int r = 0; r < RPT; ++r) x[r] = *reinterpret_cast<const ulonglong2*>(Q + (ty * RPT + r) * qp + d);
+#pragma unroll
+                for (int j = 0; j < CPT; ++j) y[j] = *reinterpret_cast<const ulonglong2*>(K + (tx + 16 * j) * qp + d);
+#pragma unroll
+                for (int r = 0; r < RPT; ++r)
+#pragma unroll
+                    for (int j = 0; j < CPT; ++j) z2[r][j] = fma2(x[r].y, y[j].y, fma2(x[r].x, y[j].x, z2[r][j]));
+            }
             float z[RPT][CPT];
 #pragma unroll
             for (int r = 0; r < RPT; ++r)
 #pragma unroll
-                for (int j = 0; j < CPT; ++j) z[r][j] = 0.0f;
-            for (uint32_t d = 0; d < s.dimp; d += 4) {
-                float4 x[RPT], y[CPT];
-#pragma unroll
-                for (int r = 0; r < RPT; ++r) x[r] = *reinterpret_cast<const float4*>(Q + (ty * RPT + r) * qp + d);
-#pragma unroll
-                for (int j = 0; j < CPT; ++j) y[j] = *reinterpret_cast<const float4*>(K + (tx + 16 * j) * qp + d);
-#pragma unroll
-                for (int r = 0; r < RPT; ++r)
-#pragma unroll
-                    for (int j = 0; j < CPT; ++j)
-                        z[r][j] = fmaf(x[r].x, y[j].x, fmaf(x[r].y, y[j].y, fmaf(x[r].z, y[j].z, fmaf(x[r].w, y[j].w, z[r][j]))));
-            }
+                for (int j = 0; j < CPT; ++j) {
+                    uint32_t even, odd;
+                    split(z2[r][j], even, odd);
+                    z[r][j] = __uint_as_float(even) + __uint_as_float(odd);
+                }
 #pragma unroll
             for (int r = 0; r < RPT; ++r) {
                 float mx = -INFINITY;
@@ -131,11 +143,11 @@ ragged_plain_kernel(const __grid_constant__ RaggedCall call) {
 #pragma unroll
                 for (int c = 0; c < VC; ++c)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) o[r][c][e] *= f;
+                    for (int e = 0; e < 2; ++e) o[r][c][e] = fma2(o[r][c][e], pair_of(f, f), 0);
             }
             copy_wait<0>();
             __syncthreads();
-            if (k0 + N < k_end) stage(K, kc, a.k_ld, qp, s.dimp, k0 + N);
+            if (k0 + N < k_end) stage_k(k0 + N);
             for (uint32_t n = 0; n < N; n += 4) {
                 float4 w[RPT];
 #pragma unroll
@@ -146,14 +158,12 @@ ragged_plain_kernel(const __grid_constant__ RaggedCall call) {
                     for (int c = 0; c < VC; ++c) {
                         const uint32_t col = tx * 4 + 64 * c;
                         if (col >= s.vdimp) continue;
-                        const float4 x = *reinterpret_cast<const float4*>(V + (n + e) * vp + col);
+                        const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(V + (n + e) * vp + col);
 #pragma unroll
                         for (int r = 0; r < RPT; ++r) {
                             const float y = e == 0 ? w[r].x : e == 1 ? w[r].y : e == 2 ? w[r].z : w[r].w;
-                            o[r][c][0] = fmaf(y, x.x, o[r][c][0]);
-                            o[r][c][1] = fmaf(y, x.y, o[r][c][1]);
-                            o[r][c][2] = fmaf(y, x.z, o[r][c][2]);
-                            o[r][c][3] = fmaf(y, x.w, o[r][c][3]);
+                            o[r][c][0] = fma2(pair_of(y, y), x.x, o[r][c][0]);
+                            o[r][c][1] = fma2(pair_of(y, y), x.y, o[r][c][1]);
                         }
                     }
             }
@@ -167,6 +177,16 @@ ragged_plain_kernel(const __grid_constant__ RaggedCall call) {
             uint32_t token, head;
             if (!row_of(p, it, ty * RPT + r, M, token, head)) continue;
             const uint32_t row = it.row0 + token, h = it.g * p.R + head;
+            float y[VC][4];
+#pragma unroll
+            for (int c = 0; c < VC; ++c)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    uint32_t u, v;
+                    split(o[r][c][e], u, v);
+                    y[c][2 * e] = __uint_as_float(u);
+                    y[c][2 * e + 1] = __uint_as_float(v);
+                }
             if (it.ranges == 1) {
                 T* out = static_cast<T*>(a.out) + (size_t)row * a.out_pitch;
                 const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
@@ -175,7 +195,7 @@ ragged_plain_kernel(const __grid_constant__ RaggedCall call) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const uint32_t col = tx * 4 + 64 * c + e;
-                        if (col < s.vdim) out[(size_t)h * s.vdim + col] = to_act<T>(o[r][c][e] * inv);
+                        if (col < s.vdim) out[(size_t)h * s.vdim + col] = to_act<T>(y[c][e] * inv);
                     }
                 if (h == 0)
                     for (uint32_t i = s.heads * s.vdim + tx; i < a.out_pitch; i += 16) out[i] = to_act<T>(0.0f);
@@ -184,7 +204,7 @@ ragged_plain_kernel(const __grid_constant__ RaggedCall call) {
 #pragma unroll
                 for (int c = 0; c < VC; ++c)
                     if (tx * 4 + 64 * c < s.vdimp)
-                        store4(p.part + at * s.vdimp + tx * 4 + 64 * c, make_float4(o[r][c][0], o[r][c][1], o[r][c][2], o[r][c][3]));
+                        store4(p.part + at * s.vdimp + tx * 4 + 64 * c, make_float4(y[c][0], y[c][1], y[c][2], y[c][3]));
                 if (tx == 0) {
                     float* ml = p.part + (size_t)a.rows * s.heads * p.max_ranges * s.vdimp + at * 2;
                     ml[0] = m[r];
@@ -757,14 +777,13 @@ int plain(const RaggedCall& c, cudaStream_t st) {
     static std::atomic<uint64_t> devices{0};
     const int rc = allow_shared(ragged_plain_kernel<T, M, N, VC>, devices);
     if (rc != ZQ_OK) return rc;
-    const uint32_t per_sm = smem <= 72 * 1024 ? 3 : smem <= 110 * 1024 ? 2 : 1;
+    const uint32_t per_sm = smem <= 68 * 1024 ? 3 : smem <= 106 * 1024 ? 2 : 1;
     return done(launch_pdl(ragged_plain_kernel<T, M, N, VC>, dim3(per_sm * sm_count()), dim3(kPlainThreads), smem, st, c));
 }
 template <typename T>
-int plain_any(const RaggedCall& c, uint32_t M, cudaStream_t st) {
+int plain_any(const RaggedCall& c, cudaStream_t st) {
     const uint32_t v = c.a.s.vdimp;
-    if (c.a.s.dimp > 256 || v > 256) return plain<T, 16, 32, 8>(c, st);
-    if (M == 16) return v <= 64 ? plain<T, 16, 64, 1>(c, st) : v <= 128 ? plain<T, 16, 64, 2>(c, st) : plain<T, 16, 64, 4>(c, st);
+    if (large(c.a.s)) return plain<T, 16, 32, 8>(c, st);
     return v <= 64 ? plain<T, 64, 64, 1>(c, st) : v <= 128 ? plain<T, 64, 64, 2>(c, st) : plain<T, 64, 64, 4>(c, st);
 }
 
@@ -814,7 +833,7 @@ int launch_ragged_attention(const RaggedArgs& a, bool f32, cudaStream_t st) {
     const uint32_t M = tile_rows(a, f32);
     if (!f32 && M == 64 && ragged_tc_takes(a)) return launch_ragged_tc(a, st);
     const RaggedCall c{a, plan_of(a, M, f32)};
-    const int rc = M <= 16 && !large(a.s) ? few_any(c, f32, st) : f32 ? plain_any<float>(c, M, st) : plain_any<bf16>(c, M, st);
+    const int rc = M <= 16 && !large(a.s) ? few_any(c, f32, st) : f32 ? plain_any<float>(c, st) : plain_any<bf16>(c, st);
     if (rc != ZQ_OK || c.p.max_ranges < 2) return rc;
     const dim3 grid(((uint64_t)a.rows * a.s.heads + 3) / 4);
     return done(f32 ? launch_pdl_split(true, ragged_combine_kernel<float>, grid, dim3(128), 0, st, c)

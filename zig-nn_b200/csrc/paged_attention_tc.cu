@@ -17,7 +17,7 @@
 // Roles: warps 0-3 (and 4-7 with two streams) softmax and results; then a warp that issues copies, and one per stream that issues its
 // MMAs (what a warp does besides, waits above all, costs more than the MMAs: one warp for both streams made the period of two tiles
 // 4400 cycles, of which their products are 2048). The first of them owns the tensor memory. Every wait is bounded, as in gemm_bf16.cu.
-#include "paged.h"
+#include "paged_common.cuh"
 #include "tc_common.cuh"
 
 namespace zq {
@@ -280,24 +280,6 @@ __device__ __forceinline__ void store32(bf16* out, const uint32_t* v) {
     asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(out), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]),
                  "r"(v[6]), "r"(v[7])
                  : "memory");
-}
-using pair = unsigned long long;  // two f32 of neighbouring registers
-__device__ __forceinline__ pair pair_of(uint32_t a, uint32_t b) {
-    pair r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(a), "r"(b));
-    return r;
-}
-__device__ __forceinline__ pair pair_of(float a, float b) { return pair_of(__float_as_uint(a), __float_as_uint(b)); }
-__device__ __forceinline__ void split(pair v, uint32_t& a, uint32_t& b) { asm("mov.b64 {%0, %1}, %2;" : "=r"(a), "=r"(b) : "l"(v)); }
-__device__ __forceinline__ pair fma2(pair a, pair b, pair c) {
-    pair r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ pair add2(pair a, pair b) {
-    pair r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;

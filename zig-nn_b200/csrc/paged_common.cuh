@@ -149,6 +149,25 @@ __device__ __forceinline__ bool row_of(const RaggedPlan& p, const Item& it, uint
 // Keys that token t of the request's rows sees.
 __device__ __forceinline__ int32_t seen_by(const Item& it, uint32_t t) { return it.len - (int32_t)it.n_rows + (int32_t)t + 1; }
 
+using pair = unsigned long long;  // two f32 of neighbouring registers
+__device__ __forceinline__ pair pair_of(uint32_t a, uint32_t b) {
+    pair r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(a), "r"(b));
+    return r;
+}
+__device__ __forceinline__ pair pair_of(float a, float b) { return pair_of(__float_as_uint(a), __float_as_uint(b)); }
+__device__ __forceinline__ void split(pair v, uint32_t& a, uint32_t& b) { asm("mov.b64 {%0, %1}, %2;" : "=r"(a), "=r"(b) : "l"(v)); }
+__device__ __forceinline__ pair fma2(pair a, pair b, pair c) {
+    pair r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ pair add2(pair a, pair b) {
+    pair r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
 // First value of a token's keys (or values) of all heads; null: a page of zeros.
 template <typename T>
 __device__ __forceinline__ const T* token_row(const RaggedArgs& a, const Item& it, const T* base, size_t ld, uint32_t key) {
