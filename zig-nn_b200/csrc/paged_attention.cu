@@ -17,8 +17,6 @@ struct RaggedCall {
     RaggedPlan p;
 };
 
-constexpr uint32_t kPlainThreads = 256;
-
 __device__ __forceinline__ void store4(float* o, float4 v) { *reinterpret_cast<float4*>(o) = v; }
 
 // Four values of a key or value row -> shared memory, zeros where there is no row.
@@ -35,12 +33,14 @@ __device__ __forceinline__ void stage4(float* dst, const bf16* src, bool ok) {
 // M rows x N keys at a time, 16 x 16 threads: thread (ty, tx) has rows ty * RPT ... of the scores and of the output, keys tx + 16 j of
 // the scores, values tx * 4 + 64 c ... of the output. S = Q K^T from shared memory, the online softmax in registers (a row's 16
 // threads are half a warp), P through shared memory, O += P V. The next keys travel under the values' product, the values under the
-// scores. What bounds it: the issue of instructions; two products per multiply-add (even and odd dimensions of a score, neighbouring
-// columns of the output), copies whose rows and columns a thread knows from the start.
+// scores. What bounds it: the loads from shared memory, eight of 16 bytes for 64 products (of 64 rows; eight rows a thread and half
+// the threads were 5 to 10 % slower). Two products per multiply-add (even
+// and odd dimensions of a score, neighbouring columns of the output), copies whose rows and columns a thread knows from the start.
 template <typename T, int M, int N, int VC>
-__global__ void __launch_bounds__(kPlainThreads)
+__global__ void __launch_bounds__(256)
 ragged_plain_kernel(const __grid_constant__ RaggedCall call) {
     constexpr int RPT = M / 16, CPT = N / 16;
+    constexpr uint32_t THREADS = 256;
     extern __shared__ __align__(16) float smf[];
     pdl_launch_dependents();
     pdl_wait();
@@ -52,9 +52,9 @@ ragged_plain_kernel(const __grid_constant__ RaggedCall call) {
     const T *q = static_cast<const T*>(a.q), *kc = static_cast<const T*>(a.k), *vc = static_cast<const T*>(a.v);
     const float scale2 = a.scale * kLog2e;
     // of the copies: four columns, the first row, rows apart (threads that are over have none)
-    const uint32_t k_per = s.dimp / 4, k_step = kPlainThreads / k_per, k_row = tid / k_per < k_step ? tid / k_per : M + N, k_col = tid % k_per * 4;
-    const uint32_t v_per = s.vdimp / 4, v_step = kPlainThreads / v_per, v_row = tid / v_per < v_step ? tid / v_per : M + N, v_col = tid % v_per * 4;
-    for_items<kPlainThreads>(a, p, [&](const Item& it) {
+    const uint32_t k_per = s.dimp / 4, k_step = THREADS / k_per, k_row = tid / k_per < k_step ? tid / k_per : M + N, k_col = tid % k_per * 4;
+    const uint32_t v_per = s.vdimp / 4, v_step = THREADS / v_per, v_row = tid / v_per < v_step ? tid / v_per : M + N, v_col = tid % v_per * 4;
+    for_items<THREADS>(a, p, [&](const Item& it) {
         const uint32_t k_first = it.k_begin;
         uint32_t k_end = it.k_end;
         {   // nothing behind what the tile's last token sees
@@ -777,8 +777,10 @@ int plain(const RaggedCall& c, cudaStream_t st) {
     static std::atomic<uint64_t> devices{0};
     const int rc = allow_shared(ragged_plain_kernel<T, M, N, VC>, devices);
     if (rc != ZQ_OK) return rc;
-    const uint32_t per_sm = smem <= 68 * 1024 ? 3 : smem <= 106 * 1024 ? 2 : 1;
-    return done(launch_pdl(ragged_plain_kernel<T, M, N, VC>, dim3(per_sm * sm_count()), dim3(kPlainThreads), smem, st, c));
+    // Four times the CTAs that run at once (two an SM up to 106 KB): the items differ, and who is done early takes another CTA's (chunks
+    // of 512 tokens, 12 heads of 64: 252 us with as many as run at once, 228 with two times, 210 with four, 210 with eight).
+    const uint32_t per_sm = smem <= 106 * 1024 ? 8 : 4;
+    return done(launch_pdl(ragged_plain_kernel<T, M, N, VC>, dim3(per_sm * sm_count()), dim3(256), smem, st, c));
 }
 template <typename T>
 int plain_any(const RaggedCall& c, cudaStream_t st) {
