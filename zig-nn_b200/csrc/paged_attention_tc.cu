@@ -857,9 +857,9 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     }
 }
 
-// The pieces of a tile, in the order of its keys: a block for 32 rows of the tile that begins in part blockIdx.x; a lane per row, eight
-// columns per warp and turn.
-constexpr uint32_t kJoinThreads = 256;
+// The pieces of a tile, in the order of its keys: a block for 32 rows of the tile that begins in part blockIdx.x, a lane per row, a warp
+// for eight columns. Maxima, sums and values of four pieces are requested together, all that the chain of loads allows.
+constexpr uint32_t kJoinThreads = 512;
 template <int STREAMS>
 __global__ void __launch_bounds__(kJoinThreads)
 ragged_join_kernel(const __grid_constant__ TcParams p) {
@@ -868,39 +868,56 @@ ragged_join_kernel(const __grid_constant__ TcParams p) {
     const RaggedArgs& a = p.a;
     const GqaShape& s = a.s;
     const uint32_t c = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.y * 32 + lane;
-    if (c >= p.w.head[0]) return;
     const SplitRec sp = p.w.splits[c];
-    if (sp.tile == ~0u) return;
+    if (c >= p.w.head[0] || sp.tile == ~0u) return;
     const TileRec t = p.w.tiles[sp.tile];
     const uint32_t m = row & 127, token = (row >> 7) * p.rt + m / p.R, head = sp.g * p.R + m % p.R;
     if (m >= p.rt * p.R || token >= t.tokens) return;
     constexpr uint32_t ROWS = STREAMS * 128;
     const size_t size = (size_t)(s.vdimp + 2) * ROWS, ml = (size_t)s.vdimp * ROWS;
-    auto piece = [&](uint32_t i) { return p.w.partial + (size_t)(i == c ? 2 * c + 1 : 2 * i) * size + row; };
-    float mx = -INFINITY, sum = 0.0f;
-#pragma unroll 4
-    for (uint32_t i = c; i <= sp.last; ++i) mx = fmaxf(mx, piece(i)[ml]);
-    const float shift = mx == -INFINITY ? 0.0f : mx;
-#pragma unroll 4
-    for (uint32_t i = c; i <= sp.last; ++i) sum += exp2f(piece(i)[ml] - shift) * piece(i)[ml + ROWS];
-    const float inv = mx > -INFINITY ? 1.0f / sum : 0.0f;
     bf16* out = static_cast<bf16*>(a.out) + (size_t)(t.row0 + token) * a.out_pitch;
+    bf16* mine = out + (size_t)head * s.vdim;
+    const bool wide = ((uintptr_t)mine & 15u) == 0;
     for (uint32_t col = warp * 8; col < s.vdimp; col += kJoinThreads / 4) {
-        float acc[8] = {};
-#pragma unroll 2
-        for (uint32_t i = c; i <= sp.last; ++i) {
-            const float* x = piece(i);
-            const float f = exp2f(x[ml] - shift);
-            float v[8];
+        float acc[8] = {}, mx = -INFINITY, sum = 0.0f;
+        for (uint32_t i0 = c; i0 <= sp.last; i0 += 4) {
+            float mi[4], li[4], v[4][8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = x[(size_t)(col + e) * ROWS];
-            if (f > 0.0f)  // not a piece of which the row sees nothing
+            for (uint32_t k = 0; k < 4; ++k) {
+                const uint32_t i = min(i0 + k, sp.last);
+                const float* x = p.w.partial + (size_t)(i == c ? 2 * c + 1 : 2 * i) * size + row;
+                mi[k] = i0 + k <= sp.last ? x[ml] : -INFINITY;
+                li[k] = x[ml + ROWS];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) acc[e] = fmaf(f, v[e], acc[e]);
+                for (int e = 0; e < 8; ++e) v[k][e] = i0 + k <= sp.last ? x[(size_t)(col + e) * ROWS] : 0.0f;
+            }
+            float to = fmaxf(fmaxf(fmaxf(mi[0], mi[1]), fmaxf(mi[2], mi[3])), mx);
+            const float shift = to == -INFINITY ? 0.0f : to, f = exp2f(mx - shift);
+            mx = to;
+            sum *= f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc[e] *= f;
+#pragma unroll
+            for (uint32_t k = 0; k < 4; ++k) {
+                const float g = exp2f(mi[k] - shift);
+                if (g > 0.0f) {  // not a piece of which the row sees nothing
+                    sum = fmaf(g, li[k], sum);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) acc[e] = fmaf(g, v[k][e], acc[e]);
+                }
+            }
         }
+        const float inv = mx > -INFINITY ? 1.0f / sum : 0.0f;
+        uint32_t o[4];
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (col + e < s.vdim) out[(size_t)head * s.vdim + col + e] = __float2bfloat16_rn(acc[e] * inv);
+        for (int e = 0; e < 4; ++e) o[e] = pack2(acc[2 * e] * inv, acc[2 * e + 1] * inv);
+        if (wide && col + 8 <= s.vdim) {
+            *reinterpret_cast<uint4*>(mine + col) = make_uint4(o[0], o[1], o[2], o[3]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (col + e < s.vdim) mine[col + e] = half_of(o[e / 2], e & 1);
+        }
     }
     if (head == 0)
         for (uint32_t i = s.heads * s.vdim + warp; i < a.out_pitch; i += kJoinThreads / 32) out[i] = __float2bfloat16_rn(0.0f);
@@ -983,9 +1000,9 @@ int launch(TcParams& p, cudaStream_t st) {
     if (rc != ZQ_OK) return rc;
     const uint32_t smem = p.slots_at + p.n_slots * p.slot + 1024;
     ZQ_CUDA(cudaFuncSetAttribute(ragged_tc_kernel<STREAMS, DK, DV>, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024));
-    rc = done(launch_pdl(ragged_prep_kernel, dim3(1), dim3(kPrepThreads), 0, st, p, STREAMS * p.rt));
+    rc = done(launch_pdl_split(true, ragged_prep_kernel, dim3(1), dim3(kPrepThreads), 0, st, p, STREAMS * p.rt));
     if (rc == ZQ_OK) rc = done(launch_pdl(ragged_tc_kernel<STREAMS, DK, DV>, dim3(p.max_parts), dim3(tc_threads(STREAMS)), smem, st, mq, mk, mv, p));
-    if (rc == ZQ_OK) rc = done(launch_pdl(ragged_join_kernel<STREAMS>, dim3(p.max_parts, STREAMS * 4), dim3(kJoinThreads), 0, st, p));
+    if (rc == ZQ_OK) rc = done(launch_pdl_split(true, ragged_join_kernel<STREAMS>, dim3(p.max_parts, STREAMS * 4), dim3(kJoinThreads), 0, st, p));
     return rc;
 }
 
