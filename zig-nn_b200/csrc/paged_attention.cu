@@ -733,12 +733,15 @@ int allow_shared(K kernel, std::atomic<uint64_t>& devices) {
 
 bool large(const GqaShape& s) { return s.dimp > 256 || s.vdimp > 256; }
 
-// Rows of a tile: 64 (or the tensor cores' tiles) where requests bring more packed rows than the small tile has, on the mean.
+// Rows of a tile: 64 (or the tensor cores' tiles) where requests bring more packed rows than some tiles of the small kernel have, on the
+// mean. bf16, requests over 4000 keys, small kernel and tensor cores, us: 64 requests, 32 heads over 8 of 128, 18 packed rows each 71 and 90,
+// 30 rows 107 and 99, 60 rows 132 and 89; four of them 19 and 30, 23 and 30, 41 and 29; 16 requests, 4 over 1 of 256, 18 rows 24 and 37, 60 rows
+// 43 and 38; 12 over 4 of 64, 14 rows 16 and 28, 45 rows 29 and 29. f32: two tiles of four rows.
 uint32_t tile_rows(const RaggedArgs& a, bool f32) {
     const uint64_t rows = (uint64_t)a.rows * (a.s.heads / a.s.kv_heads);
     if (large(a.s)) return 16;
     if (f32) return rows <= 2ull * kFewRowsF32 * a.requests ? kFewRowsF32 : 64;
-    return rows <= 16ull * a.requests ? 16 : 64;
+    return rows <= 32ull * a.requests ? 16 : 64;
 }
 
 // Ranges of a request's keys. As many as give each of the GPU's workers (a warp, or a CTA of the larger tile) one while the host sees

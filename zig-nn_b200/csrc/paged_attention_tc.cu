@@ -41,14 +41,15 @@ struct TileRec {
     uint32_t request, first_row;  // and the request's first row
     uint32_t cost0_lo, cost0_hi;  // cost of the tiles ahead (per key head)
 };
-struct PartRec {
+struct PartRec {  // where a part begins, its units (none: a CTA without work), the tile there
     uint32_t tile, g, off, n_units;
+    TileRec first;
 };
-struct SplitRec {  // the tile that begins in this part and ends in part `last`; tile = ~0: none
-    uint32_t tile, g, last, pad;
+struct SplitRec {  // the tile that begins in this part and ends in part `last`; last = 0: none
+    uint32_t g, last, pad[2];
+    TileRec tile;
 };
 struct TcWork {
-    uint32_t* head;  // parts
     PartRec* parts;
     SplitRec* splits;
     TileRec* tiles;
@@ -157,8 +158,11 @@ ragged_prep_kernel(const __grid_constant__ TcParams p, uint32_t tile_tokens) {
     }
     const uint64_t U = cost * a.s.kv_heads;
     uint64_t G = U / (kLeastPart + kTileCost);
-    G = G < 1 ? 1 : G > p.max_parts ? p.max_parts : G;
-    if (tid == 0) p.w.head[0] = U ? (uint32_t)G : 0;
+    G = U == 0 ? 0 : G < 1 ? 1 : G > p.max_parts ? p.max_parts : G;
+    if (tid < p.max_parts && tid >= (uint32_t)G) {
+        p.w.parts[tid] = PartRec{};
+        p.w.splits[tid] = SplitRec{};
+    }
     if (U == 0) return;
     auto find = [&](uint64_t u, uint32_t& tile, uint32_t& g, uint32_t& off, uint32_t& kt) {  // the tile of unit u
         uint32_t lo = 0, hi = n_tiles;
@@ -194,8 +198,9 @@ ragged_prep_kernel(const __grid_constant__ TcParams p, uint32_t tile_tokens) {
     const uint64_t b0 = bound[tid], b1 = bound[tid + 1];
     find(b0, part.tile, part.g, part.off, kt);
     part.n_units = (uint32_t)(b1 - b0);
+    part.first = p.w.tiles[part.tile];
     p.w.parts[tid] = part;
-    SplitRec s{~0u, 0, 0, 0};
+    SplitRec s{};
     uint32_t tile, g, off;
     const uint64_t begin = find(b1 - 1, tile, g, off, kt);
     if (off + 1 < kt && begin >= b0) {
@@ -203,7 +208,7 @@ ragged_prep_kernel(const __grid_constant__ TcParams p, uint32_t tile_tokens) {
         uint32_t last = (uint32_t)(((end + 1) * G - 1) / U);
         while (bound[last] > end) --last;
         while (bound[last + 1] <= end) ++last;
-        s.tile = tile;
+        s.tile = p.w.tiles[tile];
         s.g = g;
         s.last = last;
     }
@@ -413,6 +418,8 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    if (warp == LOADER && lane < 3)
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(lane == 0 ? &map_k : lane == 1 ? &map_q : &map_v)) : "memory");
     if (warp == ISSUER) {
         const uint32_t slot = (uint32_t)__cvta_generic_to_shared(&tmem_slot);
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(slot) : "memory");
@@ -426,16 +433,15 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     pdl_wait();
 
     const uint32_t c = blockIdx.x;
-    const bool busy = c < p.w.head[0];
     Walk w{};
-    if (busy) {
+    {
         const PartRec part = p.w.parts[c];
         w.tile = part.tile;
         w.g = part.g;
         w.off = part.off;
         w.left = part.n_units;
-        w.t = p.w.tiles[w.tile];
-        w.ahead = p.w.tiles[min(w.tile + 1, p.max_tiles - 1)];
+        w.t = part.first;
+        if (w.left) w.ahead = p.w.tiles[min(w.tile + 1, p.max_tiles - 1)];
     }
     auto leave = [&]() {  // behind a piece
         if (w.left) {
@@ -869,8 +875,8 @@ ragged_join_kernel(const __grid_constant__ TcParams p) {
     const GqaShape& s = a.s;
     const uint32_t c = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.y * 32 + lane;
     const SplitRec sp = p.w.splits[c];
-    if (c >= p.w.head[0] || sp.tile == ~0u) return;
-    const TileRec t = p.w.tiles[sp.tile];
+    if (sp.last == 0) return;
+    const TileRec& t = sp.tile;
     const uint32_t m = row & 127, token = (row >> 7) * p.rt + m / p.R, head = sp.g * p.R + m % p.R;
     if (m >= p.rt * p.R || token >= t.tokens) return;
     constexpr uint32_t ROWS = STREAMS * 128;
@@ -958,7 +964,6 @@ TcParams params_of(const RaggedArgs& a, size_t& bytes) {
         at += (n + 255) / 256 * 256;
         return r;
     };
-    p.w.head = reinterpret_cast<uint32_t*>(take(256));
     p.w.parts = reinterpret_cast<PartRec*>(take(p.max_parts * sizeof(PartRec)));
     p.w.splits = reinterpret_cast<SplitRec*>(take(p.max_parts * sizeof(SplitRec)));
     p.w.tiles = reinterpret_cast<TileRec*>(take(tiles * sizeof(TileRec)));
