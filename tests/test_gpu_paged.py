@@ -310,6 +310,62 @@ def test_packed_long(zq):
     check_packed(zq, 2, 1, 256, 256, False, [2200])
 
 
+# ---- sizes that take the tensor cores
+def enough(heads, dim, vdim):
+    """Rows n for which n rows of 0.7 n keys are work enough."""
+    up = lambda n: (n + 15) // 16 * 16
+    return int((0.9e9 / (2 * heads * (up(dim) + up(vdim)))) ** 0.5) + 40
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,vdim", HEADS)
+@pytest.mark.parametrize("page", [16, 128, 1024])
+def test_large_chunks(zq, heads, kv_heads, dim, vdim, page):
+    n = enough(heads, dim, vdim)
+    check_paged(zq, heads, kv_heads, dim, vdim, False, page, [n // 3, 0, 61, 17], [n, 1, 0, n // 2])
+    check_paged(zq, heads, kv_heads, dim, vdim, False, page, [n // 2], [n], seed=1, pad=0)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,vdim", HEADS)
+def test_large_packed(zq, heads, kv_heads, dim, vdim):
+    n = 2 * enough(heads, dim, vdim)
+    check_packed(zq, heads, kv_heads, dim, vdim, False, [n, 1, 0, 130, n // 2, 128, 33], pad=9, offset=16, wide=8)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 2, 128), (4, 1, 256), (12, 4, 64)])
+@pytest.mark.parametrize("more", [dict(scale=-0.2), dict(scale=0.0), dict(spread=6.0)])
+def test_large_chunks_of_other_scores(zq, heads, kv_heads, dim, more):
+    check_paged(zq, heads, kv_heads, dim, dim, False, 64, [900, 30, 0], [700, 640, 130], **more)
+
+
+@pytest.mark.parametrize("spoil", [0, 1, 2])
+def test_a_large_sequence_does_not_reach_its_neighbours(zq, spoil):
+    check_packed(zq, 8, 2, 128, 128, False, [900, 777, 1040], pad=30, spoil=spoil)
+    check_packed(zq, 4, 1, 256, 256, False, [900, 777, 1040], pad=30, spoil=spoil)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 2, 128), (4, 1, 256)])
+def test_large_chunks_over_pages_that_are_none(zq, heads, kv_heads, dim):
+    cache, q, row_start, lens, tables, keys, values = paged_case(zq, heads, kv_heads, dim, dim, False, 16, [900, 30], [700, 640])
+    for at, entry in ((1, -1), (40, cache.k.shape[0]), (41, -2 ** 31), (99, 2 ** 31 - 1)):
+        tables[0, at] = entry
+        keys[0][at * 16:(at + 1) * 16], values[0][at * 16:(at + 1) * 16] = 0, 0
+    short = i32([1600, 600])  # the second holds fewer tokens than it has rows
+    got = cache.attend(q, row_start, short, tables)
+    for i, (n, l) in enumerate(((700, 1600), (640, 600))):
+        a = int(row_start[i])
+        want, tol = plain.attention(q[a:a + n, :, :dim], keys[i][:l], values[i][:l], l - n + 1 + torch.arange(n, device="cuda"), cache.g.scale, True)
+        assert ((got[a:a + n].view(n, heads, dim).double() - want).abs() <= tol).all()
+    assert (got[700:740] == 0).all()
+
+
+@pytest.mark.parametrize("f32", [False, True])
+def test_many_requests(zq, f32):
+    """More than the kernels look at together: 128 and 1024."""
+    rng = random.Random(2)
+    check_paged(zq, 4, 2, 64, 64, f32, 16, [rng.randint(0, 90) for _ in range(300)], [rng.choice((0, 1, 1)) for _ in range(300)])
+    check_paged(zq, 4, 2, 64, 64, f32, 16, [rng.randint(0, 90) for _ in range(1100)], [rng.choice((0, 1, 60)) for _ in range(1100)], seed=1)
+
+
 # ---- together
 @pytest.mark.parametrize("f32", [False, True])
 @pytest.mark.parametrize("heads,kv_heads,dim", [(8, 2, 128), (4, 1, 256), (6, 3, 40)])

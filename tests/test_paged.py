@@ -1,0 +1,144 @@
+"""The paged cache and packed prompts on the CPU: what the entry points refuse, and which kernels their calls launch, by the library
+linked with a runtime that runs nothing."""
+import ctypes as C
+
+import pytest
+
+from host_runtime import Library, build
+from zignn_b200 import structs as S
+
+OK, BAD_ARG, UNSUPPORTED, LIMIT = 0, 1, 2, 5
+AT = C.c_void_p(1 << 20)  # nothing reads it
+
+
+@pytest.fixture(scope="module")
+def library(tmp_path_factory):
+    return Library(build(tmp_path_factory.mktemp("paged")))
+
+
+def gqa(heads=8, kv_heads=2, dim=128, vdim=128):
+    return S.Gqa(heads, kv_heads, dim, vdim, 0, 0, 0.1, 1e-6, 0.0, 0.0)
+
+
+def plan(library, pages=(100, 16, 4, 20), rows=8, **null):
+    names = ("new", "lens", "lens_out", "tables", "free", "span", "span_out", "row_start", "pos", "places")
+    a = [None if n in null else AT for n in names]
+    p = S.Pages(*pages)
+    return library.launches(lambda: library.lib.zq_page_plan(C.byref(p), *a, rows, None if "status" in null else AT, None))
+
+
+def write(library, g=None, pages=(100, 16, 1, 1), rows=8, precision=0, **given):
+    names = ("qkv", "q_norm", "k_norm", "vmix", "v_first", "q", "k", "v", "pos", "places")
+    a = [given.get(n, AT) for n in names]
+    g, p = g or gqa(), S.Pages(*pages)
+    return library.launches(lambda: library.lib.zq_paged_cache_write(C.byref(g), C.byref(p), *a, rows, precision, None))
+
+
+def attend(library, g=None, pages=(100, 16, 4, 20), rows=8, precision=0, short=0, **given):
+    names = ("q", "k", "v", "out", "row_start", "lens", "tables")
+    a = [given.get(n, AT) for n in names]
+    g, p, lib = g or gqa(), S.Pages(*pages), library.lib
+    need = lib.zq_paged_work_bytes(C.byref(g), C.byref(p), rows, precision)
+    return library.launches(lambda: lib.zq_paged_attention(C.byref(g), C.byref(p), *a, rows, given.get("work", AT), max(0, need - short), precision, None))
+
+
+def packed(library, g=None, sequences=4, rows=8, precision=0, lds=None, short=0, **given):
+    g, lib = g or gqa(), library.lib
+    up = lambda n: (n + 15) // 16 * 16
+    q_ld, k_ld, v_ld = lds or (g.heads * up(g.dim), g.kv_heads * up(g.dim), g.kv_heads * up(g.vdim))
+    need = lib.zq_packed_work_bytes(C.byref(g), sequences, rows, precision)
+    q, k, v, out, row_start, work = (given.get(n, AT) for n in ("q", "k", "v", "out", "row_start", "work"))
+    return library.launches(lambda: lib.zq_packed_attention(C.byref(g), q, q_ld, k, k_ld, v, v_ld, out, row_start, sequences, rows, work,
+                                                            max(0, need - short), precision, None))
+
+
+def refused(answer, status):
+    seen, got = answer
+    assert got == status and not seen, (got, [l.name for l in seen])
+
+
+def test_refusals_of_the_plan(library):
+    for name in ("new", "lens", "lens_out", "tables", "free", "span", "span_out", "row_start", "status", "pos", "places"):
+        refused(plan(library, **{name: None}), BAD_ARG)
+    assert plan(library, rows=0, pos=None, places=None)[1] == OK
+    for pages in ((0, 16, 4, 20), (100, 0, 4, 20), (100, 16, 0, 20), (100, 16, 4, 0)):
+        refused(plan(library, pages), BAD_ARG)
+    for size in (1, 8, 24, 2048):
+        refused(plan(library, (100, size, 4, 20)), UNSUPPORTED)
+    refused(plan(library, (1 << 27, 16, 4, 20)), LIMIT)
+    refused(plan(library, (100, 16, 4, 1 << 27)), LIMIT)
+    refused(plan(library, (100, 16, 8193, 20)), LIMIT)
+    refused(plan(library, rows=1 << 30), LIMIT)
+    assert plan(library, (100, 16, 8192, 20))[1] == OK and plan(library, ((1 << 27) - 1, 16, 1, 1))[1] == OK
+
+
+def test_refusals_of_the_write(library):
+    for name in ("qkv", "q_norm", "k_norm", "q", "k", "v", "pos", "places", "v_first"):  # the last: a mix without its other side
+        refused(write(library, **{name: None}), BAD_ARG)
+    assert write(library, vmix=None, v_first=None)[1] == OK and write(library, vmix=None)[1] == OK
+    refused(write(library, gqa(8, 3)), BAD_ARG)
+    refused(write(library, gqa(8, 2, 0)), BAD_ARG)
+    refused(write(library, precision=2), BAD_ARG)
+    refused(write(library, pages=(100, 20, 1, 1)), UNSUPPORTED)
+    refused(write(library, rows=0), OK)
+
+
+def test_refusals_of_the_attention(library):
+    for name in ("q", "k", "v", "out", "row_start", "lens", "tables"):
+        refused(attend(library, **{name: None}), BAD_ARG)
+    for name in ("q", "k", "v", "work"):
+        refused(attend(library, **{name: C.c_void_p((1 << 20) + 8)}), BAD_ARG)
+    refused(attend(library, rows=2000, short=1), BAD_ARG)
+    refused(attend(library, rows=2000, work=None), BAD_ARG)
+    refused(attend(library, gqa(8, 2, 520)), LIMIT)
+    refused(attend(library, gqa(8, 2, 128, 520)), LIMIT)
+    refused(attend(library, rows=1 << 30), LIMIT)
+    refused(attend(library, pages=(100, 48, 4, 20)), UNSUPPORTED)
+    refused(attend(library, precision=7), BAD_ARG)
+    refused(attend(library, rows=0), OK)
+
+
+def test_refusals_of_packed_prompts(library):
+    for name in ("q", "k", "v", "out", "row_start"):
+        refused(packed(library, **{name: None}), BAD_ARG)
+    for name in ("q", "k", "v", "work"):
+        refused(packed(library, **{name: C.c_void_p((1 << 20) + 4)}), BAD_ARG)
+    refused(packed(library, lds=(1023, 256, 256)), BAD_ARG)
+    refused(packed(library, lds=(1024, 255, 256)), BAD_ARG)
+    refused(packed(library, lds=(1024, 256, 264 + 4)), BAD_ARG)
+    assert packed(library, lds=(1024, 256, 264))[1] == OK and packed(library, precision=1, lds=(1024, 260, 264 + 4))[1] == OK
+    refused(packed(library, sequences=0), BAD_ARG)
+    refused(packed(library, rows=5000, work=None), BAD_ARG)
+    refused(packed(library, rows=5000, short=1), BAD_ARG)
+    refused(packed(library, gqa(8, 2, 600)), LIMIT)
+    refused(packed(library, rows=0), OK)
+
+
+@pytest.mark.parametrize("g,pages,rows,precision,kernel", [
+    (gqa(), (100, 16, 64, 1000), 64, 0, "ragged_few_kernelILi128"),                    # single tokens
+    (gqa(), (100, 16, 64, 1000), 64, 1, "ragged_few_f32_kernelILi128"),
+    (gqa(4, 1, 256, 256), (100, 16, 64, 1000), 64, 0, "ragged_few_kernelILi256"),
+    (gqa(6, 2, 80, 48), (100, 16, 64, 1000), 64, 0, "ragged_few_kernelILi128"),
+    (gqa(12, 4, 64, 64), (100, 16, 64, 1000), 64 * 10, 0, "ragged_few_kernelILi64"),   # 30 packed rows each
+    (gqa(12, 4, 64, 64), (100, 16, 64, 1000), 64 * 11, 0, "ragged_tc_kernelILi2ELi1ELi1"),
+    (gqa(), (100, 16, 4, 1000), 700, 0, "ragged_tc_kernelILi2ELi2ELi2"),
+    (gqa(8, 2, 96, 128), (100, 16, 4, 1000), 700, 0, "ragged_tc_kernelILi2ELi0ELi0"),
+    (gqa(8, 2, 256, 256), (100, 16, 4, 1000), 700, 0, "ragged_tc_kernelILi1ELi4ELi4"),
+    (gqa(8, 2, 192, 128), (100, 16, 4, 1000), 700, 0, "ragged_tc_kernelILi1ELi0ELi0"),
+    (gqa(), (100, 16, 4, 10), 200, 0, "ragged_few_kernelILi128"),                      # little work
+    (gqa(), (100, 16, 4, 1000), 700, 1, "ragged_plain_kernelIfLi64"),
+    (gqa(8, 2, 512, 512), (100, 16, 4, 1000), 700, 0, "ragged_plain_kernelI13__nv_bfloat16Li16"),
+    (gqa(130, 1, 64, 64), (100, 16, 4, 1000), 700, 0, "ragged_plain_kernelI13__nv_bfloat16Li64")])
+def test_kernels_of_the_attention(library, g, pages, rows, precision, kernel):
+    """Each by the call's sizes; all may start before the kernel ahead of them has ended."""
+    seen, status = attend(library, g, pages, rows, precision)
+    assert status == OK and any(kernel in l.name for l in seen), [l.name for l in seen]
+    assert all(l.dependent and l.smem <= 227 * 1024 for l in seen)
+
+
+def test_work_memory_of_long_tables_stays_bounded(library):
+    """The sums of ranges: 2^19 rows of them, however many requests and however long their tables."""
+    for requests, most in ((1, 1 << 17), (64, 4096), (4096, 4096), (8000, 1 << 17)):
+        g, p = gqa(32, 8), S.Pages(1 << 20, 16, requests, min(most, (1 << 27) - 1))
+        need = library.lib.zq_paged_work_bytes(C.byref(g), C.byref(p), requests, 0)
+        assert need <= 2 ** 19 * 4 * 130 * 4 + 4 * requests, (requests, most, need)

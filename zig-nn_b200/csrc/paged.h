@@ -31,8 +31,8 @@ int launch_paged_write(const PagedWriteArgs& a, bool f32, cudaStream_t st);
 
 // ---- attention of ragged rows (paged_attention.cu, paged_attention_tc.cu) ----------------------------------------------
 // Rows row_start[i] .. row_start[i + 1] - 1 are the last tokens of request i. Over pages: it holds lens[i] tokens, token t in place
-// t % page of page tables[i][t / page]; an entry outside 0 .. pages - 1 stands for a page of zeros. Packed (lens null): its tokens
-// are its rows, k and v their own.
+// t % page of page tables[i][t / page]; an entry outside 0 .. pages - 1 stands for a page of zeros. Packed: its tokens are its
+// rows, k and v their own.
 struct RaggedArgs {
     GqaShape s;
     const void *q, *k, *v;
@@ -43,6 +43,7 @@ struct RaggedArgs {
     const int32_t *row_start, *lens, *tables;
     uint32_t requests, rows, table_ld, shift, pages;
     uint32_t capacity;  // tokens of a request at most
+    bool paged;
     void* work;
 };
 size_t ragged_work_bytes(const RaggedArgs& a, bool f32);

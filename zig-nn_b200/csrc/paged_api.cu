@@ -24,7 +24,7 @@ int check(const zq_pages* p, uint32_t& shift) {
     return ZQ_OK;
 }
 
-RaggedArgs args_of(const zq_gqa* g, uint32_t rows, uint32_t requests, uint32_t capacity) {
+RaggedArgs args_of(const zq_gqa* g, bool paged, uint32_t rows, uint32_t requests, uint32_t capacity) {
     RaggedArgs a{};
     a.s = shape_of(g);
     a.q_ld = (size_t)g->heads * a.s.dimp;
@@ -35,6 +35,7 @@ RaggedArgs args_of(const zq_gqa* g, uint32_t rows, uint32_t requests, uint32_t c
     a.rows = rows;
     a.requests = requests;
     a.capacity = capacity;
+    a.paged = paged;
     return a;
 }
 
@@ -103,7 +104,7 @@ int zq_paged_cache_write(const zq_gqa* g, const zq_pages* p, const float* d_qkv,
 size_t zq_paged_work_bytes(const zq_gqa* g, const zq_pages* p, uint32_t rows, int precision) {
     uint32_t shift;
     if (!valid(g) || !small(g) || check(p, shift) != ZQ_OK || !known(precision)) return 0;
-    return ragged_work_bytes(args_of(g, rows, p->requests, p->max_pages * p->page_size), is_f32(precision));
+    return ragged_work_bytes(args_of(g, true, rows, p->requests, p->max_pages * p->page_size), is_f32(precision));
 }
 
 int zq_paged_attention(const zq_gqa* g, const zq_pages* p, const void* d_q, const void* d_k_cache, const void* d_v_cache, void* d_out,
@@ -117,7 +118,7 @@ int zq_paged_attention(const zq_gqa* g, const zq_pages* p, const void* d_q, cons
     if (!small(g) || rows >= 1u << 30) return ZQ_ERR_LIMIT;
     if (rows == 0) return ZQ_OK;
     if (!d_q || !d_out || !aligned(d_q) || !aligned(d_k_cache) || !aligned(d_v_cache) || !aligned(d_work)) return ZQ_ERR_BAD_ARG;
-    RaggedArgs a = args_of(g, rows, p->requests, p->max_pages * p->page_size);
+    RaggedArgs a = args_of(g, true, rows, p->requests, p->max_pages * p->page_size);
     a.q = d_q;
     a.k = d_k_cache;
     a.v = d_v_cache;
@@ -136,7 +137,7 @@ int zq_paged_attention(const zq_gqa* g, const zq_pages* p, const void* d_q, cons
 
 size_t zq_packed_work_bytes(const zq_gqa* g, uint32_t sequences, uint32_t rows, int precision) {
     if (!valid(g) || !small(g) || !known(precision)) return 0;
-    return ragged_work_bytes(args_of(g, rows, sequences, rows), is_f32(precision));
+    return ragged_work_bytes(args_of(g, false, rows, sequences, rows), is_f32(precision));
 }
 
 int zq_packed_attention(const zq_gqa* g, const void* d_q, size_t q_ld, const void* d_k, size_t k_ld, const void* d_v, size_t v_ld,
@@ -145,7 +146,7 @@ int zq_packed_attention(const zq_gqa* g, const void* d_q, size_t q_ld, const voi
     if (!valid(g) || !d_row_start || !sequences || !known(precision)) return ZQ_ERR_BAD_ARG;
     if (!small(g) || rows >= 1u << 30) return ZQ_ERR_LIMIT;
     if (rows == 0) return ZQ_OK;
-    RaggedArgs a = args_of(g, rows, sequences, rows);
+    RaggedArgs a = args_of(g, false, rows, sequences, rows);
     const size_t even = is_f32(precision) ? 4 : 8;  // rows start on 16-byte boundaries
     if (!d_q || !d_k || !d_v || !d_out || !aligned(d_q) || !aligned(d_k) || !aligned(d_v) || !aligned(d_work) || q_ld < a.q_ld ||
         k_ld < a.k_ld || v_ld < a.v_ld || q_ld % even || k_ld % even || v_ld % even)

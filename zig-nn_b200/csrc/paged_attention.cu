@@ -242,7 +242,7 @@ struct KeyStream {
           ring(shared + (threadIdx.x >> 5) * STAGES * stage_bytes), warps(gridDim.x * (THREADS / 32)) {}
 
     __device__ __forceinline__ void look_up() {
-        if (a.lens) page = (uint32_t)__ldg(a.tables + (size_t)it.request * a.table_ld + (key >> a.shift));
+        if (a.paged) page = (uint32_t)__ldg(a.tables + (size_t)it.request * a.table_ld + (key >> a.shift));
     }
     __device__ __forceinline__ void advance() {  // to an item that has keys
         more = false;
@@ -300,8 +300,8 @@ struct KeyStream {
     __device__ __forceinline__ void produce() {
         if (more) {
             const uint32_t dst = ring + filled * stage_bytes;
-            const bool there = !a.lens || page < a.pages;
-            const size_t row0 = !there ? 0 : a.lens ? ((size_t)page << a.shift) + (key & ((1u << a.shift) - 1)) : (size_t)it.row0 + key;
+            const bool there = !a.paged || page < a.pages;
+            const size_t row0 = !there ? 0 : a.paged ? ((size_t)page << a.shift) + (key & ((1u << a.shift) - 1)) : (size_t)it.row0 + key;
             const uint32_t rows = there ? min(16u, it.k_end - key) : 0, g = it.g;
             key += 16;
             if (key < it.k_end) look_up();
@@ -736,12 +736,17 @@ bool large(const GqaShape& s) { return s.dimp > 256 || s.vdimp > 256; }
 // Rows of a tile: 64 (or the tensor cores' tiles) where requests bring more packed rows than some tiles of the small kernel have, on the
 // mean. bf16, requests over 4000 keys, small kernel and tensor cores, us: 64 requests, 32 heads over 8 of 128, 18 packed rows each 71 and 90,
 // 30 rows 107 and 99, 60 rows 132 and 89; four of them 19 and 30, 23 and 30, 41 and 29; 16 requests, 4 over 1 of 256, 18 rows 24 and 37, 60 rows
-// 43 and 38; 12 over 4 of 64, 14 rows 16 and 28, 45 rows 29 and 29. f32: two tiles of four rows.
+// 43 and 38; 12 over 4 of 64, 14 rows 16 and 28, 45 rows 29 and 29. Small work goes there too: the tensor cores' three kernels take 26 us
+// whatever they have to do, the small one's rate is a tenth of theirs (packed, one sequence of 300 tokens, 8 heads over 2 of 128, 0.2
+// GFLOP, 13 and 30; six of up to 300, 12 over 4 of 64, 16 and 29; twenty of up to 200, 32 over 8 of 128, 0.8 GFLOP, 36 and 31; one of 500, 2
+// GFLOP, 43 and 31). f32: two tiles of four rows.
 uint32_t tile_rows(const RaggedArgs& a, bool f32) {
     const uint64_t rows = (uint64_t)a.rows * (a.s.heads / a.s.kv_heads);
     if (large(a.s)) return 16;
     if (f32) return rows <= 2ull * kFewRowsF32 * a.requests ? kFewRowsF32 : 64;
-    return rows <= 32ull * a.requests ? 16 : 64;
+    // keys of a row: half of a sequence on the mean; over pages what a table holds is all that the host knows
+    const double keys = a.paged ? a.capacity : 0.5 * a.rows / a.requests, flops = 2.0 * a.rows * a.s.heads * (a.s.dimp + a.s.vdimp) * keys;
+    return rows <= 32ull * a.requests || flops <= 0.6e9 ? 16 : 64;
 }
 
 // Ranges of a request's keys. As many as give each of the GPU's workers (a warp, or a CTA of the larger tile) one while the host sees

@@ -112,7 +112,7 @@ ragged_prep_kernel(const __grid_constant__ TcParams p, uint32_t tile_tokens) {
             const int32_t b = a.row_start[c + tid], e = a.row_start[c + tid + 1];
             const uint32_t row0 = b < 0 ? 0 : min((uint32_t)b, a.rows), end = e < 0 ? 0 : min((uint32_t)e, a.rows);
             n_rows = end > row0 ? end - row0 : 0;
-            len_of[tid] = a.lens ? min(a.lens[c + tid], (int32_t)a.capacity) : (int32_t)n_rows;
+            len_of[tid] = a.paged ? min(a.lens[c + tid], (int32_t)a.capacity) : (int32_t)n_rows;
             rows_of[tid] = n_rows;
             tiles = (n_rows + tile_tokens - 1) / tile_tokens;
         }
@@ -492,11 +492,11 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             // Pages of a tile's keys, 16 keys a lane; looked up a tile ahead. What is no page is one behind the last: zeros.
             auto look_up = [&](uint32_t t) {
                 const uint32_t j = (t * TK + (lane & 7) * 16) >> a.shift;
-                const uint32_t page = a.lens && j < a.table_ld ? (uint32_t)__ldg(a.tables + (size_t)w.t.request * a.table_ld + j) : a.pages;
+                const uint32_t page = a.paged && j < a.table_ld ? (uint32_t)__ldg(a.tables + (size_t)w.t.request * a.table_ld + j) : a.pages;
                 return min(page, a.pages);
             };
             auto copy = [&](const CUtensorMap* map, uint32_t dst, uint32_t key, uint32_t page, uint32_t col) {
-                tensor_copy_4d(dst, map, col, w.g, a.lens ? key & in_page : w.t.first_row + key, a.lens ? page : 0, full(slot));
+                tensor_copy_4d(dst, map, col, w.g, a.paged ? key & in_page : w.t.first_row + key, a.paged ? page : 0, full(slot));
             };
             asm volatile("fence.proxy.async.global;" ::: "memory");
             while (alive && next()) {
@@ -945,7 +945,7 @@ TcParams params_of(const RaggedArgs& a, size_t& bytes) {
     p.dv = (s.vdimp + 63) / 64;
     p.slot = (p.dk == 1 && p.dv == 1 ? 1 : 2) * ATOM;
     p.vk = p.dv <= 2 ? 128 : 64;
-    const uint32_t page = a.lens ? 1u << a.shift : TK;
+    const uint32_t page = a.paged ? 1u << a.shift : TK;
     p.kbox = page < TK ? page : TK;
     p.vbox = page < p.vk ? page : p.vk;
     p.slots_at = streams * p.dk * ATOM;
@@ -1000,7 +1000,7 @@ int launch(TcParams& p, cudaStream_t st) {
     const RaggedArgs& a = p.a;
     const GqaShape& s = a.s;
     CUtensorMap mq, mk, mv;
-    const uint64_t rows = a.lens ? 1ull << a.shift : a.rows, outer = a.lens ? a.pages : 1;
+    const uint64_t rows = a.paged ? 1ull << a.shift : a.rows, outer = a.paged ? a.pages : 1;
     int rc = map_4d(a.q, s.dimp, s.heads, a.rows, 1, a.q_ld, p.R, p.rt, &mq);
     if (rc == ZQ_OK) rc = map_4d(a.k, s.dimp, s.kv_heads, rows, outer, a.k_ld, 1, p.kbox, &mk);
     if (rc == ZQ_OK) rc = map_4d(a.v, s.vdimp, s.kv_heads, rows, outer, a.v_ld, 1, p.vbox, &mv);

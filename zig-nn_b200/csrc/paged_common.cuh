@@ -46,7 +46,7 @@ __device__ __forceinline__ void span_of(const RaggedArgs& a, uint32_t i, uint32_
     row0 = b < 0 ? 0 : min((uint32_t)b, a.rows);
     const uint32_t end = e < 0 ? 0 : min((uint32_t)e, a.rows);
     n_rows = end > row0 ? end - row0 : 0;
-    len = a.lens ? min(a.lens[i], (int32_t)a.capacity) : (int32_t)n_rows;
+    len = a.paged ? min(a.lens[i], (int32_t)a.capacity) : (int32_t)n_rows;
 }
 
 // Up to THREADS requests from one on: their items before one another, and what item_at needs of each.
@@ -171,7 +171,7 @@ __device__ __forceinline__ pair add2(pair a, pair b) {
 // First value of a token's keys (or values) of all heads; null: a page of zeros.
 template <typename T>
 __device__ __forceinline__ const T* token_row(const RaggedArgs& a, const Item& it, const T* base, size_t ld, uint32_t key) {
-    if (!a.lens) return base + (size_t)(it.row0 + key) * ld;
+    if (!a.paged) return base + (size_t)(it.row0 + key) * ld;
     const uint32_t page = (uint32_t)__ldg(a.tables + (size_t)it.request * a.table_ld + (key >> a.shift));
     if (page >= a.pages) return nullptr;
     return base + (((size_t)page << a.shift) + (key & ((1u << a.shift) - 1))) * ld;
