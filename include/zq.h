@@ -591,7 +591,7 @@ int zq_gqa_attention(const zq_gqa* g, const void* d_q, const void* d_k_cache, co
 
 /* ---- a cache of pages that requests share ---------------------------------------------------------------------
  * Keys and values of a layer lie in pages of page_size tokens (16, 32, ... 1024): [pages][page_size][kv_heads][dim up to 16],
- * initialised with finite values (zeros). Token t of request i is in place t % page_size of page d_tables[i][t / page_size]
+ * initialised with finite values (zeros); what a request holds stays finite. Token t of request i is in place t % page_size of page d_tables[i][t / page_size]
  * ([requests][max_pages]). Pages without a request lie in a ring d_free [pages]: d_span[1] of them, from place d_span[0] on.
  * pages * page_size and max_pages * page_size stay below 2^31, requests of a plan at 8192 (else ZQ_ERR_LIMIT); another page_size is
  * ZQ_ERR_UNSUPPORTED. Everything that changes from step to step is read on the device, so a step replays from a recording. */
@@ -614,14 +614,14 @@ int zq_page_plan(const zq_pages* p, const int32_t* d_new, const int32_t* d_lens,
                  int32_t* d_free, const int32_t* d_span, int32_t* d_span_out, int32_t* d_row_start, int32_t* d_pos,
                  int32_t* d_places, uint32_t rows, int32_t* d_status, zq_stream stream);
 /* zq_gqa_cache_write for pages: the rows' normalised queries to d_q, keys and values to d_places; a row whose place is none of the
- * cache's has its query only. ctx and slots of zq_gqa are not read here and below. */
+ * cache's has its query only; no place twice. ctx and slots of zq_gqa are not read here and below. */
 int zq_paged_cache_write(const zq_gqa* g, const zq_pages* p, const float* d_qkv, const float* d_q_norm, const float* d_k_norm,
                          const float* d_vmix, float* d_v_first, void* d_q, void* d_k_cache, void* d_v_cache, const int32_t* d_pos,
                          const int32_t* d_places, uint32_t rows, int precision, zq_stream stream);
 /* Causal softmax attention of a step: rows d_row_start[i] ... d_row_start[i + 1] - 1 of d_q are the last tokens of request i, which
  * holds d_lens[i] tokens (d_lens_out of the plan), each sees the tokens up to its own. Single tokens, chunks of prompts, or both.
  * d_out: act rows of pitch zq_dense_pitch(heads * vdim); rows of no request are left as they are, a row that sees no token is zero. A
- * table entry that is no page stands for a page of zeros. dim and vdim up to 512 (else ZQ_ERR_LIMIT). d_q, caches and d_work on
+ * table entry that is no page stands for a page of zeros. dim and vdim up to 512 (else ZQ_ERR_LIMIT). d_q, d_out, caches and d_work on
  * 16-byte boundaries; d_work: zq_paged_work_bytes, for one call at a time. */
 int zq_paged_attention(const zq_gqa* g, const zq_pages* p, const void* d_q, const void* d_k_cache, const void* d_v_cache,
                        void* d_out, const int32_t* d_row_start, const int32_t* d_lens, const int32_t* d_tables, uint32_t rows,
@@ -629,7 +629,8 @@ int zq_paged_attention(const zq_gqa* g, const zq_pages* p, const void* d_q, cons
 size_t zq_paged_work_bytes(const zq_gqa* g, const zq_pages* p, uint32_t rows, int precision);
 /* The same for whole sequences without a cache: rows d_row_start[i] ... d_row_start[i + 1] - 1 are sequence i, each row sees the
  * sequence's rows up to itself. d_q [rows][heads][dim up to 16], d_k [rows][kv_heads][dim up to 16], d_v [rows][kv_heads][vdim up to
- * 16] (zeros beyond dim); *_ld: values from row to row (parts of one projected row may be given), 16-byte boundaries. */
+ * 16] (zeros beyond dim); *_ld: values from row to row (parts of one projected row may be given); all, d_out and d_work too, on
+ * 16-byte boundaries. */
 int zq_packed_attention(const zq_gqa* g, const void* d_q, size_t q_ld, const void* d_k, size_t k_ld, const void* d_v, size_t v_ld,
                         void* d_out, const int32_t* d_row_start, uint32_t sequences, uint32_t rows, void* d_work,
                         size_t work_bytes, int precision, zq_stream stream);

@@ -1,5 +1,6 @@
 """The paged cache and packed prompts on the GPU against plain forms in 64 bits."""
 import random
+import threading
 
 import pytest
 import torch
@@ -162,8 +163,9 @@ def paged_case(zq, heads, kv_heads, dim, vdim, f32, page, held, new, seed=0, pad
     return cache, q, i32(row_start), i32(lens), tables.cuda(), keys, values
 
 
-def check_paged(zq, heads, kv_heads, dim, vdim, f32, page, held, new, seed=0, pad=3, **more):
+def check_paged(zq, heads, kv_heads, dim, vdim, f32, page, held, new, seed=0, pad=3, wide=0, **more):
     cache, q, row_start, lens, tables, keys, values = paged_case(zq, heads, kv_heads, dim, vdim, f32, page, held, new, seed, pad, **more)
+    tables = torch.nn.functional.pad(tables, (0, wide), value=-1)
     out = torch.full((q.shape[0], zq.dense_pitch(heads * vdim)), 7.0, dtype=q.dtype, device="cuda")
     got = cache.attend(q, row_start, lens, tables, out=out)
     assert got is out
@@ -366,6 +368,42 @@ def test_many_requests(zq, f32):
     check_paged(zq, 4, 2, 64, 64, f32, 16, [rng.randint(0, 90) for _ in range(1100)], [rng.choice((0, 1, 60)) for _ in range(1100)], seed=1)
 
 
+@pytest.mark.parametrize("heads,kv_heads,dim,vdim", [h for h in HEADS if h[0] // h[1] < 32])
+@pytest.mark.parametrize("page", [16, 256])
+def test_chunks_beside_single_tokens(zq, heads, kv_heads, dim, vdim, page):
+    """No more rows on the mean than the small kernel takes, and some requests with more than that: each kind has its kernel."""
+    rng, R = random.Random(heads), heads // kv_heads
+    some = 32 // R
+    new = [1] * 20 + [0, some, some + 1, 0, 1, some] + [1] * 14
+    new[rng.randrange(20)] = 40 * some - sum(new) - 5
+    held = [rng.choice((0, 5, 17, 130, 400, 900)) for _ in new]
+    check_paged(zq, heads, kv_heads, dim, vdim, False, page, held, new, wide=(1 << 21) // page)
+    check_paged(zq, heads, kv_heads, dim, vdim, False, page, held, [min(n, some) for n in new], seed=1, wide=(1 << 21) // page)
+
+
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("new", [1, 700])
+def test_queries_that_are_nan_stay_so(zq, f32, new):
+    cache, q, row_start, lens, tables, *_ = paged_case(zq, 8, 2, 128, 128, f32, 16, [1500, 40], [new, new])
+    want = cache.attend(q, row_start, lens, tables)
+    q[new, 3] = float("nan")
+    got = cache.attend(q, row_start, lens, tables)
+    mine = slice(3 * 128, 4 * 128)
+    assert torch.isnan(got[new, mine]).all()
+    got[new, mine] = want[new, mine]
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("new", [1, 700])
+def test_lengths_that_cannot_be_hold_nothing(zq, f32, new):
+    cache, q, row_start, lens, tables, keys, values = paged_case(zq, 8, 2, 128, 128, f32, 16, [1500, 40], [new, new])
+    lens[0] = -2 ** 31
+    got = cache.attend(q, row_start, lens, tables)
+    want, tol = plain.attention(q[new:], keys[1], values[1], 41 + torch.arange(new, device="cuda"), cache.g.scale, not f32)
+    assert (got[:new] == 0).all() and ((got[new:].view(new, 8, 128).double() - want).abs() <= tol).all()
+
+
 # ---- together
 @pytest.mark.parametrize("f32", [False, True])
 @pytest.mark.parametrize("heads,kv_heads,dim", [(8, 2, 128), (4, 1, 256), (6, 3, 40)])
@@ -454,7 +492,49 @@ def test_calls_on_two_streams_at_once(zq):
         assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+def test_one_cache_from_two_threads(zq):
+    """Calls of different sizes, each with its own streams and results."""
+    cache, q, row_start, lens, tables, *_ = paged_case(zq, 8, 2, 128, 128, False, 16, [2000, 30, 400], [200, 1, 1])
+    parts = [(q, row_start, lens, tables), (q[200:].contiguous(), i32([0, 1, 2]), lens[1:].clone(), tables[1:, :30].contiguous())]
+    want, bad = [cache.attend(*p) for p in parts], []
+    torch.cuda.synchronize()
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got = [cache.attend(*parts[i]) for _ in range(200)]
+            torch.cuda.current_stream().synchronize()
+        bad.extend(i for g in got if not torch.equal(g, want[i]))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not bad
+
+
 # ---- refusals
+def test_refusals_of_memory_elsewhere(zq):
+    from zignn_b200 import _lib
+    cache, q, row_start, lens, tables, *_ = paged_case(zq, 4, 2, 64, 64, False, 16, [60, 20], [1, 1])
+    odd = torch.zeros(2 * 256 + 1, dtype=torch.bfloat16, device="cuda")[1:].view(2, 256)
+    with pytest.raises(_lib.ZqError) as e:
+        cache.attend(q, row_start, lens, tables, out=odd)
+    assert e.value.status == 1
+    with pytest.raises(_lib.ZqError) as e:
+        zq.packed_attention(q, q[:, :2], q[:, :2], row_start, 0.1, out=odd)
+    assert e.value.status == 1
+    for none in (i32([]), i32([0])):
+        with pytest.raises(ValueError):
+            zq.packed_attention(q, q[:, :2], q[:, :2], none, 0.1)
+    cache.k = cache.k.cpu()  # stands for a cache of another device
+    with pytest.raises(ValueError):
+        cache.attend(q, row_start, lens, tables)
+    with pytest.raises(ValueError):
+        cache.write(torch.zeros(2, (4 + 2 * 2) * 64, device="cuda"), torch.ones(64, device="cuda"), torch.ones(64, device="cuda"), lens, lens)
+
+
 def test_refusals(zq):
     from zignn_b200 import _lib
     cache, q, row_start, lens, tables, *_ = paged_case(zq, 4, 2, 64, 64, False, 16, [60, 20], [1, 1])

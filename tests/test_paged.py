@@ -80,13 +80,14 @@ def test_refusals_of_the_write(library):
     refused(write(library, gqa(8, 2, 0)), BAD_ARG)
     refused(write(library, precision=2), BAD_ARG)
     refused(write(library, pages=(100, 20, 1, 1)), UNSUPPORTED)
+    refused(write(library, rows=1 << 30), LIMIT)
     refused(write(library, rows=0), OK)
 
 
 def test_refusals_of_the_attention(library):
     for name in ("q", "k", "v", "out", "row_start", "lens", "tables"):
         refused(attend(library, **{name: None}), BAD_ARG)
-    for name in ("q", "k", "v", "work"):
+    for name in ("q", "k", "v", "out", "work"):
         refused(attend(library, **{name: C.c_void_p((1 << 20) + 8)}), BAD_ARG)
     refused(attend(library, rows=2000, short=1), BAD_ARG)
     refused(attend(library, rows=2000, work=None), BAD_ARG)
@@ -101,7 +102,7 @@ def test_refusals_of_the_attention(library):
 def test_refusals_of_packed_prompts(library):
     for name in ("q", "k", "v", "out", "row_start"):
         refused(packed(library, **{name: None}), BAD_ARG)
-    for name in ("q", "k", "v", "work"):
+    for name in ("q", "k", "v", "out", "work"):
         refused(packed(library, **{name: C.c_void_p((1 << 20) + 4)}), BAD_ARG)
     refused(packed(library, lds=(1023, 256, 256)), BAD_ARG)
     refused(packed(library, lds=(1024, 255, 256)), BAD_ARG)
@@ -134,6 +135,15 @@ def test_kernels_of_the_attention(library, g, pages, rows, precision, kernel):
     seen, status = attend(library, g, pages, rows, precision)
     assert status == OK and any(kernel in l.name for l in seen), [l.name for l in seen]
     assert all(l.dependent and l.smem <= 227 * 1024 for l in seen)
+
+
+@pytest.mark.parametrize("rows,kernels", [
+    (64, {"few"}), (66, {"few"}),                       # single tokens; two rows more are little work
+    (64 * 8, {"few", "tc"}),                            # 32 packed rows on the mean: single tokens and chunks may lie behind that
+    (64 * 8 + 1, {"tc"})])
+def test_both_kernels_where_requests_may_differ(library, rows, kernels):
+    seen, status = attend(library, pages=(100, 16, 64, 1000), rows=rows)
+    assert status == OK and {k for k in ("few", "tc", "plain") if any("ragged_%s_kernel" % k in l.name for l in seen)} == kernels
 
 
 def test_work_memory_of_long_tables_stays_bounded(library):

@@ -668,11 +668,12 @@ class PagedCache:
         self.k = torch.zeros(pages, page_size, kv_heads, up16(dim), dtype=self._dtype, device="cuda")
         self.v = torch.zeros(pages, page_size, kv_heads, up16(vdim), dtype=self._dtype, device="cuda")
         self._pages = S.Pages(pages, page_size, 1, 1)
-        self._need = (0, 0, 0, 0)  # requests, pages of a table, rows and work bytes of the last call
+        self._last = (0, 0, 0), self._pages, 0  # of the last call: requests, pages of a table, rows; its sizes and work bytes
 
     def write(self, qkv, q_norm, k_norm, pos, places, vmix=None, v_first=None):
         """Normalised queries [rows, heads, dim up to 16] of the projected rows; their keys and values go to the places of the plan."""
         g, rows = self.g, qkv.shape[0]
+        _here(self.k, "the cache")
         if _here(_dev_f32(qkv), "qkv").shape != (rows, (g.heads + g.kv_heads) * g.dim + g.kv_heads * g.vdim):
             raise ValueError("qkv: shape %s" % list(qkv.shape))
         _int_rows(pos, "pos", rows)
@@ -696,12 +697,13 @@ class PagedCache:
         _int_rows(lens, "lens", requests)
         if q.dtype != self._dtype or not q.is_contiguous() or q.shape != (rows, g.heads, self.k.shape[3]):
             raise ValueError("q: expected the contiguous %s rows of write()" % self._dtype)
+        _here(self.k, "the cache")
         out = _result(_here(q, "q"), out, rows, self._pitch)
-        p = self._pages
-        p.requests, p.max_pages = requests, width
-        if self._need[:3] != (requests, width, rows):
-            self._need = (requests, width, rows, lib.zq_paged_work_bytes(C.byref(g), C.byref(p), rows, int(self.f32)))
-        need = self._need[3]
+        last, p, need = self._last  # replaced as a whole: another thread's call may be under way
+        if last != (requests, width, rows):
+            p = S.Pages(self._pages.pages, self._pages.page_size, requests, width)
+            need = lib.zq_paged_work_bytes(C.byref(g), C.byref(p), rows, int(self.f32))
+            self._last = (requests, width, rows), p, need
         work = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
         rc = lib.zq_paged_attention(C.byref(g), C.byref(p), q.data_ptr(), self.k.data_ptr(), self.v.data_ptr(), out.data_ptr(),
                                     row_start.data_ptr(), lens.data_ptr(), tables.data_ptr(), rows, _address(work), need,
@@ -736,13 +738,14 @@ def packed_attention(q, k, v, row_start, scale, vdim=None, out=None):
         if t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != t.shape[2]) or (rows > 1 and ld < n):
             raise ValueError("%s: a row's heads have to lie behind one another" % name)
         lds.append(ld if rows > 1 else n)
-    _int_rows(row_start, "row_start", -1)
+    sequences = _int_rows(row_start, "row_start", -1).shape[0] - 1
+    if sequences < 1:
+        raise ValueError("row_start: no sequence")
     vdim = e if vdim is None else int(vdim)
     if not e - 16 < vdim <= e:
         raise ValueError("vdim %d of %d columns" % (vdim, e))
     out = _result(q, out, rows, (heads * vdim + 63) // 64 * 64)
     g = S.Gqa(heads, kv_heads, d, vdim, 0, 0, scale, 0.0, 0.0, 0.0)
-    sequences = row_start.shape[0] - 1
     need = lib.zq_packed_work_bytes(C.byref(g), sequences, rows, int(f32))
     work = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
     rc = lib.zq_packed_attention(C.byref(g), q.data_ptr(), lds[0], k.data_ptr(), lds[1], v.data_ptr(), lds[2], out.data_ptr(),

@@ -44,6 +44,8 @@ struct RaggedArgs {
     uint32_t requests, rows, table_ld, shift, pages;
     uint32_t capacity;  // tokens of a request at most
     bool paged;
+    // Tokens of a request up to which the kernel of few rows takes it, when the tensor cores take the others; 0: one form for all.
+    uint32_t split;
     void* work;
 };
 size_t ragged_work_bytes(const RaggedArgs& a, bool f32);
@@ -51,6 +53,7 @@ int launch_ragged_attention(const RaggedArgs& a, bool f32, cudaStream_t st);
 // Its form on tcgen05, for requests with more than a few rows (bf16): whether it has one, its work memory.
 bool ragged_tc_takes(const RaggedArgs& a);
 size_t ragged_tc_work_bytes(const RaggedArgs& a);
-int launch_ragged_tc(const RaggedArgs& a, cudaStream_t st);
+// n_ranges: a word per row that it sets to 0, or null.
+int launch_ragged_tc(const RaggedArgs& a, uint32_t* n_ranges, cudaStream_t st);
 
 }  // namespace zq

@@ -79,6 +79,7 @@ int zq_paged_cache_write(const zq_gqa* g, const zq_pages* p, const float* d_qkv,
     const int rc = check(p, shift);
     if (rc != ZQ_OK) return rc;
     if (!d_k_cache || !d_v_cache || !d_q_norm || !d_k_norm || !known(precision)) return ZQ_ERR_BAD_ARG;
+    if (rows >= 1u << 30) return ZQ_ERR_LIMIT;
     if (rows == 0) return ZQ_OK;
     if (!d_qkv || (d_vmix && !d_v_first) || !d_q || !d_pos || !d_places) return ZQ_ERR_BAD_ARG;
     PagedWriteArgs a{};
@@ -117,7 +118,7 @@ int zq_paged_attention(const zq_gqa* g, const zq_pages* p, const void* d_q, cons
     if (!d_k_cache || !d_v_cache || !d_row_start || !d_lens || !d_tables || !known(precision)) return ZQ_ERR_BAD_ARG;
     if (!small(g) || rows >= 1u << 30) return ZQ_ERR_LIMIT;
     if (rows == 0) return ZQ_OK;
-    if (!d_q || !d_out || !aligned(d_q) || !aligned(d_k_cache) || !aligned(d_v_cache) || !aligned(d_work)) return ZQ_ERR_BAD_ARG;
+    if (!d_q || !d_out || !aligned(d_q) || !aligned(d_out) || !aligned(d_k_cache) || !aligned(d_v_cache) || !aligned(d_work)) return ZQ_ERR_BAD_ARG;
     RaggedArgs a = args_of(g, true, rows, p->requests, p->max_pages * p->page_size);
     a.q = d_q;
     a.k = d_k_cache;
@@ -148,8 +149,8 @@ int zq_packed_attention(const zq_gqa* g, const void* d_q, size_t q_ld, const voi
     if (rows == 0) return ZQ_OK;
     RaggedArgs a = args_of(g, false, rows, sequences, rows);
     const size_t even = is_f32(precision) ? 4 : 8;  // rows start on 16-byte boundaries
-    if (!d_q || !d_k || !d_v || !d_out || !aligned(d_q) || !aligned(d_k) || !aligned(d_v) || !aligned(d_work) || q_ld < a.q_ld ||
-        k_ld < a.k_ld || v_ld < a.v_ld || q_ld % even || k_ld % even || v_ld % even)
+    if (!d_q || !d_k || !d_v || !d_out || !aligned(d_q) || !aligned(d_k) || !aligned(d_v) || !aligned(d_out) || !aligned(d_work) ||
+        q_ld < a.q_ld || k_ld < a.k_ld || v_ld < a.v_ld || q_ld % even || k_ld % even || v_ld % even)
         return ZQ_ERR_BAD_ARG;
     a.q = d_q;
     a.k = d_k;

@@ -740,14 +740,22 @@ bool large(const GqaShape& s) { return s.dimp > 256 || s.vdimp > 256; }
 // whatever they have to do, the small one's rate is a tenth of theirs (packed, one sequence of 300 tokens, 8 heads over 2 of 128, 0.2
 // GFLOP, 13 and 30; six of up to 300, 12 over 4 of 64, 16 and 29; twenty of up to 200, 32 over 8 of 128, 0.8 GFLOP, 36 and 31; one of 500, 2
 // GFLOP, 43 and 31). f32: two tiles of four rows.
-uint32_t tile_rows(const RaggedArgs& a, bool f32) {
+// (The rows counted are those beyond one of each request: single tokens are the small kernel's.) Up to 32 packed rows on the mean the
+// rows may be single tokens of most requests and a chunk of one: both forms run, and each takes the requests of its kind. Over 4096 keys,
+// 32 heads over 8 of 128, us, small kernel, tensor cores, both: 127 tokens and a chunk of 512 404, 279, 211; 255 and one of 1500 1106, 520,
+// 476; four rows each of 64 requests, nothing for the tensor cores, 74, 114, 84.
+enum class Form { kFew, kTensor, kBoth, kPlain };
+Form form_of(const RaggedArgs& a, bool f32) {
     const uint64_t rows = (uint64_t)a.rows * (a.s.heads / a.s.kv_heads);
-    if (large(a.s)) return 16;
-    if (f32) return rows <= 2ull * kFewRowsF32 * a.requests ? kFewRowsF32 : 64;
+    if (large(a.s)) return Form::kPlain;
+    if (f32) return rows <= 2ull * kFewRowsF32 * a.requests ? Form::kFew : Form::kPlain;
     // keys of a row: half of a sequence on the mean; over pages what a table holds is all that the host knows
-    const double keys = a.paged ? a.capacity : 0.5 * a.rows / a.requests, flops = 2.0 * a.rows * a.s.heads * (a.s.dimp + a.s.vdimp) * keys;
-    return rows <= 32ull * a.requests || flops <= 0.6e9 ? 16 : 64;
+    const double keys = a.paged ? a.capacity : 0.5 * a.rows / a.requests, more = (double)a.rows - a.requests;
+    if (2.0 * more * a.s.heads * (a.s.dimp + a.s.vdimp) * keys <= 0.6e9) return Form::kFew;
+    if (!ragged_tc_takes(a)) return Form::kPlain;
+    return rows <= 32ull * a.requests ? Form::kBoth : Form::kTensor;
 }
+uint32_t tile_rows(const RaggedArgs& a, Form form, bool f32) { return form != Form::kPlain ? (f32 ? kFewRowsF32 : 16) : large(a.s) ? 16 : 64; }
 
 // Ranges of a request's keys. As many as give each of the GPU's workers (a warp, or a CTA of the larger tile) one while the host sees
 // fewer units of work than that, but no more than sqrt(0.4 keys): a range less costs a worker 16 keys (0.5 us), a range more costs the
@@ -834,16 +842,28 @@ int few_any(const RaggedCall& c, bool f32, cudaStream_t st) {
 }  // namespace
 
 size_t ragged_work_bytes(const RaggedArgs& a, bool f32) {
-    const uint32_t M = tile_rows(a, f32);
-    return !f32 && M == 64 && ragged_tc_takes(a) ? ragged_tc_work_bytes(a) : plan_bytes(a, plan_of(a, M, f32));
+    const Form form = form_of(a, f32);
+    const size_t tc = form == Form::kTensor || form == Form::kBoth ? ragged_tc_work_bytes(a) : 0;
+    return form == Form::kTensor ? tc : tc + plan_bytes(a, plan_of(a, tile_rows(a, form, f32), f32));
 }
 
-int launch_ragged_attention(const RaggedArgs& a, bool f32, cudaStream_t st) {
+int launch_ragged_attention(const RaggedArgs& args, bool f32, cudaStream_t st) {
+    RaggedArgs a = args;
     if (a.rows == 0 || a.requests == 0) return ZQ_OK;
-    const uint32_t M = tile_rows(a, f32);
-    if (!f32 && M == 64 && ragged_tc_takes(a)) return launch_ragged_tc(a, st);
-    const RaggedCall c{a, plan_of(a, M, f32)};
-    const int rc = M <= 16 && !large(a.s) ? few_any(c, f32, st) : f32 ? plain_any<float>(c, st) : plain_any<bf16>(c, st);
+    const Form form = form_of(a, f32);
+    if (form == Form::kTensor) return launch_ragged_tc(a, nullptr, st);
+    const uint32_t R = a.s.heads / a.s.kv_heads;
+    if (form == Form::kBoth) {
+        a.split = R <= 32 ? 32 / R : 1;
+        a.work = static_cast<char*>(args.work) + ragged_tc_work_bytes(a);
+    }
+    const RaggedCall c{a, plan_of(a, tile_rows(a, form, f32), f32)};
+    int rc = ZQ_OK;
+    if (form == Form::kBoth) {
+        a.work = args.work;
+        rc = launch_ragged_tc(a, c.p.max_ranges < 2 ? nullptr : c.p.n_ranges, st);
+    }
+    if (rc == ZQ_OK) rc = form != Form::kPlain ? few_any(c, f32, st) : f32 ? plain_any<float>(c, st) : plain_any<bf16>(c, st);
     if (rc != ZQ_OK || c.p.max_ranges < 2) return rc;
     const dim3 grid(((uint64_t)a.rows * a.s.heads + 3) / 4);
     return done(f32 ? launch_pdl_split(true, ragged_combine_kernel<float>, grid, dim3(128), 0, st, c)

@@ -65,6 +65,7 @@ struct TcParams {
     uint32_t slot, vk;         // bytes of a slot; keys of a slot of values
     uint32_t kbox, vbox;       // rows of a copy
     uint32_t n_slots, slots_at;
+    uint32_t* n_ranges;        // a word per row for the kernel of few rows, set to 0; or null
     unsigned int* err;
 };
 
@@ -104,6 +105,8 @@ ragged_prep_kernel(const __grid_constant__ TcParams p, uint32_t tile_tokens) {
     pdl_wait();
     const RaggedArgs& a = p.a;
     const uint32_t tid = threadIdx.x;
+    if (p.n_ranges)
+        for (uint32_t i = tid; i < a.rows; i += kPrepThreads) p.n_ranges[i] = 0;
     uint32_t n_tiles = 0;
     uint64_t cost = 0;
     for (uint32_t c = 0; c < a.requests; c += kPrepThreads) {
@@ -112,9 +115,9 @@ ragged_prep_kernel(const __grid_constant__ TcParams p, uint32_t tile_tokens) {
             const int32_t b = a.row_start[c + tid], e = a.row_start[c + tid + 1];
             const uint32_t row0 = b < 0 ? 0 : min((uint32_t)b, a.rows), end = e < 0 ? 0 : min((uint32_t)e, a.rows);
             n_rows = end > row0 ? end - row0 : 0;
-            len_of[tid] = a.paged ? min(a.lens[c + tid], (int32_t)a.capacity) : (int32_t)n_rows;
+            len_of[tid] = a.paged ? max(0, min(a.lens[c + tid], (int32_t)a.capacity)) : (int32_t)n_rows;
             rows_of[tid] = n_rows;
-            tiles = (n_rows + tile_tokens - 1) / tile_tokens;
+            tiles = n_rows > a.split ? (n_rows + tile_tokens - 1) / tile_tokens : 0;
         }
         uint64_t total;
         const uint64_t scan = block_scan(tiles, sums, total);
@@ -301,13 +304,19 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
 // 2^x of two numbers up to 2^16 by multiply-adds: x = j + f with j the nearest integer (by adding 1.5 x 2^23, which leaves j in the low
 // bits), 2^f on [-1/2, 1/2] by the cubic of least relative error (7.5e-5, a thirtieth of the rounding to bf16 that follows), j added to the
-// exponent. Below 2^-125 the result is 2^-125: a hidden key's weight, then, which no sum notices.
+// exponent. Below 2^-125 the result is 2^-125: a hidden key's weight, then, which no sum notices. Of a NaN it is
+// 2^128 - 2^104, which bf16 rounds to infinity.
 __device__ __forceinline__ void exp2_pair(pair x, uint32_t& a, uint32_t& b) {
     uint32_t u, v;
     split(x, u, v);
-    x = pair_of(fmaxf(__uint_as_float(u), -125.0f), fmaxf(__uint_as_float(v), -125.0f));
+    x = pair_of(max_nan(__uint_as_float(u), -125.0f), max_nan(__uint_as_float(v), -125.0f));
     const pair t = add2(x, pair_of(12582912.0f, 12582912.0f)), j = add2(t, pair_of(-12582912.0f, -12582912.0f));
     const pair f = fma2(j, pair_of(-1.0f, -1.0f), x);
     pair y = fma2(f, pair_of(0.05517167f, 0.05517167f), pair_of(0.24261113f, 0.24261113f));
@@ -726,7 +735,7 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
 #pragma unroll
                         for (int i = 0; i < 128; ++i) sv[i >> 5][i & 31] = __float_as_uint(__uint_as_float(sv[i >> 5][i & 31]) * p.scale2);
                     }
-                    if (w.t.see0 < (int32_t)((t + 1) * TK)) {  // some row does not see all of the tile
+                    if (w.t.see0 - (int32_t)(t * TK) < (int32_t)TK) {  // some row does not see all of the tile
                         const int lim = see - (int)(t * TK);
 #pragma unroll
                         for (int i = 0; i < 128; ++i)
@@ -786,7 +795,8 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             if (w.whole) {
                 bf16* row = static_cast<bf16*>(a.out) + (size_t)(w.t.row0 + token) * a.out_pitch;
                 bf16* out = row + (size_t)head * s.vdim;
-                const float inv = mx_run > -INFINITY ? 1.0f / l : 0.0f;
+                const bool none = mx_run == -INFINITY && l == l;  // sees nothing; scores that are NaN stay so
+                const float inv = 1.0f / l;
                 const uint32_t even = (uint32_t)(uintptr_t)out & 31u;  // 32-byte stores where they may be: a sector each
 #pragma unroll 1
                 for (uint32_t col = 0; col < s.vdim; col += 32) {
@@ -796,7 +806,7 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                         tc_wait_ld();
                     }
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) o[i] = mx_run > -INFINITY ? __float_as_uint(__uint_as_float(o[i]) * inv) : 0u;
+                    for (int i = 0; i < 32; ++i) o[i] = none ? 0u : __float_as_uint(__uint_as_float(o[i]) * inv);
 #pragma unroll
                     for (int i = 0; i < 16; ++i) o[i] = pack2(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1]));
                     if (real && even == 0 && col + 32 <= s.vdim) {
@@ -906,14 +916,14 @@ ragged_join_kernel(const __grid_constant__ TcParams p) {
 #pragma unroll
             for (uint32_t k = 0; k < 4; ++k) {
                 const float g = exp2f(mi[k] - shift);
-                if (g > 0.0f) {  // not a piece of which the row sees nothing
+                if (g > 0.0f || li[k] != li[k]) {  // not a piece of which the row sees nothing
                     sum = fmaf(g, li[k], sum);
 #pragma unroll
                     for (int e = 0; e < 8; ++e) acc[e] = fmaf(g, v[k][e], acc[e]);
                 }
             }
         }
-        const float inv = mx > -INFINITY ? 1.0f / sum : 0.0f;
+        const float inv = mx > -INFINITY || sum != sum ? 1.0f / sum : 0.0f;
         uint32_t o[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] = pack2(acc[2 * e] * inv, acc[2 * e + 1] * inv);
@@ -1024,9 +1034,10 @@ size_t ragged_tc_work_bytes(const RaggedArgs& a) {
     return bytes;
 }
 
-int launch_ragged_tc(const RaggedArgs& a, cudaStream_t st) {
+int launch_ragged_tc(const RaggedArgs& a, uint32_t* n_ranges, cudaStream_t st) {
     size_t bytes;
     TcParams p = params_of(a, bytes);
+    p.n_ranges = n_ranges;
     const uint32_t d = a.s.dimp == a.s.vdimp ? a.s.dimp : 0;
     if (streams_of(a.s) == 2) return d == 64 ? launch<2, 1, 1>(p, st) : d == 128 ? launch<2, 2, 2>(p, st) : launch<2, 0, 0>(p, st);
     return d == 256 ? launch<1, 4, 4>(p, st) : launch<1, 0, 0>(p, st);

@@ -46,7 +46,7 @@ __device__ __forceinline__ void span_of(const RaggedArgs& a, uint32_t i, uint32_
     row0 = b < 0 ? 0 : min((uint32_t)b, a.rows);
     const uint32_t end = e < 0 ? 0 : min((uint32_t)e, a.rows);
     n_rows = end > row0 ? end - row0 : 0;
-    len = a.paged ? min(a.lens[i], (int32_t)a.capacity) : (int32_t)n_rows;
+    len = a.paged ? max(0, min(a.lens[i], (int32_t)a.capacity)) : (int32_t)n_rows;
 }
 
 // Up to THREADS requests from one on: their items before one another, and what item_at needs of each.
@@ -66,7 +66,8 @@ __device__ __forceinline__ uint32_t count_items(const RaggedArgs& a, const Ragge
     int32_t len = 0;
     if (c + tid < a.requests) {
         span_of(a, c + tid, row0, n_rows, len);
-        ranges = ranges_of(len > 0 ? len : 0, p.block, p.fill, p.most_keys, per);
+        if (a.split && n_rows > a.split) n_rows = 0;  // the tensor cores'
+        ranges = ranges_of(len, p.block, p.fill, p.most_keys, per);
         scan = (p.tokens > 1 ? (n_rows + p.tokens - 1) / p.tokens : n_rows) * ranges * a.s.kv_heads * p.head_tiles;
     }
 #pragma unroll
@@ -119,7 +120,7 @@ __device__ __forceinline__ Item item_at(const RaggedArgs& a, const RaggedPlan& p
     }
     it.range = u;
     it.k_begin = u * q.per[lo];
-    it.k_end = min(it.len > 0 ? (uint32_t)it.len : 0u, it.k_begin + q.per[lo]);
+    it.k_end = min((uint32_t)it.len, it.k_begin + q.per[lo]);
     return it;
 }
 
