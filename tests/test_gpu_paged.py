@@ -369,16 +369,17 @@ def test_many_requests(zq, f32):
 
 
 @pytest.mark.parametrize("heads,kv_heads,dim,vdim", [h for h in HEADS if h[0] // h[1] < 32])
+@pytest.mark.parametrize("f32", [False, True])
 @pytest.mark.parametrize("page", [16, 256])
-def test_chunks_beside_single_tokens(zq, heads, kv_heads, dim, vdim, page):
+def test_chunks_beside_single_tokens(zq, heads, kv_heads, dim, vdim, page, f32):
     """No more rows on the mean than the small kernel takes, and some requests with more than that: each kind has its kernel."""
     rng, R = random.Random(heads), heads // kv_heads
     some = 32 // R
     new = [1] * 20 + [0, some, some + 1, 0, 1, some] + [1] * 14
     new[rng.randrange(20)] = 40 * some - sum(new) - 5
     held = [rng.choice((0, 5, 17, 130, 400, 900)) for _ in new]
-    check_paged(zq, heads, kv_heads, dim, vdim, False, page, held, new, wide=(1 << 21) // page)
-    check_paged(zq, heads, kv_heads, dim, vdim, False, page, held, [min(n, some) for n in new], seed=1, wide=(1 << 21) // page)
+    check_paged(zq, heads, kv_heads, dim, vdim, f32, page, held, new, wide=(1 << 21) // page)
+    check_paged(zq, heads, kv_heads, dim, vdim, f32, page, held, [min(n, some) for n in new], seed=1, wide=(1 << 21) // page)
 
 
 @pytest.mark.parametrize("f32", [False, True])

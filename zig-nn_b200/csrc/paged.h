@@ -44,8 +44,9 @@ struct RaggedArgs {
     uint32_t requests, rows, table_ld, shift, pages;
     uint32_t capacity;  // tokens of a request at most
     bool paged;
-    // Tokens of a request up to which the kernel of few rows takes it, when the tensor cores take the others; 0: one form for all.
+    // Tokens of a request up to which the kernel of few rows takes it, when another one takes the others (`rest`); 0: one form for all.
     uint32_t split;
+    bool rest;
     void* work;
 };
 size_t ragged_work_bytes(const RaggedArgs& a, bool f32);

@@ -733,29 +733,39 @@ int allow_shared(K kernel, std::atomic<uint64_t>& devices) {
 
 bool large(const GqaShape& s) { return s.dimp > 256 || s.vdimp > 256; }
 
-// Rows of a tile: 64 (or the tensor cores' tiles) where requests bring more packed rows than some tiles of the small kernel have, on the
-// mean. bf16, requests over 4000 keys, small kernel and tensor cores, us: 64 requests, 32 heads over 8 of 128, 18 packed rows each 71 and 90,
-// 30 rows 107 and 99, 60 rows 132 and 89; four of them 19 and 30, 23 and 30, 41 and 29; 16 requests, 4 over 1 of 256, 18 rows 24 and 37, 60 rows
-// 43 and 38; 12 over 4 of 64, 14 rows 16 and 28, 45 rows 29 and 29. Small work goes there too: the tensor cores' three kernels take 26 us
-// whatever they have to do, the small one's rate is a tenth of theirs (packed, one sequence of 300 tokens, 8 heads over 2 of 128, 0.2
-// GFLOP, 13 and 30; six of up to 300, 12 over 4 of 64, 16 and 29; twenty of up to 200, 32 over 8 of 128, 0.8 GFLOP, 36 and 31; one of 500, 2
-// GFLOP, 43 and 31). f32: two tiles of four rows.
-// (The rows counted are those beyond one of each request: single tokens are the small kernel's.) Up to 32 packed rows on the mean the
-// rows may be single tokens of most requests and a chunk of one: both forms run, and each takes the requests of its kind. Over 4096 keys,
-// 32 heads over 8 of 128, us, small kernel, tensor cores, both: 127 tokens and a chunk of 512 404, 279, 211; 255 and one of 1500 1106, 520,
-// 476; four rows each of 64 requests, nothing for the tensor cores, 74, 114, 84.
+// Which kernels a call takes. The host knows rows, requests and the longest request; times are in us, small kernel and the other one.
+//   * Little work beyond a row of each request: the small kernel. bf16: the tensor cores' three kernels take 26 us whatever they have to
+//     do, the small one's rate is a tenth of theirs (packed, one sequence of 300 tokens, 8 heads over 2 of 128, 0.2 GFLOP, 13 and 30; six of up
+//     to 300, 12 over 4 of 64, 16 and 29; twenty of up to 200, 32 over 8 of 128, 0.8 GFLOP, 36 and 31; one of 500, 2 GFLOP, 43 and 31). f32: a
+//     third of the rate (8 requests over 500 keys, 12 heads over 4 of 64, a chunk of 30 16 and 18; seven sequences of up to 700, 6
+//     heads over 2, 0.25 GFLOP, 344 and 50).
+//   * More than 32 packed rows on the mean (f32: 64): the tensor cores, or the plain kernel. Requests over 4000 keys: 64 of them, 32 heads
+//     over 8 of 128, 18 packed rows each 71 and 90, 30 rows 107 and 99, 60 rows 132 and 89; 16 requests, 4 over 1 of 256, 18 rows 24 and 37, 60 rows
+//     43 and 38; 12 over 4 of 64, 14 rows 16 and 28, 45 rows 29 and 29.
+//   * Between: single tokens of most requests, it may be, and a chunk of one. Both run, each with the requests of its kind, again by 32
+//     packed rows. bf16 over 4096 keys, 32 heads over 8 of 128, small, tensor cores, both: 127 tokens and a chunk of 512 404, 279, 211; 255 and
+//     one of 1500 1106, 520, 476; four rows each of 64 requests, nothing for the tensor cores, 74, 114, 84. f32 over 2000 keys: 63 tokens and a
+//     chunk of 128 460, 741, 362; 124 and four of 300 1725, 1853, 1065; four rows each of 64 requests 237, 512, 264.
 enum class Form { kFew, kTensor, kBoth, kPlain };
 Form form_of(const RaggedArgs& a, bool f32) {
     const uint64_t rows = (uint64_t)a.rows * (a.s.heads / a.s.kv_heads);
     if (large(a.s)) return Form::kPlain;
-    if (f32) return rows <= 2ull * kFewRowsF32 * a.requests ? Form::kFew : Form::kPlain;
     // keys of a row: half of a sequence on the mean; over pages what a table holds is all that the host knows
     const double keys = a.paged ? a.capacity : 0.5 * a.rows / a.requests, more = (double)a.rows - a.requests;
-    if (2.0 * more * a.s.heads * (a.s.dimp + a.s.vdimp) * keys <= 0.6e9) return Form::kFew;
-    if (!ragged_tc_takes(a)) return Form::kPlain;
-    return rows <= 32ull * a.requests ? Form::kBoth : Form::kTensor;
+    if (2.0 * more * a.s.heads * (a.s.dimp + a.s.vdimp) * keys <= (f32 ? 0.1e9 : 0.6e9)) return Form::kFew;
+    if (!f32 && !ragged_tc_takes(a)) return Form::kPlain;
+    return rows <= (f32 ? 64ull : 32ull) * a.requests ? Form::kBoth : f32 ? Form::kPlain : Form::kTensor;
 }
-uint32_t tile_rows(const RaggedArgs& a, Form form, bool f32) { return form != Form::kPlain ? (f32 ? kFewRowsF32 : 16) : large(a.s) ? 16 : 64; }
+// Rows of the tile that the ranges are made for (f32, both: the larger one's, since it has the longer items).
+uint32_t tile_rows(const RaggedArgs& a, Form form, bool f32) {
+    if (f32) return form == Form::kFew ? kFewRowsF32 : large(a.s) ? 16 : 64;
+    return form == Form::kPlain && !large(a.s) ? 64 : 16;
+}
+
+void set_tile(RaggedPlan& p, uint32_t M) {
+    p.tokens = p.R <= M ? M / p.R : 1;
+    p.head_tiles = p.R <= M ? 1 : (p.R + M - 1) / M;
+}
 
 // Ranges of a request's keys. As many as give each of the GPU's workers (a warp, or a CTA of the larger tile) one while the host sees
 // fewer units of work than that, but no more than sqrt(0.4 keys): a range less costs a worker 16 keys (0.5 us), a range more costs the
@@ -764,8 +774,7 @@ uint32_t tile_rows(const RaggedArgs& a, Form form, bool f32) { return form != Fo
 RaggedPlan plan_of(const RaggedArgs& a, uint32_t M, bool f32) {
     RaggedPlan p{};
     p.R = a.s.heads / a.s.kv_heads;
-    p.tokens = p.R <= M ? M / p.R : 1;
-    p.head_tiles = p.R <= M ? 1 : (p.R + M - 1) / M;
+    set_tile(p, M);
     const uint64_t per_tile = a.s.kv_heads * p.head_tiles, some = a.requests < a.rows ? a.requests : a.rows;  // requests with rows at most
     const uint64_t packed = ((uint64_t)a.rows + p.tokens - 1) / p.tokens, least_units = (packed > some ? packed : some) * per_tile;
     const bool wide = a.s.dimp > 128 || a.s.vdimp > 128, narrow = a.s.dimp <= 64 && a.s.vdimp <= 64;
@@ -853,15 +862,19 @@ int launch_ragged_attention(const RaggedArgs& args, bool f32, cudaStream_t st) {
     const Form form = form_of(a, f32);
     if (form == Form::kTensor) return launch_ragged_tc(a, nullptr, st);
     const uint32_t R = a.s.heads / a.s.kv_heads;
-    if (form == Form::kBoth) {
-        a.split = R <= 32 ? 32 / R : 1;
-        a.work = static_cast<char*>(args.work) + ragged_tc_work_bytes(a);
-    }
-    const RaggedCall c{a, plan_of(a, tile_rows(a, form, f32), f32)};
+    const bool tc = form == Form::kBoth && !f32;
+    if (form == Form::kBoth) a.split = R <= 32 ? 32 / R : 1;
+    if (tc) a.work = static_cast<char*>(args.work) + ragged_tc_work_bytes(a);
+    RaggedCall c{a, plan_of(a, tile_rows(a, form, f32), f32)};
     int rc = ZQ_OK;
-    if (form == Form::kBoth) {
+    if (tc) {
         a.work = args.work;
         rc = launch_ragged_tc(a, c.p.max_ranges < 2 ? nullptr : c.p.n_ranges, st);
+    } else if (form == Form::kBoth) {  // the same ranges for both kernels, one join
+        RaggedCall rest = c;
+        rest.a.rest = true;
+        rc = plain_any<float>(rest, st);
+        set_tile(c.p, kFewRowsF32);
     }
     if (rc == ZQ_OK) rc = form != Form::kPlain ? few_any(c, f32, st) : f32 ? plain_any<float>(c, st) : plain_any<bf16>(c, st);
     if (rc != ZQ_OK || c.p.max_ranges < 2) return rc;

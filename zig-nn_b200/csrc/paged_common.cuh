@@ -66,7 +66,7 @@ __device__ __forceinline__ uint32_t count_items(const RaggedArgs& a, const Ragge
     int32_t len = 0;
     if (c + tid < a.requests) {
         span_of(a, c + tid, row0, n_rows, len);
-        if (a.split && n_rows > a.split) n_rows = 0;  // the tensor cores'
+        if (a.split && (n_rows > a.split) != a.rest) n_rows = 0;  // another kernel's
         ranges = ranges_of(len, p.block, p.fill, p.most_keys, per);
         scan = (p.tokens > 1 ? (n_rows + p.tokens - 1) / p.tokens : n_rows) * ranges * a.s.kv_heads * p.head_tiles;
     }
