@@ -1,6 +1,6 @@
 // Causal grouped-query attention of ragged rows over pages of keys and values, or over packed prompts; softmax in f32.
 //   * a few rows of each request: a warp per range of keys, the packed rows as the 16 rows of mma.sync (bf16) or by plain
-//     multiply-adds (f32);
+//     multiply-adds (f32); their tensor work is small beside the keys' bytes, so that mma.sync, which needs no tile of 128 rows, does;
 //   * more rows (bf16): paged_attention_tc.cu;
 //   * more rows (f32), and heads beyond 256 dimensions: tiles of 16 or 64 packed rows against tiles of keys, plain multiply-adds;
 //   * where a request's keys are cut into ranges, the ranges meet in a second small kernel.
@@ -34,8 +34,8 @@ __device__ __forceinline__ void stage4(float* dst, const bf16* src, bool ok) {
 // the scores, values tx * 4 + 64 c ... of the output. S = Q K^T from shared memory, the online softmax in registers (a row's 16
 // threads are half a warp), P through shared memory, O += P V. The next keys travel under the values' product, the values under the
 // scores. What bounds it: the loads from shared memory, eight of 16 bytes for 64 products (of 64 rows; eight rows a thread and half
-// the threads were 5 to 10 % slower). Two products per multiply-add (even
-// and odd dimensions of a score, neighbouring columns of the output), copies whose rows and columns a thread knows from the start.
+// the threads were 5 to 10 % slower): chunks of 512 tokens, 12 heads of 64, 210 us. Two products per multiply-add (even and odd
+// dimensions of a score, neighbouring columns of the output), copies whose rows and columns a thread knows from the start.
 template <typename T, int M, int N, int VC>
 __global__ void __launch_bounds__(256)
 ragged_plain_kernel(const __grid_constant__ RaggedCall call) {
@@ -491,7 +491,8 @@ ragged_few_kernel(const __grid_constant__ RaggedCall call) {
 
 // f32: plain multiply-adds from shared memory, up to four packed rows. Scores: a lane has one of the 16 keys and half of the
 // dimensions, the rows' queries come as broadcasts; values: a lane has four columns (of 64 columns the half-warps take every other
-// key), the weights come as broadcasts.
+// key), the weights come as broadcasts. What bounds it: loads from shared memory and the chain of a step; single tokens of
+// 24 requests of up to 1500 tokens, 12 heads over 4 of 64, 19 us.
 constexpr uint32_t kFewRowsF32 = 4;
 
 template <int D, int STAGES, bool FULL, uint32_t THREADS>
@@ -769,8 +770,9 @@ void set_tile(RaggedPlan& p, uint32_t M) {
 
 // Ranges of a request's keys. As many as give each of the GPU's workers (a warp, or a CTA of the larger tile) one while the host sees
 // fewer units of work than that, but no more than sqrt(0.4 keys): a range less costs a worker 16 keys (0.5 us), a range more costs the
-// join 0.08 us. (The larger tile: eight times as many, since its items differ in what they see.) Beyond that no range longer than 512 keys, so that requests of different lengths share the GPU evenly (one decode step
-// of 64 requests: 256 keys 228 us, 512 214, 1024 224), or as much longer as keeps the sums of the ranges within 2^19 rows.
+// join 0.08 us. (The larger tile: eight times as many, since its items differ in what they see.) Beyond that no range
+// longer than 512 keys, so that requests of different lengths share the GPU evenly (one decode step of 64 requests: 256 keys 228 us,
+// 512 214, 1024 224), or as much longer as keeps the sums of the ranges within 2^19 rows.
 RaggedPlan plan_of(const RaggedArgs& a, uint32_t M, bool f32) {
     RaggedPlan p{};
     p.R = a.s.heads / a.s.kv_heads;
