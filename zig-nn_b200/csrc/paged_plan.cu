@@ -35,7 +35,7 @@ __device__ __forceinline__ int64_t warp_scan(int64_t v, uint32_t lane) {
 // shuffles, one pass through shared memory): that is cheaper than to hand them round. Behind a barrier of the cluster, which ends all
 // reads of what may be overwritten in place, the CTAs share rows and pages; a row, or a page, finds its request by bisection.
 // What bounds it: latency (a load, the sums, a barrier, 6 to 13 steps of bisection, a load of the table, a store): 6.7 us for 256 requests
-// of a token, 12.4 us for 2000 requests and 67 000 rows.
+// of a token, 12.4 us for 2000 requests and 52 000 rows.
 __global__ void __launch_bounds__(kPlanThreads)
 page_plan_kernel(const __grid_constant__ PagePlanArgs a) {
     extern __shared__ __align__(16) int32_t sm[];
@@ -202,7 +202,7 @@ __device__ __forceinline__ void store_four(bf16* o, float4 v) {
 }
 
 // The same where heads are whole groups of four values, up to 128 N of them: N accesses of 16 bytes a lane and head, HEADS heads of a row
-// requested together. What bounds it: the rows' bytes (13 000 rows of 32 and 8 heads of 128, 0.36 GB in 76 us, 4.7 TB/s; two heads a warp 82, eight
+// requested together. What bounds it: the rows' bytes (9700 rows of 32 and 8 heads of 128, 0.36 GB in 76 us, 4.7 TB/s; two heads a warp 82, eight
 // 85, CTAs of 512 threads 91).
 template <typename TA, int N, int HEADS>
 __global__ void __launch_bounds__(128)
