@@ -123,9 +123,9 @@ def test_refusals_of_packed_prompts(library):
     (gqa(12, 4, 64, 64), (100, 16, 64, 1000), 64 * 10, 0, "ragged_few_kernelILi64"),   # 30 packed rows each
     (gqa(12, 4, 64, 64), (100, 16, 64, 1000), 64 * 11, 0, "ragged_tc_kernelILi2ELi1ELi1"),
     (gqa(), (100, 16, 4, 1000), 700, 0, "ragged_tc_kernelILi2ELi2ELi2"),
-    (gqa(8, 2, 96, 128), (100, 16, 4, 1000), 700, 0, "ragged_tc_kernelILi2ELi0ELi0"),
+    (gqa(8, 2, 96, 128), (100, 16, 4, 1000), 700, 0, "ragged_tc_kernelILi2ELi2ELi2"),
     (gqa(8, 2, 256, 256), (100, 16, 4, 1000), 700, 0, "ragged_tc_kernelILi1ELi4ELi4"),
-    (gqa(8, 2, 192, 128), (100, 16, 4, 1000), 700, 0, "ragged_tc_kernelILi1ELi0ELi0"),
+    (gqa(8, 2, 192, 128), (100, 16, 4, 1000), 700, 0, "ragged_tc_kernelILi1ELi3ELi2"),
     (gqa(), (100, 16, 4, 10), 200, 0, "ragged_few_kernelILi128"),                      # little work
     (gqa(), (100, 16, 4, 1000), 700, 1, "ragged_plain_kernelIfLi64"),
     (gqa(8, 2, 512, 512), (100, 16, 4, 1000), 700, 0, "ragged_plain_kernelI13__nv_bfloat16Li16"),

@@ -235,11 +235,18 @@ struct KeyStream {
     uint32_t c, base, end, ahead, key, filled = 0, page = 0;
     Item it;
     bool more = false;
+    // a lane's place in the copies of rows that are no power of two long: its first row and 16 bytes, and what 32 of these are further on
+    struct Lanes {
+        uint32_t r, c, dr, dc;
+        __device__ __forceinline__ explicit Lanes(uint32_t cpr) : r((threadIdx.x & 31) / cpr), c((threadIdx.x & 31) % cpr), dr(32 / cpr), dc(32 % cpr) {}
+    };
+    const Lanes k_lanes, v_lanes;
 
     __device__ __forceinline__ KeyStream(const RaggedCall& call, const Requests<THREADS>& q, uint32_t shared)
         : a(call.a), p(call.p), rq(q), dimp(FULL ? D : a.s.dimp), vdimp(FULL ? D : a.s.vdimp), kpitch(dimp * sizeof(T) + 16),
           vpitch(vdimp * sizeof(T) + 16), k_bytes(16 * kpitch), stage_bytes(16 * (kpitch + vpitch)),
-          ring(shared + (threadIdx.x >> 5) * STAGES * stage_bytes), warps(gridDim.x * (THREADS / 32)) {}
+          ring(shared + (threadIdx.x >> 5) * STAGES * stage_bytes), warps(gridDim.x * (THREADS / 32)),
+          k_lanes(dimp * sizeof(T) / 16), v_lanes(vdimp * sizeof(T) / 16) {}
 
     __device__ __forceinline__ void look_up() {
         if (a.paged) page = (uint32_t)__ldg(a.tables + (size_t)it.request * a.table_ld + (key >> a.shift));
@@ -266,7 +273,8 @@ struct KeyStream {
         advance();
     }
     // 16 rows of one array, 16 bytes a lane and turn; zeros from row `rows` on
-    __device__ __forceinline__ void copy_rows(uint32_t dst, uint32_t pitch, const T* array, size_t ld, size_t row0, uint32_t col, uint32_t dp, uint32_t rows) {
+    __device__ __forceinline__ void copy_rows(uint32_t dst, uint32_t pitch, const T* array, size_t ld, size_t row0, uint32_t col, uint32_t dp, uint32_t rows,
+                                              const Lanes& at) {
         constexpr uint32_t E = 16 / sizeof(T);
         const uint32_t lane = threadIdx.x & 31, cpr = dp / E;
         const T* from = array + row0 * ld + col;
@@ -288,12 +296,17 @@ struct KeyStream {
                     for (uint32_t t = 0; t < TURNS; ++t) copy16(dst + t * 512, r < rows ? from + t * 32 * E : array, r < rows);
             }
         } else {
-            uint32_t r = lane / cpr, c16 = lane % cpr;
-#pragma unroll 1
+            uint32_t r = at.r, c16 = at.c;
+#pragma unroll 4
             for (uint32_t i = 0; i < cpr / 2; ++i) {
                 const bool ok = r < rows;
                 copy16(dst + r * pitch + c16 * 16, ok ? from + r * ld + c16 * E : array, ok);
-                for (c16 += 32; c16 >= cpr; c16 -= cpr) ++r;
+                c16 += at.dc;
+                r += at.dr;
+                if (c16 >= cpr) {
+                    c16 -= cpr;
+                    ++r;
+                }
             }
         }
     }
@@ -305,8 +318,8 @@ struct KeyStream {
             const uint32_t rows = there ? min(16u, it.k_end - key) : 0, g = it.g;
             key += 16;
             if (key < it.k_end) look_up();
-            copy_rows(dst, kpitch, static_cast<const T*>(a.k), a.k_ld, row0, g * dimp, dimp, rows);
-            copy_rows(dst + k_bytes, vpitch, static_cast<const T*>(a.v), a.v_ld, row0, g * vdimp, vdimp, rows);
+            copy_rows(dst, kpitch, static_cast<const T*>(a.k), a.k_ld, row0, g * dimp, dimp, rows, k_lanes);
+            copy_rows(dst + k_bytes, vpitch, static_cast<const T*>(a.v), a.v_ld, row0, g * vdimp, vdimp, rows, v_lanes);
             filled = filled + 1 == STAGES ? 0 : filled + 1;
             if (key >= it.k_end) advance();
         }
@@ -734,12 +747,23 @@ int allow_shared(K kernel, std::atomic<uint64_t>& devices) {
 
 bool large(const GqaShape& s) { return s.dimp > 256 || s.vdimp > 256; }
 
+void set_tile(RaggedPlan& p, uint32_t M) {
+    p.tokens = p.R <= M ? M / p.R : 1;
+    p.head_tiles = p.R <= M ? 1 : (p.R + M - 1) / M;
+}
+
+// Warps of the small kernel (CTAs of the one for large heads) that the GPU runs at once.
+uint64_t few_workers(const RaggedArgs& a, bool f32) {
+    const bool wide = a.s.dimp > 128 || a.s.vdimp > 128, narrow = a.s.dimp <= 64 && a.s.vdimp <= 64;
+    return (uint64_t)sm_count() * (large(a.s) ? 2 : f32 ? (wide ? 3 : narrow ? 8 : 4) : (wide ? 4 : narrow ? 12 : 8));
+}
+
 // Which kernels a call takes. The host knows rows, requests and the longest request; times are in us, small kernel and the other one.
 //   * Little work beyond a row of each request: the small kernel. bf16: the tensor cores' three kernels take 26 us whatever they have to
 //     do, the small one's rate is a tenth of theirs (packed, one sequence of 300 tokens, 8 heads over 2 of 128, 0.2 GFLOP, 13 and 30; six of up
-//     to 300, 12 over 4 of 64, 16 and 29; twenty of up to 200, 32 over 8 of 128, 0.8 GFLOP, 36 and 31; one of 500, 2 GFLOP, 43 and 31). f32: a
-//     third of the rate (8 requests over 500 keys, 12 heads over 4 of 64, a chunk of 30 16 and 18; seven sequences of up to 700, 6
-//     heads over 2, 0.25 GFLOP, 344 and 50).
+//     to 300, 12 over 4 of 64, 16 and 29; twenty of up to 200, 32 over 8 of 128, 0.8 GFLOP, 36 and 31; one of 500, 2 GFLOP, 43 and 31). f32:
+//     four rows an item, so by the items (8 requests over 500 keys, 12 heads over 4 of 64, a chunk of 30 16 and 18, of 80 29 and 20; 63 tokens and
+//     a chunk of 16 over 2000 keys, 32 over 8 of 128, 152 and 218; seven sequences of up to 700, 6 heads over 2, 344 and 50).
 //   * More than 32 packed rows on the mean (f32: 64): the tensor cores, or the plain kernel. Requests over 4000 keys: 64 of them, 32 heads
 //     over 8 of 128, 18 packed rows each 71 and 90, 30 rows 107 and 99, 60 rows 132 and 89; 16 requests, 4 over 1 of 256, 18 rows 24 and 37, 60 rows
 //     43 and 38; 12 over 4 of 64, 14 rows 16 and 28, 45 rows 29 and 29.
@@ -751,9 +775,16 @@ enum class Form { kFew, kTensor, kBoth, kPlain };
 Form form_of(const RaggedArgs& a, bool f32) {
     const uint64_t rows = (uint64_t)a.rows * (a.s.heads / a.s.kv_heads);
     if (large(a.s)) return Form::kPlain;
-    // keys of a row: half of a sequence on the mean; over pages what a table holds is all that the host knows
-    const double keys = a.paged ? a.capacity : 0.5 * a.rows / a.requests, more = (double)a.rows - a.requests;
-    if (2.0 * more * a.s.heads * (a.s.dimp + a.s.vdimp) * keys <= (f32 ? 0.1e9 : 0.6e9)) return Form::kFew;
+    const uint64_t more = a.rows > a.requests ? a.rows - a.requests : 0;
+    if (f32) {  // items of the small kernel beyond a row of each request, and warps that run at once
+        RaggedPlan p{};
+        p.R = a.s.heads / a.s.kv_heads;
+        set_tile(p, kFewRowsF32);
+        if ((more + p.tokens - 1) / p.tokens * a.s.kv_heads * p.head_tiles <= few_workers(a, true) / 4) return Form::kFew;
+    } else {  // keys of a row: half of a sequence on the mean; over pages what a table holds is all that the host knows
+        const double keys = a.paged ? a.capacity : 0.5 * a.rows / a.requests;
+        if (2.0 * more * a.s.heads * (a.s.dimp + a.s.vdimp) * keys <= 0.6e9) return Form::kFew;
+    }
     if (!f32 && !ragged_tc_takes(a)) return Form::kPlain;
     return rows <= (f32 ? 64ull : 32ull) * a.requests ? Form::kBoth : f32 ? Form::kPlain : Form::kTensor;
 }
@@ -761,11 +792,6 @@ Form form_of(const RaggedArgs& a, bool f32) {
 uint32_t tile_rows(const RaggedArgs& a, Form form, bool f32) {
     if (f32) return form == Form::kFew ? kFewRowsF32 : large(a.s) ? 16 : 64;
     return form == Form::kPlain && !large(a.s) ? 64 : 16;
-}
-
-void set_tile(RaggedPlan& p, uint32_t M) {
-    p.tokens = p.R <= M ? M / p.R : 1;
-    p.head_tiles = p.R <= M ? 1 : (p.R + M - 1) / M;
 }
 
 // Ranges of a request's keys. As many as give each of the GPU's workers (a warp, or a CTA of the larger tile) one while the host sees
@@ -779,10 +805,8 @@ RaggedPlan plan_of(const RaggedArgs& a, uint32_t M, bool f32) {
     set_tile(p, M);
     const uint64_t per_tile = a.s.kv_heads * p.head_tiles, some = a.requests < a.rows ? a.requests : a.rows;  // requests with rows at most
     const uint64_t packed = ((uint64_t)a.rows + p.tokens - 1) / p.tokens, least_units = (packed > some ? packed : some) * per_tile;
-    const bool wide = a.s.dimp > 128 || a.s.vdimp > 128, narrow = a.s.dimp <= 64 && a.s.vdimp <= 64;
     p.block = M == 64 ? 64 : 16;  // the steps of the kernels
-    const uint64_t per_sm = M == 64 ? 8 : large(a.s) ? 2 : f32 ? (wide ? 3 : narrow ? 8 : 4) : (wide ? 4 : narrow ? 12 : 8);
-    const uint64_t fill = per_sm * sm_count() / (least_units ? least_units : 1);
+    const uint64_t workers = M == 64 ? 8ull * sm_count() : few_workers(a, f32), fill = workers / (least_units ? least_units : 1);
     p.fill = fill < 1 ? 1 : (uint32_t)fill;
     uint64_t most = 512;
     const uint64_t most_units = (packed + some) * per_tile;

@@ -382,7 +382,7 @@ struct Walk {
     bool whole;
 };
 
-// DK, DV: blocks of 64 dimensions of a key and of a value, full ones; 0: as the parameters say.
+// DK, DV: blocks of 64 dimensions of a key and of a value.
 template <int STREAMS, int DK, int DV>
 __global__ void __launch_bounds__(tc_threads(STREAMS), 1)
 ragged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
@@ -409,9 +409,9 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     auto my_turn = [&](uint32_t i) { return bar32 + 8 * (16 + i); };  // of the issuers
     auto full = [&](uint32_t i) { return bar32 + 8 * (18 + i); };
     auto empty = [&](uint32_t i) { return bar32 + 8 * (18 + kMaxSlots + i); };
-    const uint32_t dk = DK ? DK : p.dk, dv = DV ? DV : p.dv, vk = DV ? (DV <= 2 ? 128 : 64) : p.vk;
-    const uint32_t SLOT = DK && DV ? (DK == 1 && DV == 1 ? 1 : 2) * ATOM : p.slot, kb_slot = SLOT / ATOM;  // blocks of keys in a slot
-    const uint32_t ks = (dk + kb_slot - 1) / kb_slot, vs = TK / vk;                                       // slots of a tile's keys, values
+    constexpr uint32_t dk = DK, dv = DV, vk = DV <= 2 ? 128 : 64;
+    constexpr uint32_t SLOT = (DK == 1 && DV == 1 ? 1 : 2) * ATOM, kb_slot = SLOT / ATOM;  // blocks of keys in a slot
+    constexpr uint32_t ks = (dk + kb_slot - 1) / kb_slot, vs = TK / vk;                                       // slots of a tile's keys, values
     auto slot_at = [&](uint32_t i) { return base + p.slots_at + i * SLOT; };
 
     if (tid == 0) {
@@ -590,7 +590,7 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             const uint64_t q_desc = smem_desc_sw128(base + q * dk * ATOM), k_desc = smem_desc_sw128(slot_at(0)),
                            v_desc = smem_desc_mn_sw128(slot_at(0), vk * 128);
             const uint64_t slot_desc = SLOT >> 4, atom_desc = ATOM >> 4;
-            const uint32_t steps_last = DK ? 4 : s.dimp / 16 - (dk - 1) * 4, o_col = 256 + q * 128;
+            const uint32_t o_col = 256 + q * 128;
             auto after = [&](uint32_t& at, uint32_t& round) {
                 if (++at == p.n_slots) {
                     at = 0;
@@ -619,12 +619,8 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
 #pragma unroll
                     for (uint32_t b = b0; b < b0 + kb_slot; ++b, qd += atom_desc, kd += atom_desc) {
                         if (b >= dk) break;
-                        if (DK || b + 1 < dk || steps_last == 4) {
 #pragma unroll
-                            for (uint32_t k = 0; k < 4; ++k) mma_ss(tm + col, qd + 2 * k, kd + 2 * k, id_s, (b | k) != 0 ? 1u : 0u, lead);
-                        } else {
-                            for (uint32_t k = 0; k < steps_last; ++k) mma_ss(tm + col, qd + 2 * k, kd + 2 * k, id_s, (b | k) != 0 ? 1u : 0u, lead);
-                        }
+                        for (uint32_t k = 0; k < 4; ++k) mma_ss(tm + col, qd + 2 * k, kd + 2 * k, id_s, (b | k) != 0 ? 1u : 0u, lead);
                     }
                     after(at, round);
                 }
@@ -836,8 +832,11 @@ ragged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                     }
                     __syncwarp();
                 }
-                if (real && head == 0)  // columns beyond the heads
-                    for (uint32_t i = s.heads * s.vdim; i < a.out_pitch; ++i) row[i] = __float2bfloat16_rn(0.0f);
+                if (real && head == 0) {  // columns beyond the heads
+                    uint32_t i = s.heads * s.vdim;
+                    for (; i % 8 != 0; ++i) row[i] = __float2bfloat16_rn(0.0f);
+                    for (; i < a.out_pitch; i += 8) *reinterpret_cast<uint4*>(row + i) = make_uint4(0, 0, 0, 0);
+                }
             } else {  // [vdimp + 2][rows]: values, maximum, sum; a tile's first piece goes to the second slot of its part
                 float* part = p.w.partial + (size_t)(2 * c + (w.kb == 0 ? 1 : 0)) * (s.vdimp + 2) * (STREAMS * 128) + tid;
 #pragma unroll 1
@@ -948,6 +947,15 @@ ragged_join_kernel(const __grid_constant__ TcParams p) {
 
 int done(cudaError_t e) { return e == cudaSuccess ? ZQ_OK : cuda_fail(e); }
 
+// Blocks of 64 dimensions that the kernels have, at least as many as the heads: the rest are coordinates outside the tensors, zeros that cost
+// no traffic. (Loops over a head's own number of blocks cost more than the products with zeros: prompts of up to 2458
+// tokens, 24 heads over 8 of 192 and 128, 243 us by these, 198 with three and two.)
+void blocks_of(const GqaShape& s, uint32_t& dk, uint32_t& dv) {
+    if (s.dimp <= 64 && s.vdimp <= 64) dk = dv = 1;
+    else if (s.dimp <= 128 && s.vdimp <= 128) dk = dv = 2;
+    else if (s.dimp <= 192 && s.vdimp <= 128) dk = 3, dv = 2;
+    else dk = dv = 4;
+}
 int streams_of(const GqaShape& s) { return s.dimp <= 128 && s.vdimp <= 128 ? 2 : 1; }
 
 TcParams params_of(const RaggedArgs& a, size_t& bytes) {
@@ -958,8 +966,7 @@ TcParams params_of(const RaggedArgs& a, size_t& bytes) {
     p.R = s.heads / s.kv_heads;
     p.rt = 128 / p.R;
     p.scale2 = a.scale * kLog2e;
-    p.dk = (s.dimp + 63) / 64;
-    p.dv = (s.vdimp + 63) / 64;
+    blocks_of(s, p.dk, p.dv);
     p.slot = (p.dk == 1 && p.dv == 1 ? 1 : 2) * ATOM;
     p.vk = p.dv <= 2 ? 128 : 64;
     const uint32_t page = a.paged ? 1u << a.shift : TK;
@@ -1045,9 +1052,7 @@ int launch_ragged_tc(const RaggedArgs& a, uint32_t* n_ranges, cudaStream_t st) {
     size_t bytes;
     TcParams p = params_of(a, bytes);
     p.n_ranges = n_ranges;
-    const uint32_t d = a.s.dimp == a.s.vdimp ? a.s.dimp : 0;
-    if (streams_of(a.s) == 2) return d == 64 ? launch<2, 1, 1>(p, st) : d == 128 ? launch<2, 2, 2>(p, st) : launch<2, 0, 0>(p, st);
-    return d == 256 ? launch<1, 4, 4>(p, st) : launch<1, 0, 0>(p, st);
+    return p.dk == 1 ? launch<2, 1, 1>(p, st) : p.dk == 2 ? launch<2, 2, 2>(p, st) : p.dk == 3 ? launch<1, 3, 2>(p, st) : launch<1, 4, 4>(p, st);
 }
 
 }  // namespace zq
